@@ -595,6 +595,78 @@ int spot_adamw_f32(float* params, const float* grads, float* exp_avg, float* exp
 long spot_clip_grad_norm_ws_floats(void);
 int spot_clip_grad_norm_f32(float* grads, long n, float max_norm, float* norm_out, float* ws, hipStream_t stream);
 
+/* ---- attention with a learned relative position bias --------------------------- */
+
+/* softmax(scale * q k^T + table[bucket(key - query), head]) v per head, and its gradients.  The reference has no
+ * counterpart: its fusion network adds sine rows to the tokens (ltr/models/neck/transt_fusion.py:142-143,205-206).
+ *
+ * q [B, Lq, H, head_dim], k and v [B, Lk, Hkv, head_dim] of one dtype (0 f32, 1 bf16, 2 f16), H a multiple of Hkv (query
+ * head h reads key/value head h / (H / Hkv)), head_dim 32, 64 or 128; strides in elements, the last dimension dense;
+ * bases and strides are whole numbers of 16 bytes.  out, d_out, dq [B, Lq, H, head_dim] and dk, dv
+ * [B, Lk, Hkv, head_dim] are dense and of that dtype too.
+ *
+ * Positions: key j stands at j, query i of sequence b at offset_b + i, where offset_b is q_offset (q_offset_mode 0),
+ * q_offsets[b] (1) or kv_len[b] - Lq (2: the queries are the last of the keys).  A query whose position is negative or
+ * not below max_len sees no key.
+ * Buckets: the offset delta = key - query of a pair, and on a map of `width` > 0 columns the class
+ * [key % width < query % width], select cells[class][delta + max_len - 1], an entry of 0 .. num_buckets - 1; cells is
+ * int [width > 0 ? 2 : 1][2 max_len - 1].  table [num_buckets, H] of table_dtype.
+ * Hidden keys: j >= kv_len[b] (NULL: none; clamped to 0 .. Lk), bytes of key_padding_mask [B, Lk] that are not zero
+ * (NULL: none), and with causal those behind the query.  What kv_len and the mask hide may hold anything, NaN
+ * included; keys hidden by causal alone have to be finite.  A query without a visible key has output and gradients 0.
+ *
+ * Forward: writes out, and for a backward pass stats [B, H, Lq, 2] floats (NULL: none) and out_lo (NULL: none; the
+ * rounding error of a 16-bit out, from which the backward takes rowsum(out * d_out) to 32-bit precision).
+ * Backward: reads what the forward read and wrote, and d_out; writes dq, dk and dv (both NULL: not wanted) and dtable
+ * (table_dtype, [num_buckets, H]; NULL: not wanted).  cell_order int [cells]: the cells sorted by bucket; cell_start
+ * int [num_buckets + 1]: where each bucket's begin in it.  ws: spot_bias_attention_bwd_ws_bytes bytes, 16-byte aligned.
+ * No atomics between workgroups: the same inputs give the same bits. */
+#define SPOT_BIAS_ATTN_MAX_LEN 1048576
+typedef struct spot_bias_attn_desc {
+    const void *q, *k, *v;
+    void *out, *out_lo;
+    float* stats;
+    const void* table;
+    const int *cells, *q_offsets, *kv_len;
+    const unsigned char* key_padding_mask;
+    const void* d_out;
+    void *dq, *dk, *dv, *dtable;
+    const int *cell_order, *cell_start;
+    void* ws;
+    long ws_bytes;
+    long q_stride_b, q_stride_l, q_stride_h, k_stride_b, k_stride_l, k_stride_h, v_stride_b, v_stride_l, v_stride_h;
+    int dtype, table_dtype, B, Lq, Lk, H, Hkv, head_dim;
+    int num_buckets, max_len, width, causal, q_offset_mode, q_offset;
+    float scale;
+} spot_bias_attn_desc;
+int spot_bias_attention_fwd(const spot_bias_attn_desc* desc /* host */, hipStream_t stream);
+int spot_bias_attention_bwd_ws_bytes(const spot_bias_attn_desc* desc /* host */, long* bytes /* host */);
+int spot_bias_attention_bwd(const spot_bias_attn_desc* desc /* host */, hipStream_t stream);
+
+/* ---- top logits and distillation ----------------------------------------------- */
+
+/* The k largest of each row of logits [N, V] (dtype 0 f32, 1 bf16, 2 f16; rows ld elements apart), largest first, with
+ * their places; among equal values the lowest place is taken and stands first, -0 equals 0, and a NaN is above every
+ * number.  values [N, k] of the same dtype, indices [N, k].  ws: spot_top_logits_ws_bytes bytes, 16-byte aligned. */
+#define SPOT_TOP_LOGITS_MAX_K 128
+#define SPOT_TOP_LOGITS_MAX_V 1048576
+int spot_top_logits_ws_bytes(int dtype, int N, int V, int k, long* bytes /* host */);
+int spot_top_logits(int dtype, const void* logits, long ld, int N, int V, int k, void* values, int* indices, void* ws,
+                    long ws_bytes, hipStream_t stream);
+
+/* T^2 KL(p || q) per row: p = softmax(values / T) over the row's k listed entries, q = softmax(student / T) over all V.
+ * The soft counterpart of the one pseudo-label per clip (ltr/actor/transt_sparse_actor.py:57-98).  Entries with an
+ * index outside of 0 .. V - 1 or the value -inf are absent; a row without any has loss and gradient 0.  An index that
+ * is listed twice counts twice.  student [N, V] of dtype, rows ld elements apart; values [N, k] of values_dtype (0 f32,
+ * 1 bf16, 2 f16), indices [N, k].
+ * Forward: loss [N], and for the backward norm [N, 2] and p [N, k].  ws: spot_top_distill_ws_bytes bytes, 16-byte
+ * aligned.  Backward: d_student [N, V] dense, of the student's dtype, from d_loss [N]. */
+int spot_top_distill_ws_bytes(int dtype, int N, int V, int k, long* bytes /* host */);
+int spot_top_distill_fwd(int dtype, const void* student, long ld, int values_dtype, const void* values, const int* indices, int N,
+                         int V, int k, float temperature, float* loss, float* norm, float* p, void* ws, long ws_bytes, hipStream_t stream);
+int spot_top_distill_bwd(int dtype, const void* student, long ld, const int* indices, const float* norm, const float* p,
+                         const float* d_loss, int N, int V, int k, float temperature, void* d_student, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,483 @@
+// The k largest entries of a row with their places, and the distillation loss of a student row against them.
+//
+// Both are bound by reading the rows once (the loss's gradient: reading and writing them once): N * V elements against
+// 5 to 10 lane operations each, which is under the vector rate at the card's copy bandwidth.
+#include <float.h>
+
+#include "common.h"
+#include "../../include/spot_hip.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int NT = 256;              // threads of a workgroup
+constexpr int KMAX = SPOT_TOP_LOGITS_MAX_K;
+enum { F32 = 0, BF16 = 1, F16 = 2 };
+
+template <class T> struct Vec16 {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T v __attribute__((ext_vector_type(16 / sizeof(T))));
+};
+
+// Elements [j VE - skew, j VE - skew + VE) of a row piece of n elements, where `skew` elements lie between the last
+// 16-byte border and the piece: one 16-byte load inside the piece, single elements at its ends, `fill` outside of it.
+template <class T> __device__ __forceinline__ typename Vec16<T>::v load_vec(const T* x, int n, int e0, T fill) {
+    constexpr int VE = Vec16<T>::N;
+    if (e0 >= 0 && e0 + VE <= n) return *reinterpret_cast<const typename Vec16<T>::v*>(x + e0);
+    typename Vec16<T>::v r;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) r[i] = (unsigned)(e0 + i) < (unsigned)n ? x[e0 + i] : fill;
+    return r;
+}
+template <class T> __device__ __forceinline__ int skew_of(const T* x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+
+// Whole number that orders as the value does: -0 and +0 are one value, a NaN is above everything.
+template <class T> __device__ __forceinline__ int order_key(T x) {
+    const float f = (float)x + 0.f;
+    const int b = __float_as_int(f), t = b ^ ((b >> 31) & 0x7fffffff);
+    return f != f ? 0x7fffffff : t;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// One workgroup takes a piece of a row, held in registers.
+//   1. The k-th largest of the 256 threads' maxima is a bound that at least k elements reach, and few more do: for
+//      values in random places about 256 ln(256 / (256 - k)), 74 for k = 64.
+//   2. What reaches it goes to a list in LDS; an element's rank is how many of the list stand before it (greater, or
+//      equal at a lower place), and the first k are written at their rank.
+//   3. Only if the list overflows (many equal values) the k-th value is found by bisection over the keys, and among
+//      its equals the last place by bisection over the places.
+// Rows too long for one workgroup, or too few to fill the card, are cut in pieces; a second launch of the same kernel
+// takes the pieces' candidates, whose order is that of the places among equals.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int LIST = 1024;
+
+__device__ __forceinline__ int block_sum(int v, int* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+template <class T, int NV>
+__global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ x, long ld, int V, int pieces, int k,
+                                                 const int* __restrict__ places, T* __restrict__ values, int* __restrict__ indices) {
+    constexpr int VE = Vec16<T>::N;
+    __shared__ __attribute__((aligned(16))) int s_max[NT];
+    __shared__ int s_key[LIST], s_at[LIST];
+    __shared__ int s_count, s_bound, red[4];
+    const long row = blockIdx.x / pieces;
+    const int piece = blockIdx.x % pieces;
+    const int begin = (int)((long)V * piece / pieces), n = (int)((long)V * (piece + 1) / pieces) - begin;
+    const T* xr = x + row * ld + begin;
+    const int skew = skew_of(xr);
+
+    typename Vec16<T>::v r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r[i] = load_vec(xr, n, (i * NT + (int)threadIdx.x) * VE - skew, (T)0.f);
+    int top = (int)0x80000000;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const int e = (i * NT + threadIdx.x) * VE - skew + j;
+            if ((unsigned)e < (unsigned)n) top = max(top, order_key(r[i][j]));
+        }
+    s_max[threadIdx.x] = top;
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < NT; i += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(s_max + i);
+        rank += (o.x > top || (o.x == top && i < (int)threadIdx.x)) + (o.y > top || (o.y == top && i + 1 < (int)threadIdx.x)) +
+                (o.z > top || (o.z == top && i + 2 < (int)threadIdx.x)) + (o.w > top || (o.w == top && i + 3 < (int)threadIdx.x));
+    }
+    if (rank == k - 1) s_bound = top;
+    __syncthreads();
+    int bound = s_bound;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const int e = (i * NT + threadIdx.x) * VE - skew + j, key = order_key(r[i][j]);
+            if ((unsigned)e < (unsigned)n && key >= bound) {
+                const int at = atomicAdd(&s_count, 1);
+                if (at < LIST) {
+                    s_key[at] = key;
+                    s_at[at] = e;
+                }
+            }
+        }
+    __syncthreads();
+    int count = s_count;
+    if (count > LIST) {
+        // the largest key that k elements reach: bound reaches it, lo holds that invariant
+        auto reach = [&](long key) {
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    const int e = (i * NT + threadIdx.x) * VE - skew + j;
+                    c += (unsigned)e < (unsigned)n && order_key(r[i][j]) >= key;
+                }
+            return block_sum(c, red);
+        };
+        long lo = bound, hi = 0x80000000L;              // reach(lo) >= k > reach(hi)
+        while (hi - lo > 1) {
+            const long mid = (lo + hi) >> 1;
+            if (reach(mid) >= k) lo = mid; else hi = mid;
+        }
+        const int kth = (int)lo, left = k - reach(hi);  // how many of those equal to the k-th are taken
+        int first = -1, last = n - 1;                   // of them, up to `last` at least `left`, up to `first` fewer
+        while (last - first > 1) {
+            const int mid = (first + last) >> 1;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    const int e = (i * NT + threadIdx.x) * VE - skew + j;
+                    c += (unsigned)e <= (unsigned)mid && e < n && order_key(r[i][j]) == kth;
+                }
+            if (block_sum(c, red) >= left) last = mid; else first = mid;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s_count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const int e = (i * NT + threadIdx.x) * VE - skew + j, key = order_key(r[i][j]);
+                if ((unsigned)e < (unsigned)n && (key > kth || (key == kth && e <= last))) {
+                    const int at = atomicAdd(&s_count, 1);
+                    s_key[at] = key;
+                    s_at[at] = e;
+                }
+            }
+        __syncthreads();
+        count = s_count;
+    }
+    const long out = (long)blockIdx.x * k;
+    for (int c = threadIdx.x; c < count; c += NT) {
+        const int key = s_key[c], at = s_at[c];
+        int before = 0;
+        for (int i = 0; i < count; ++i) before += s_key[i] > key || (s_key[i] == key && s_at[i] < at);
+        if (before < k) {
+            values[out + before] = xr[at];
+            indices[out + before] = places ? places[row * V + at] : begin + at;
+        }
+    }
+}
+
+template <class T> constexpr int capacity(int nv) { return (nv * NT - 1) * Vec16<T>::N; }   // whatever the skew is
+
+// Pieces per row: what the registers of a workgroup hold at most, and about 512 workgroups where the rows are few (two
+// per CU), but no piece under 4096 elements, where a workgroup's fixed work is longer than its loads.
+template <class T> int top_pieces(int N, int V, int k) {
+    const long most = capacity<T>(16);
+    long pieces = (V + most - 1) / most;
+    const long fill = (512 + N - 1) / N, floor_ = V / 4096;
+    if (fill > pieces) pieces = fill < floor_ ? fill : (floor_ > pieces ? floor_ : pieces);
+    while (pieces > 1 && pieces * k > most) --pieces;
+    return (int)pieces;
+}
+
+template <class T>
+int top_launch(const T* x, long ld, int N, int V, int pieces, int k, const int* places, T* values, int* indices, hipStream_t stream) {
+    const int n = (V + pieces - 1) / pieces;
+    const unsigned grid = (unsigned)N * pieces;
+    if (n <= capacity<T>(1)) top_kernel<T, 1><<<grid, NT, 0, stream>>>(x, ld, V, pieces, k, places, values, indices);
+    else if (n <= capacity<T>(4)) top_kernel<T, 4><<<grid, NT, 0, stream>>>(x, ld, V, pieces, k, places, values, indices);
+    else top_kernel<T, 16><<<grid, NT, 0, stream>>>(x, ld, V, pieces, k, places, values, indices);
+    SPOT_CHECK_LAUNCH("spot_top_logits");
+    return SPOT_OK;
+}
+
+int top_pieces_of(int dtype, int N, int V, int k) { return dtype == F32 ? top_pieces<float>(N, V, k) : top_pieces<_Float16>(N, V, k); }
+
+template <class T>
+int top_run(const void* x, long ld, int N, int V, int k, void* values, int* indices, void* ws, hipStream_t stream) {
+    const int pieces = top_pieces<T>(N, V, k);
+    if (pieces == 1) return top_launch<T>(static_cast<const T*>(x), ld, N, V, 1, k, nullptr, static_cast<T*>(values), indices, stream);
+    const long found = (long)N * pieces * k;
+    T* wv = static_cast<T*>(ws);
+    int* wi = reinterpret_cast<int*>(static_cast<char*>(ws) + ((found * sizeof(T) + 15) & ~15L));
+    if (const int rc = top_launch<T>(static_cast<const T*>(x), ld, N, V, pieces, k, nullptr, wv, wi, stream)) return rc;
+    return top_launch<T>(wv, (long)pieces * k, N, pieces * k, 1, k, wi, static_cast<T*>(values), indices, stream);
+}
+
+int check_rows(const char* name, int dtype, int N, int V, int k, long ld) {
+    SPOT_CHECK_ARG(dtype >= F32 && dtype <= F16, "%s: dtype %d is none of 0 (f32), 1 (bf16), 2 (f16)", name, dtype);
+    SPOT_CHECK_ARG(N >= 0 && V >= 1 && V <= SPOT_TOP_LOGITS_MAX_V && ld >= V, "%s: %d rows of %d logits (1 to %d), %ld apart", name, N, V,
+                   SPOT_TOP_LOGITS_MAX_V, ld);
+    SPOT_CHECK_ARG(k >= 1 && k <= KMAX, "%s: k = %d is not in 1 .. %d", name, k, KMAX);
+    SPOT_CHECK_ARG((long)N * ((V + 2047) / 2048) < (1L << 31), "%s: %d rows of %d logits need too many workgroups", name, N, V);
+    return SPOT_OK;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Distillation.  With p = softmax(t / T) over the row's present entries and q = softmax(s / T) over the whole row
+//   loss = T^2 sum_i p_i (log p_i - log q[c_i]),   d loss / d s_c = T (q_c - sum_{i: c_i = c} p_i).
+// Exponents are taken against one reference per row, mc = log2 e / T * max s, as fma(s, log2 e / T, -mc): whatever
+// mc was rounded to, it is the same number in the sum, in q and in log q.
+// ---------------------------------------------------------------------------------------------------------------------
+struct Norm { float m, l; };          // sum of exp2(x - m) is l; m = -inf: nothing yet
+__device__ __forceinline__ Norm join(Norm a, Norm b) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return {m, a.l + b.l};
+    return {m, a.l * __builtin_amdgcn_exp2f(a.m - m) + b.l * __builtin_amdgcn_exp2f(b.m - m)};
+}
+__device__ __forceinline__ Norm block_join(Norm v, Norm* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = join(v, Norm{__shfl_xor(v.m, o), __shfl_xor(v.l, o)});
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = join(join(red[0], red[1]), join(red[2], red[3]));
+    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ float block_add(float v, float* red) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+    __syncthreads();
+    return v;
+}
+
+struct Distill {
+    const void *student, *values;
+    const int* indices;
+    long ld;
+    int N, V, k, pieces, values_type;
+    float c, T;                       // c = log2 e / T
+    float *loss, *norm, *p;           // norm [N, 2]: mc, 1 / sum (0 for a row without entries); p [N, k]
+    Norm* ws;
+    const float* d_loss;
+    void* d_student;
+};
+
+// (mc, l) over a piece of a row
+template <class T> __device__ __forceinline__ Norm row_norm(const T* x, int n, float c) {
+    constexpr int VE = Vec16<T>::N;
+    const int skew = skew_of(x), nv = (n + skew + VE - 1) / VE;
+    float top = -INFINITY;
+    Norm r = {0.f, 0.f};
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += NT) {
+        const typename Vec16<T>::v v = load_vec(x, n, i * VE - skew, (T)-INFINITY);
+        float m = top;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) m = fmaxf(m, (float)v[j]);
+        if (m > top) {
+            r.l *= __builtin_amdgcn_exp2f(fminf(r.m - m * c, 0.f));     // the first reference is no power to scale by
+            r.m = m * c;
+            top = m;
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) r.l += __builtin_amdgcn_exp2f(fmaf((float)v[j], c, -r.m));
+    }
+    if (top == -INFINITY) r.m = -INFINITY;
+    return r;
+}
+
+__device__ __forceinline__ float teacher_at(const Distill& a, long i) {
+    return a.values_type == F32 ? static_cast<const float*>(a.values)[i]
+         : a.values_type == BF16 ? (float)static_cast<const __bf16*>(a.values)[i] : (float)static_cast<const _Float16*>(a.values)[i];
+}
+
+// the loss of one row from its (mc, l), by the whole workgroup
+template <class T> __device__ void row_loss(const Distill& a, long row, Norm z, Norm* red_n, float* red_f) {
+    const T* x = static_cast<const T*>(a.student) + row * a.ld;
+    const int i = threadIdx.x;
+    float t = -INFINITY;
+    int at = -1;
+    if (i < a.k) {
+        at = a.indices[row * a.k + i];
+        if ((unsigned)at < (unsigned)a.V) t = teacher_at(a, row * a.k + i) * a.c;
+    }
+    const Norm tn = block_join(Norm{t, t == -INFINITY ? 0.f : 1.f}, red_n);
+    const bool none = tn.m == -INFINITY;
+    const float logl = __builtin_amdgcn_logf(z.l), logt = __builtin_amdgcn_logf(tn.l);
+    float p = 0.f, term = 0.f;
+    if (t != -INFINITY) {
+        p = __builtin_amdgcn_exp2f(t - tn.m) / tn.l;
+        const float lq = fmaf((float)x[at], a.c, -z.m) - logl;
+        if (p != 0.f) term = p * ((t - tn.m - logt) - lq);
+    }
+    if (i < a.k) a.p[row * a.k + i] = p;
+    const float sum = block_add(term, red_f);
+    if (i == 0) {
+        a.loss[row] = none ? 0.f : a.T * a.T * LN2 * sum;
+        a.norm[2 * row] = z.m;
+        a.norm[2 * row + 1] = none ? 0.f : 1.f / z.l;
+    }
+}
+
+template <class T> __global__ __launch_bounds__(NT) void distill_fwd_kernel(const Distill a) {
+    __shared__ Norm red_n[4];
+    __shared__ float red_f[4];
+    const long row = blockIdx.x / a.pieces;
+    const int piece = blockIdx.x % a.pieces;
+    const int begin = (int)((long)a.V * piece / a.pieces), n = (int)((long)a.V * (piece + 1) / a.pieces) - begin;
+    const Norm z = block_join(row_norm(static_cast<const T*>(a.student) + row * a.ld + begin, n, a.c), red_n);
+    if (a.pieces == 1) row_loss<T>(a, row, z, red_n, red_f);
+    else if (threadIdx.x == 0) a.ws[blockIdx.x] = z;
+}
+template <class T> __global__ __launch_bounds__(NT) void distill_join_kernel(const Distill a) {
+    __shared__ Norm red_n[4];
+    __shared__ float red_f[4];
+    const long row = blockIdx.x;
+    Norm z = {-INFINITY, 0.f};
+    for (int i = threadIdx.x; i < a.pieces; i += NT) z = join(z, a.ws[row * a.pieces + i]);
+    row_loss<T>(a, row, block_join(z, red_n), red_n, red_f);
+}
+
+// One workgroup per piece of a row: q for the whole piece, then the few taken places again with their p.  A place that
+// is listed more than once is written by its first listing, with the sum over all of them.
+template <class T> __global__ __launch_bounds__(NT) void distill_bwd_kernel(const Distill a) {
+    constexpr int VE = Vec16<T>::N;
+    __shared__ float s_p[KMAX];
+    __shared__ int s_at[KMAX];
+    const long row = blockIdx.x / a.pieces;
+    const int piece = blockIdx.x % a.pieces;
+    const int begin = (int)((long)a.V * piece / a.pieces), n = (int)((long)a.V * (piece + 1) / a.pieces) - begin;
+    const T* x = static_cast<const T*>(a.student) + row * a.ld + begin;
+    T* dx = static_cast<T*>(a.d_student) + row * a.V + begin;
+    const float mc = a.norm[2 * row], inv = a.norm[2 * row + 1], g = a.T * a.d_loss[row];
+    const bool none = inv == 0.f;
+    for (int i = threadIdx.x; i < a.k; i += NT) {
+        s_p[i] = a.p[row * a.k + i];
+        s_at[i] = a.indices[row * a.k + i];
+    }
+    const float f = g * inv;
+    const int skew = skew_of(dx), nv = (n + skew + VE - 1) / VE;
+    const bool same = skew_of(x) == skew;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += NT) {
+        const int e0 = i * VE - skew;
+        typename Vec16<T>::v v, o;
+        if (same) v = load_vec(x, n, e0, (T)0.f);
+        else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[j] = (unsigned)(e0 + j) < (unsigned)n ? x[e0 + j] : (T)0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) o[j] = none ? (T)0.f : (T)(f * __builtin_amdgcn_exp2f(fmaf((float)v[j], a.c, -mc)));
+        if (e0 >= 0 && e0 + VE <= n) *reinterpret_cast<typename Vec16<T>::v*>(dx + e0) = o;
+        else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if ((unsigned)(e0 + j) < (unsigned)n) dx[e0 + j] = o[j];
+        }
+    }
+    // the stores above have to be in memory before another wave writes some of the same places
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (none) return;
+    for (int i = threadIdx.x; i < a.k; i += NT) {
+        const int at = s_at[i] - begin;
+        if ((unsigned)at >= (unsigned)n) continue;
+        float p = 0.f;
+        bool first = true;
+        for (int j = 0; j < a.k; ++j)
+            if (s_at[j] - begin == at) {
+                p += s_p[j];
+                first = first && j >= i;
+            }
+        if (first) dx[at] = (T)(g * (inv * __builtin_amdgcn_exp2f(fmaf((float)x[at], a.c, -mc)) - p));
+    }
+}
+
+// Pieces per row: about 1024 workgroups where the rows are few, no piece under 4096 elements.
+int distill_pieces(int N, int V) {
+    const long fill = (1024 + N - 1) / N, most = V / 4096;
+    const long pieces = fill < most ? fill : most;
+    return pieces < 1 ? 1 : (int)pieces;
+}
+
+template <class T> int distill_fwd(Distill& a, hipStream_t stream) {
+    distill_fwd_kernel<T><<<(unsigned)a.N * a.pieces, NT, 0, stream>>>(a);
+    SPOT_CHECK_LAUNCH("spot_top_distill_fwd");
+    if (a.pieces > 1) {
+        distill_join_kernel<T><<<a.N, NT, 0, stream>>>(a);
+        SPOT_CHECK_LAUNCH("spot_top_distill_fwd");
+    }
+    return SPOT_OK;
+}
+template <class T> int distill_bwd(Distill& a, hipStream_t stream) {
+    distill_bwd_kernel<T><<<(unsigned)a.N * a.pieces, NT, 0, stream>>>(a);
+    SPOT_CHECK_LAUNCH("spot_top_distill_bwd");
+    return SPOT_OK;
+}
+
+}  // namespace
+
+extern "C" int spot_top_logits_ws_bytes(int dtype, int N, int V, int k, long* bytes) {
+    if (const int rc = check_rows("spot_top_logits", dtype, N, V, k, V)) return rc;
+    SPOT_CHECK_ARG(bytes != nullptr && k <= V, "spot_top_logits: k = %d of %d logits", k, V);
+    const long pieces = N ? top_pieces_of(dtype, N, V, k) : 1, found = N * pieces * k;
+    *bytes = pieces > 1 ? ((found * (dtype == F32 ? 4 : 2) + 15) & ~15L) + found * 4 : 0;
+    return SPOT_OK;
+}
+
+extern "C" int spot_top_logits(int dtype, const void* logits, long ld, int N, int V, int k, void* values, int* indices, void* ws,
+                               long ws_bytes, hipStream_t stream) {
+    if (const int rc = check_rows("spot_top_logits", dtype, N, V, k, ld)) return rc;
+    SPOT_CHECK_ARG(k <= V, "spot_top_logits: k = %d of %d logits", k, V);
+    if (N == 0) return SPOT_OK;
+    SPOT_CHECK_ARG(logits && values && indices, "spot_top_logits: null pointer");
+    long need = 0;
+    if (const int rc = spot_top_logits_ws_bytes(dtype, N, V, k, &need)) return rc;
+    SPOT_CHECK_ARG(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need),
+                   "spot_top_logits: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", need, ws_bytes);
+    if (dtype == F32) return top_run<float>(logits, ld, N, V, k, values, indices, ws, stream);
+    if (dtype == BF16) return top_run<__bf16>(logits, ld, N, V, k, values, indices, ws, stream);
+    return top_run<_Float16>(logits, ld, N, V, k, values, indices, ws, stream);
+}
+
+extern "C" int spot_top_distill_ws_bytes(int dtype, int N, int V, int k, long* bytes) {
+    if (const int rc = check_rows("spot_top_distill", dtype, N, V, k, V)) return rc;
+    SPOT_CHECK_ARG(bytes != nullptr, "spot_top_distill: null pointer");
+    const long pieces = N ? distill_pieces(N, V) : 1;
+    *bytes = pieces > 1 ? (long)N * pieces * (long)sizeof(Norm) : 0;
+    return SPOT_OK;
+}
+
+extern "C" int spot_top_distill_fwd(int dtype, const void* student, long ld, int values_dtype, const void* values,
+                                    const int* indices, int N, int V, int k, float temperature, float* loss, float* norm, float* p, void* ws, long ws_bytes,
+                                    hipStream_t stream) {
+    if (const int rc = check_rows("spot_top_distill_fwd", dtype, N, V, k, ld)) return rc;
+    SPOT_CHECK_ARG(values_dtype >= F32 && values_dtype <= F16, "spot_top_distill_fwd: values_dtype %d is none of 0 (f32), 1 (bf16), 2 (f16)",
+                   values_dtype);
+    SPOT_CHECK_ARG(temperature > 0.f && temperature <= FLT_MAX, "spot_top_distill_fwd: temperature %g", temperature);
+    if (N == 0) return SPOT_OK;
+    SPOT_CHECK_ARG(student && values && indices && loss && norm && p, "spot_top_distill_fwd: null pointer");
+    Distill a = {};
+    a.student = student; a.values = values; a.indices = indices; a.ld = ld; a.N = N; a.V = V; a.k = k;
+    a.pieces = distill_pieces(N, V);
+    a.values_type = values_dtype;
+    a.T = temperature; a.c = LOG2E / temperature; a.loss = loss; a.norm = norm; a.p = p;
+    a.ws = static_cast<Norm*>(ws);
+    const long need = a.pieces > 1 ? (long)N * a.pieces * (long)sizeof(Norm) : 0;
+    SPOT_CHECK_ARG(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need),
+                   "spot_top_distill_fwd: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", need, ws_bytes);
+    return dtype == F32 ? distill_fwd<float>(a, stream) : dtype == BF16 ? distill_fwd<__bf16>(a, stream) : distill_fwd<_Float16>(a, stream);
+}
+
+extern "C" int spot_top_distill_bwd(int dtype, const void* student, long ld, const int* indices, const float* norm, const float* p,
+                                    const float* d_loss, int N, int V, int k, float temperature, void* d_student, hipStream_t stream) {
+    if (const int rc = check_rows("spot_top_distill_bwd", dtype, N, V, k, ld)) return rc;
+    SPOT_CHECK_ARG(temperature > 0.f && temperature <= FLT_MAX, "spot_top_distill_bwd: temperature %g", temperature);
+    if (N == 0) return SPOT_OK;
+    SPOT_CHECK_ARG(student && indices && norm && p && d_loss && d_student, "spot_top_distill_bwd: null pointer");
+    Distill a = {};
+    a.student = student; a.indices = indices; a.ld = ld; a.N = N; a.V = V; a.k = k;
+    a.pieces = distill_pieces(N, V);
+    a.T = temperature; a.c = LOG2E / temperature; a.d_loss = d_loss; a.d_student = d_student;
+    a.norm = const_cast<float*>(norm); a.p = const_cast<float*>(p);
+    return dtype == F32 ? distill_bwd<float>(a, stream) : dtype == BF16 ? distill_bwd<__bf16>(a, stream) : distill_bwd<_Float16>(a, stream);
+}

@@ -56,6 +56,16 @@ class WinogradOpts(C.Structure):
                 ("bn_var", vp), ("bn_eps", f32), ("relu", i32), ("in_bn", C.POINTER(BnTrainIn))]
 
 
+class BiasAttnDesc(C.Structure):
+    """Mirror of ``spot_bias_attn_desc``."""
+    _fields_ = ([(n, vp) for n in ("q", "k", "v", "out", "out_lo", "stats", "table", "cells", "q_offsets", "kv_len",
+                                   "key_padding_mask", "d_out", "dq", "dk", "dv", "dtable", "cell_order", "cell_start", "ws")] +
+                [(n, i64) for n in ("ws_bytes", "q_stride_b", "q_stride_l", "q_stride_h", "k_stride_b", "k_stride_l", "k_stride_h",
+                                    "v_stride_b", "v_stride_l", "v_stride_h")] +
+                [(n, i32) for n in ("dtype", "table_dtype", "B", "Lq", "Lk", "H", "Hkv", "head_dim", "num_buckets", "max_len",
+                                    "width", "causal", "q_offset_mode", "q_offset")] + [("scale", f32)])
+
+
 # name -> argument ctypes (all return int unless noted); the trailing hipStream_t is a void*
 SIGNATURES = {
     "spot_preprocess_u8_f32": [vp, vp, C.POINTER(f32), C.POINTER(f32), vp, i32, i32, i32, i32, vp],
@@ -121,6 +131,14 @@ SIGNATURES = {
     "spot_dropout_f32": [vp, vp, i64, i32, f32, C.c_uint, vp],
     "spot_layernorm_fwd_f32": [vp, vp, vp, vp, vp, vp, i64, i32, f32, vp],
     "spot_batchnorm_stats_f32": [vp, vp, i32, i32, i32, vp],
+    "spot_bias_attention_fwd": [C.POINTER(BiasAttnDesc), vp],
+    "spot_bias_attention_bwd_ws_bytes": [C.POINTER(BiasAttnDesc), C.POINTER(i64)],
+    "spot_bias_attention_bwd": [C.POINTER(BiasAttnDesc), vp],
+    "spot_top_logits_ws_bytes": [i32] * 4 + [C.POINTER(i64)],
+    "spot_top_logits": [i32, vp, i64, i32, i32, i32, vp, vp, vp, i64, vp],
+    "spot_top_distill_ws_bytes": [i32] * 4 + [C.POINTER(i64)],
+    "spot_top_distill_fwd": [i32, vp, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, vp, i64, vp],
+    "spot_top_distill_bwd": [i32, vp, i64, vp, vp, vp, vp, i32, i32, i32, f32, vp, vp],
     "spot_layernorm_bwd_f32": [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, f32, C.c_uint, vp],
 }
 

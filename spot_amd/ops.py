@@ -1962,3 +1962,345 @@ def mha_block(xq, xkv, pos_q, pos_k, in_w, in_b, out_w, out_b, kpm, add_residual
     """bf16=True takes the attention core's matrix products in bf16 (fp32 softmax and accumulation)."""
     return MHAFn.apply(xq, xkv, pos_q, pos_k, in_w, in_b, out_w, out_b, kpm, add_residual, nhead, self_attn,
                        p_attn, p_out, bf16)
+
+
+# ---------------------------------------------------------------------------
+# attention with a learned relative position bias by buckets
+# ---------------------------------------------------------------------------
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class RelativeBuckets:
+    """Which bucket each relative position of a key to a query has: what bias_attention looks a bias up by.
+
+    ``cells[delta + max_len - 1]`` is the bucket of a key ``delta`` places behind the query (delta < 0: before it), for
+    sequences of up to ``max_len`` positions.  On a map of ``width`` columns (positions row by row) ``cells`` has two
+    rows: the first for keys whose column is not left of the query's, the second for those left of it, so that an entry
+    stands for one (row offset, column offset).  Build it once per model: it also holds, for the gradient, the cells
+    sorted by bucket."""
+
+    def __init__(self, cells, num_buckets, width=0, device="cuda"):
+        cells = torch.as_tensor(cells, dtype=torch.int64, device="cpu")
+        cells = cells.reshape(1, -1) if cells.dim() == 1 else cells
+        if cells.dim() != 2 or cells.shape[0] != (2 if width else 1) or cells.shape[1] % 2 != 1:
+            raise RuntimeError("spot_amd: bucket cells of shape %s: [2 max_len - 1], or with a width [2, 2 max_len - 1]"
+                               % (tuple(cells.shape),))
+        if width < 0 or num_buckets < 1 or int(cells.min()) < 0 or int(cells.max()) >= num_buckets:
+            raise RuntimeError("spot_amd: width %d, bucket cells from %d to %d for %d buckets"
+                               % (width, int(cells.min()), int(cells.max()), num_buckets))
+        self.num_buckets, self.width, self.max_len = int(num_buckets), int(width), (cells.shape[1] + 1) // 2
+        flat = cells.reshape(-1)
+        start = torch.zeros(num_buckets + 1, dtype=torch.int64)
+        start[1:] = torch.bincount(flat, minlength=num_buckets).cumsum(0)
+        self.cells = cells.to(torch.int32).to(device)
+        self.order = torch.argsort(flat, stable=True).to(torch.int32).to(device)
+        self.start = start.to(torch.int32).to(device)
+
+
+def sequence_buckets(max_len, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+    """Buckets of a sequence: one per offset up to half of them, then borders that grow geometrically up to
+    ``max_distance``, from where on all offsets share the last.  ``bidirectional``: one half of the buckets for keys at
+    or before the query, the other for those behind it; otherwise keys behind the query share bucket 0.  The borders
+    come from whole numbers: an offset on one has the same bucket everywhere."""
+    buckets = num_buckets // 2 if bidirectional else num_buckets
+    near = buckets // 2
+    logs = buckets - near
+    if max_len < 1 or near < 1 or max_distance <= near:
+        raise RuntimeError("spot_amd: sequence_buckets of %d positions, %d buckets, max_distance %d"
+                           % (max_len, num_buckets, max_distance))
+    # offset n belongs to logarithmic bucket j when (n / near)^logs >= (max_distance / near)^j
+    borders, n = [], near
+    for j in range(1, logs):
+        while n ** logs * near ** j < max_distance ** j * near ** logs:
+            n += 1
+        borders.append(n)
+    d = torch.arange(max_len)
+    before = torch.where(d < near, d, near + torch.bucketize(d, torch.tensor(borders, dtype=torch.int64), right=True))
+    behind = before + buckets if bidirectional else torch.zeros_like(before)
+    return RelativeBuckets(torch.cat([before.flip(0), behind[1:]]), num_buckets, 0, device)
+
+
+def grid_buckets(height, width, device="cuda"):
+    """Buckets of a map of height x width tokens, row by row: one per (row offset, column offset),
+    (dy + height - 1) * (2 width - 1) + dx + width - 1."""
+    if height < 1 or width < 1:
+        raise RuntimeError("spot_amd: grid_buckets of a %d x %d map" % (height, width))
+    n = height * width
+    delta = torch.arange(1 - n, n)
+    dx = torch.stack([delta % width, delta % width - width])
+    dy = torch.div(delta - dx, width, rounding_mode="floor")
+    # offsets that no pair of the map has: any bucket
+    dx, dy = dx.clamp(1 - width, width - 1), dy.clamp(1 - height, height - 1)
+    return RelativeBuckets((dy + height - 1) * (2 * width - 1) + dx + width - 1, (2 * height - 1) * (2 * width - 1), width, device)
+
+
+class _on:
+    """Makes a tensor's device the current one for the launches inside the block."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t):
+        i = t.device.index
+        here = _current_device() if _current_device is not None else torch.cuda.current_device()
+        self.guard = torch.cuda.device(i) if i != here else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _aligned16(t):
+    """t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes, else a copy."""
+    es = t.element_size()
+    if t.data_ptr() % 16 == 0 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])) \
+            and (t.shape[-1] == 1 or t.stride(-1) == 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _dense16(t):
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_bias_attention(q, k, v, table, buckets, q_offset, kv_len, key_padding_mask):
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (table, "table")):
+        if not t.is_cuda:
+            raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
+        if t.device != q.device:
+            raise RuntimeError("spot_amd: %s is on %s, q on %s" % (name, t.device, q.device))
+        if t.dtype not in _DTYPE_CODE or (name != "table" and t.dtype != q.dtype):
+            raise RuntimeError("spot_amd: %s is %s: q, k and v have one dtype of float32, bfloat16, float16, the table one of these"
+                               % (name, t.dtype))
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError("spot_amd: q %s, k %s, v %s: [B, Lq, H, D] and twice [B, Lk, Hkv, D]"
+                           % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if D not in (32, 64, 128):
+        raise RuntimeError("spot_amd: bias_attention is built for heads of 32, 64 or 128 channels, not %d" % D)
+    if Hkv == 0 or H == 0 or H % Hkv:
+        raise RuntimeError("spot_amd: %d query heads over %d key/value heads" % (H, Hkv))
+    if tuple(table.shape) != (buckets.num_buckets, H):
+        raise RuntimeError("spot_amd: table %s for %d buckets and %d heads" % (tuple(table.shape), buckets.num_buckets, H))
+    if buckets.cells.device != q.device:
+        raise RuntimeError("spot_amd: buckets are on %s, q on %s" % (buckets.cells.device, q.device))
+    if Lk > buckets.max_len:
+        raise RuntimeError("spot_amd: %d keys, but the buckets end at %d positions" % (Lk, buckets.max_len))
+    if torch.is_tensor(q_offset):
+        _check_per_sequence(q_offset, B, q, "q_offset")
+    elif q_offset != "end":
+        if isinstance(q_offset, str) or int(q_offset) != q_offset or q_offset < 0 or q_offset + Lq > buckets.max_len:
+            raise RuntimeError("spot_amd: q_offset %r for %d queries and buckets of %d positions (a number, \"end\" or int32 [B])"
+                               % (q_offset, Lq, buckets.max_len))
+    if kv_len is not None:
+        _check_per_sequence(kv_len, B, q, "kv_len")
+    if key_padding_mask is not None:
+        m = key_padding_mask
+        if m.device != q.device or m.dtype not in (torch.bool, torch.uint8) or tuple(m.shape) != (B, Lk):
+            raise RuntimeError("spot_amd: key_padding_mask must be bool or uint8 [%d, %d] on %s, got %s %s on %s"
+                               % (B, Lk, q.device, m.dtype, tuple(m.shape), m.device))
+
+
+def _check_per_sequence(t, B, q, name):
+    if not torch.is_tensor(t) or t.device != q.device or t.dtype != torch.int32 or tuple(t.shape) != (B,):
+        raise RuntimeError("spot_amd: %s must be an int32 tensor [%d] on %s" % (name, B, q.device))
+
+
+def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, train):
+    """-> out, out_lo, stats, and the descriptor with the tensors whose addresses it holds."""
+    q, k, v = _aligned16(q), _aligned16(k), _aligned16(v)
+    table = table if table.is_contiguous() else table.contiguous()
+    off_t = q_offset.contiguous() if torch.is_tensor(q_offset) else None
+    kv_len = kv_len.contiguous() if kv_len is not None else None
+    kpm = key_padding_mask.contiguous() if key_padding_mask is not None else None
+    B, Lq, H, D = q.shape
+    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    out_lo = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device) if train else None
+    ptr = lambda t: None if t is None else t.data_ptr()
+    d = lib.BiasAttnDesc(
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(out_lo), ptr(stats), ptr(table), ptr(buckets.cells), ptr(off_t), ptr(kv_len), ptr(kpm),
+        None, None, None, None, None, ptr(buckets.order), ptr(buckets.start), None, 0,
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        _DTYPE_CODE[q.dtype], _DTYPE_CODE[table.dtype], B, Lq, k.shape[1], H, k.shape[2], D, buckets.num_buckets, buckets.max_len,
+        buckets.width, int(bool(causal)), 1 if off_t is not None else 2 if q_offset == "end" else 0,
+        0 if off_t is not None or q_offset == "end" else int(q_offset), 1.0 / math.sqrt(D) if scale is None else float(scale))
+    # strides of dimensions of length one say nothing
+    if B == 1:
+        d.q_stride_b = d.k_stride_b = d.v_stride_b = 0
+    if Lq == 1:
+        d.q_stride_l = 0
+    if k.shape[1] == 1:
+        d.k_stride_l = d.v_stride_l = 0
+    if H == 1:
+        d.q_stride_h = 0
+    if k.shape[2] == 1:
+        d.k_stride_h = d.v_stride_h = 0
+    lib.keep(q, k, v, out, out_lo, stats, table, buckets.cells, off_t, kv_len, kpm)
+    with _on(q):
+        lib.call("spot_bias_attention_fwd", C.byref(d), _st())
+    return out, out_lo, stats, d, (q, k, v, table, off_t, kv_len, kpm)
+
+
+class BiasAttentionFn(_Fn):
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale):
+        train = _wants(ctx)
+        out, out_lo, stats, d, held = _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, train)
+        if train:
+            ctx.save_for_backward(*held, out, out_lo, stats)
+            ctx.desc, ctx.buckets = d, buckets
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, off_t, kv_len, kpm, out, out_lo, stats = ctx.saved_tensors
+        dout = _dense16(dout)
+        dev = q.device
+        d = lib.BiasAttnDesc.from_buffer_copy(ctx.desc)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2)) if any(ctx.needs_input_grad[1:3]) else (None, None)
+        dtable = torch.empty(table.shape, dtype=table.dtype, device=dev) if ctx.needs_input_grad[3] else None
+        for name, t in (("q", q), ("k", k), ("v", v), ("table", table), ("out", out), ("out_lo", out_lo), ("stats", stats),
+                        ("q_offsets", off_t), ("kv_len", kv_len), ("key_padding_mask", kpm), ("d_out", dout), ("dq", dq), ("dk", dk),
+                        ("dv", dv), ("dtable", dtable)):
+            setattr(d, name, None if t is None else t.data_ptr())
+        with _on(q):
+            need = C.c_long(0)
+            lib.call("spot_bias_attention_bwd_ws_bytes", C.byref(d), C.byref(need))
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
+            d.ws, d.ws_bytes = ws.data_ptr(), need.value
+            lib.call("spot_bias_attention_bwd", C.byref(d), _st())
+        grads = [g if w else None for g, w in zip((dq, dk, dv, dtable), ctx.needs_input_grad)]
+        return (*grads, None, None, None, None, None, None)
+
+
+def bias_attention(q, k, v, table, buckets, causal=False, q_offset=0, kv_len=None, key_padding_mask=None, scale=None):
+    """softmax(scale * q k^T + bias) v with a learned bias ``table[bucket, head]`` by relative position, differentiable in
+    q, k, v and table.
+
+    q [B, Lq, H, D], k and v [B, Lk, Hkv, D], all float32, bfloat16 or float16; H a multiple of Hkv (query head h reads
+    key/value head h // (H // Hkv)), D 32, 64 or 128; any strides (inputs that are not 16-byte aligned are copied).
+    table [buckets.num_buckets, H] in one of these types; buckets a RelativeBuckets (sequence_buckets, grid_buckets).
+    scale: 1 / sqrt(D) if None.
+
+    Keys stand at positions 0 .. Lk - 1, the queries of a sequence at q_offset + 0 .. Lq - 1: a number for all sequences,
+    an int32 tensor [B], or "end" - the last Lq of a sequence's keys, as when new tokens attend to a cache that holds
+    them already.  A query before position 0, or behind buckets.max_len, sees no key.
+    Hidden are keys from kv_len[b] (int32 [B]) on, keys whose key_padding_mask [B, Lk] (bool or uint8) is set, and with
+    ``causal`` keys behind the query.  What kv_len and the mask hide may hold anything; keys that only ``causal`` hides
+    have to be finite.  A bias of -inf hides a key, too; the type's lowest value does not: a row of nothing else is
+    averaged.  A query that sees no key has output 0 and gradients 0.
+
+    Scores, probabilities, sums and the table's gradient are 32 bits or more; products of 16-bit inputs take
+    probabilities and score gradients rounded to that type.  Deterministic.  Capturable into a graph: the tensors
+    kv_len and q_offset are read when it is replayed.  Not twice differentiable."""
+    _check_bias_attention(q, k, v, table, buckets, q_offset, kv_len, key_padding_mask)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+        return BiasAttentionFn.apply(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale)
+    return _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, False)[0]
+
+
+# ---------------------------------------------------------------------------
+# the teacher's top logits, and distillation from them
+# ---------------------------------------------------------------------------
+def _logit_rows(x, name):
+    """[..., V] as rows [N, V] with a dense last dimension, and their distance in elements (a view where one exists)."""
+    if not x.is_cuda:
+        raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
+    if x.dtype not in _DTYPE_CODE:
+        raise RuntimeError("spot_amd: %s must be float32, bfloat16 or float16, got %s" % (name, x.dtype))
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError("spot_amd: %s of shape %s has no logits" % (name, tuple(x.shape)))
+    V = x.shape[-1]
+    x2 = x.reshape(-1, V) if x.numel() else x.new_empty((0, V))
+    if V > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < V:
+        x2 = x2.contiguous()
+    return x2, max(x2.stride(0), V) if x2.shape[0] > 1 else V
+
+
+def _ws(query, device, *args):
+    need = C.c_long(0)
+    lib.call(query, *args, C.byref(need))
+    return (torch.empty((need.value,), dtype=torch.uint8, device=device) if need.value else None), need.value
+
+
+def top_logits(logits, k):
+    """(values, indices) of the k largest of each row of logits [..., V] (float32, bfloat16, float16; V up to 2^20, k up
+    to 128), largest first; of equal values those with the lowest indices, in their order.  A NaN counts as larger than
+    every number.  values [..., k] has the logits' type, indices [..., k] is int32.  No gradient flows through it: it is
+    the teacher's side of top_logit_distillation."""
+    x, ld = _logit_rows(logits.detach(), "logits")
+    N, V = x.shape
+    if not 1 <= k <= min(V, 128):
+        raise RuntimeError("spot_amd: top_logits takes 1 to %d of %d logits, not %r" % (min(V, 128), V, k))
+    shape = tuple(logits.shape[:-1]) + (int(k),)
+    values = torch.empty(shape, dtype=x.dtype, device=x.device)
+    indices = torch.empty(shape, dtype=torch.int32, device=x.device)
+    if N:
+        with _on(x):
+            ws, n = _ws("spot_top_logits_ws_bytes", x.device, _DTYPE_CODE[x.dtype], N, V, int(k))
+            lib.call("spot_top_logits", _DTYPE_CODE[x.dtype], _p(x), ld, N, V, int(k), _p(values), _p(indices), _p(ws), n, _st())
+    return values, indices
+
+
+class TopLogitDistillationFn(_Fn):
+    @staticmethod
+    def forward(ctx, student, values, indices, T):
+        x, ld = _logit_rows(student, "student")
+        N, V = x.shape
+        k = values.shape[-1]
+        f = lambda *s: torch.empty(s, dtype=torch.float32, device=x.device)
+        loss, norm, p = f(*student.shape[:-1]), f(N, 2), f(N, k)
+        if N:
+            with _on(x):
+                code = _DTYPE_CODE[x.dtype]
+                ws, n = _ws("spot_top_distill_ws_bytes", x.device, code, N, V, k)
+                lib.call("spot_top_distill_fwd", code, _p(x), ld, _DTYPE_CODE[values.dtype], _p(values), _p(indices), N, V, k, T,
+                         _p(loss), _p(norm), _p(p), _p(ws), n, _st())
+        if _wants(ctx):
+            ctx.save_for_backward(x, indices, norm, p)
+            ctx.dims = (tuple(student.shape), ld, T)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, indices, norm, p = ctx.saved_tensors
+        shape, ld, T = ctx.dims
+        N, V = x.shape
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+        if N:
+            dloss = dloss.to(torch.float32).contiguous()
+            with _on(x):
+                lib.call("spot_top_distill_bwd", _DTYPE_CODE[x.dtype], _p(x), ld, _p(indices), _p(norm), _p(p), _p(dloss), N, V,
+                         p.shape[1], T, _p(dx), _st())
+        return dx, None, None, None
+
+
+def top_logit_distillation(student, values, indices, temperature=1.0):
+    """Per row T^2 KL(p || q): p = softmax(values / T) over the teacher's k listed logits, q = softmax(student / T) over
+    the student's whole row; differentiable in student (in values not).
+
+    student [..., V] in float32, bfloat16 or float16; values [..., k] in any of these and indices [..., k] int32, as
+    top_logits gives them (k up to 128).  An entry whose index is outside of 0 .. V - 1 (-1: rows with fewer entries) or
+    whose value is -inf is absent; a row without entries has loss 0 and gradient 0.  An index listed twice counts twice.
+    -> float32 [...]."""
+    if not (student.is_cuda and values.is_cuda and indices.is_cuda and values.device == indices.device == student.device):
+        raise RuntimeError("spot_amd: student, values and indices must live on one GPU (no CPU path exists)")
+    if values.dtype not in _DTYPE_CODE or indices.dtype != torch.int32:
+        raise RuntimeError("spot_amd: values must be float32, bfloat16 or float16 and indices int32, got %s and %s"
+                           % (values.dtype, indices.dtype))
+    if student.dim() == 0 or values.shape != indices.shape or values.dim() != student.dim() or values.shape[:-1] != student.shape[:-1]:
+        raise RuntimeError("spot_amd: student %s, values %s, indices %s: [..., V] and twice [..., k]"
+                           % (tuple(student.shape), tuple(values.shape), tuple(indices.shape)))
+    if not 1 <= values.shape[-1] <= 128:
+        raise RuntimeError("spot_amd: top_logit_distillation takes 1 to 128 entries per row, not %d" % values.shape[-1])
+    T = float(temperature)
+    if not 0.0 < T < math.inf:
+        raise RuntimeError("spot_amd: temperature %r" % (temperature,))
+    return TopLogitDistillationFn.apply(student, values.detach().contiguous(), indices.contiguous(), T)

@@ -1,0 +1,108 @@
+"""Host side of the biased attention and the top-logit operators: bucket plans and what the library refuses (no GPU)."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def test_sequence_buckets():
+    from spot_amd import ops
+    b = ops.sequence_buckets(300, 32, 128, device="cpu")
+    cells = b.cells[0].tolist()
+    at = lambda d: cells[d + 299]
+    assert [at(-n) for n in range(8)] == list(range(8)) and [at(n) for n in range(1, 8)] == [16 + n for n in range(1, 8)]
+    # half 16 buckets, 8 of them exact; the others double every two: 8, 11.3, 16, 22.6, 32, 45.3, 64, 90.5
+    for n, bucket in ((8, 8), (11, 8), (12, 9), (15, 9), (16, 10), (22, 10), (23, 11), (31, 11), (32, 12), (45, 12), (46, 13), (63, 13),
+                      (64, 14), (90, 14), (91, 15), (128, 15), (299, 15)):
+        assert at(-n) == bucket and at(n) == 16 + bucket, n
+    one = ops.sequence_buckets(300, 32, 128, bidirectional=False, device="cpu")
+    cells = one.cells[0].tolist()
+    assert set(cells[300:]) == {0} and cells[299 - 15] == 15 and cells[299 - 16] == 16 and cells[0] == 31
+    assert ops.sequence_buckets(1, 4, 8, device="cpu").cells.shape == (1, 1)
+
+
+@pytest.mark.parametrize("h,w", [(1, 1), (1, 6), (6, 1), (4, 5), (7, 3)])
+def test_grid_buckets(h, w):
+    from spot_amd import ops
+    b = ops.grid_buckets(h, w, device="cpu")
+    n = h * w
+    assert b.max_len == n and b.width == w and b.num_buckets == (2 * h - 1) * (2 * w - 1)
+    for q in range(n):
+        for k in range(n):
+            dy, dx = k // w - q // w, k % w - q % w
+            assert b.cells[int(dx < 0), k - q + n - 1] == (dy + h - 1) * (2 * w - 1) + dx + w - 1
+    flat = b.cells.reshape(-1)
+    assert torch.equal(flat[b.order.long()], flat.sort().values)
+    for i in range(b.num_buckets):
+        assert (flat[b.order[b.start[i]:b.start[i + 1]].long()] == i).all()
+    assert b.start[-1] == flat.numel()
+
+
+def test_bucket_plans_refuse():
+    from spot_amd import ops
+    for cells, nb, width in (([0, 1], 2, 0), ([0, 2, 1], 2, 0), ([0, -1, 1], 2, 0), ([0, 1, 0], 2, 3), ([[0, 1, 0]], 2, 3),
+                             ([[0, 1, 0]] * 2, 2, 0), ([0], 0, 0), ([[[0]]], 1, 0)):
+        with pytest.raises(RuntimeError, match="spot_amd"):
+            ops.RelativeBuckets(cells, nb, width, device="cpu")
+    for args in ((0, 32, 128), (10, 2, 128), (10, 32, 8), (10, 0, 128)):
+        with pytest.raises(RuntimeError, match="spot_amd"):
+            ops.sequence_buckets(*args, device="cpu")
+    for args in ((0, 4), (4, 0)):
+        with pytest.raises(RuntimeError, match="spot_amd"):
+            ops.grid_buckets(*args, device="cpu")
+
+
+def _desc(**kw):
+    from spot_amd import lib
+    d = lib.BiasAttnDesc(B=2, Lq=8, Lk=16, H=4, Hkv=2, head_dim=32, num_buckets=4, max_len=32, scale=1.0)
+    for n in ("q", "k", "v", "out", "table", "cells", "d_out", "dq", "dk", "dv", "stats"):
+        setattr(d, n, 4096)
+    for n in "qkv":
+        setattr(d, n + "_stride_l", 128)
+    for n, x in kw.items():
+        setattr(d, n, x)
+    return d
+
+
+@pytest.mark.parametrize("field,value", [
+    ("dtype", 3), ("dtype", -1), ("table_dtype", 5), ("head_dim", 48), ("Hkv", 3), ("Hkv", 0), ("B", -1), ("Lk", 33), ("max_len", 0),
+    ("max_len", (1 << 20) + 1), ("num_buckets", 0), ("width", -1), ("q_offset", -1), ("q_offset", 25), ("q_offset_mode", 1),
+    ("q_offset_mode", 3), ("q", None), ("k", None), ("out", None), ("table", None), ("cells", None), ("q", 4100), ("v", 4104),
+    ("q_stride_l", 130), ("k_stride_b", 2), ("v_stride_h", 1), ("Lq", (1 << 20) + 1)])
+def test_forward_refuses_bad_descriptors(field, value):
+    from spot_amd import lib
+    l = lib.load()
+    rc = l.spot_bias_attention_fwd(C.byref(_desc(**{field: value})), None)
+    assert rc < 0 and b"spot_bias_attention" in l.spot_last_error()
+
+
+def test_backward_refuses():
+    from spot_amd import lib
+    l = lib.load()
+    n = C.c_long(-1)
+    assert l.spot_bias_attention_bwd_ws_bytes(C.byref(_desc()), C.byref(n)) == 0 and n.value == 4 * 2 * 4 * 8
+    for kw in ({"stats": None}, {"d_out": None}, {"dq": None}, {"dk": None}, {"dtable": 4096}, {"d_out": 4100}, {}, {"ws": 4096, "ws_bytes": 255},
+               {"ws": 4100, "ws_bytes": 256}):
+        rc = l.spot_bias_attention_bwd(C.byref(_desc(**kw)), None)
+        assert rc < 0 and b"spot_bias_attention" in l.spot_last_error(), kw
+    assert l.spot_bias_attention_fwd(None, None) < 0 and l.spot_bias_attention_bwd(None, None) < 0
+    assert l.spot_bias_attention_fwd(C.byref(_desc(B=0)), None) == 0
+
+
+def test_rows_refuse():
+    from spot_amd import lib
+    l = lib.load()
+    n = C.c_long(-1)
+    assert l.spot_top_logits_ws_bytes(0, 4, 1000, 8, C.byref(n)) == 0 and n.value == 0
+    assert l.spot_top_logits_ws_bytes(2, 3, 100003, 8, C.byref(n)) == 0 and n.value > 0
+    p = 4096
+    for a in ((3, p, 10, 1, 10, 2, p, p), (0, p, 9, 1, 10, 2, p, p), (0, p, 10, -1, 10, 2, p, p), (0, p, 10, 1, 10, 0, p, p),
+              (0, p, 10, 1, 10, 11, p, p), (0, p, 200, 1, 200, 129, p, p), (0, p, 1 << 21, 1, 1 << 21, 2, p, p), (0, None, 10, 1, 10, 2, p, p),
+              (0, p, 10, 1, 10, 2, None, p), (0, p, 10, 1, 10, 2, p, None), (2, p, 100003, 3, 100003, 8, p, p)):
+        assert l.spot_top_logits(*a, None, 0, None) < 0 and b"spot_top_logits" in l.spot_last_error(), a
+    for a in ((3, p, 10, 0, p, p, 1, 10, 2, 1.0), (0, p, 10, 4, p, p, 1, 10, 2, 1.0), (0, p, 10, 0, p, p, 1, 10, 2, 0.0),
+              (0, p, 10, 0, p, p, 1, 10, 2, float("nan")), (0, p, 10, 0, None, p, 1, 10, 2, 1.0), (0, p, 10, 0, p, p, 1, 10, 129, 1.0),
+              (0, p, 100003, 0, p, p, 3, 100003, 2, 1.0)):
+        assert l.spot_top_distill_fwd(*a, p, p, p, None, 0, None) < 0 and b"spot_top_distill" in l.spot_last_error(), a
+    assert l.spot_top_distill_bwd(0, p, 10, None, p, p, p, 1, 10, 2, 1.0, p, None) < 0
+    assert l.spot_top_logits(0, None, 10, 0, 10, 2, None, None, None, 0, None) == 0

@@ -1,0 +1,447 @@
+"""Attention with a relative position bias against its definition in 64 bits, with bounds that follow the arithmetic."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from spot_amd import lib, ops as _ops
+    lib.load()
+    return _ops
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def reference(q, k, v, table, cells, width, max_len, causal, off, kv_len, kpm, scale, g=None):
+    """float64 outputs and, for each, how far a kernel may be off: inputs are exact, products accumulate in 32 bits,
+    probabilities, score gradients and results are rounded once to the inputs' type."""
+    T = q.dtype
+    u = half_step(T)
+    u_op = 0.0 if T == torch.float32 else u                  # rounding of an operand made on the way
+    # a half float below 2^-14 has steps of 2^-24; probabilities are rounded 2^12 up
+    a_p, a_ds = (2.0 ** -37, 2.0 ** -25) if T == torch.float16 else (0.0, 0.0)
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    G = H // Hkv
+    dev = q.device
+    live = torch.arange(Lk, device=dev)[None] < kv_len.long()[:, None]
+    if kpm is not None:
+        live = live & ~kpm.bool()
+    Q = q.double().permute(0, 2, 1, 3)
+    K = k.double().masked_fill(~live[:, :, None, None], 0).permute(0, 2, 1, 3).repeat_interleave(G, 1)
+    V = v.double().masked_fill(~live[:, :, None, None], 0).permute(0, 2, 1, 3).repeat_interleave(G, 1)
+    p = off.long()[:, None, None] + torch.arange(Lq, device=dev)[None, :, None]
+    j = torch.arange(Lk, device=dev)[None, None]
+    seen = live[:, None] & (p >= 0) & (p < max_len)
+    if causal:
+        seen = seen & (j <= p)
+    delta = (j - p).clamp(1 - max_len, max_len - 1)
+    cls = (j % width < p % width).long() if width else torch.zeros_like(delta)
+    bucket = cells.long().reshape(-1, 2 * max_len - 1)[cls, delta + max_len - 1]
+    bias = table.double()[bucket].permute(0, 3, 1, 2)
+    raw = Q @ K.transpose(2, 3) * scale
+    S = (raw + bias).masked_fill(~seen[:, None], -math.inf)
+    top = S.amax(3, keepdim=True) if Lk else S.new_full((B, H, Lq, 1), -math.inf)
+    none = top == -math.inf
+    E = (S - top.masked_fill(none, 0)).exp().masked_fill(~seen[:, None] | none, 0)
+    Z = E.sum(3, keepdim=True)
+    P = E / Z.masked_fill(Z == 0, 1)
+    O = P @ V
+    # a score: D + 1 roundings of the product, one each of scale and log2 e in c, of the bias, of the sum; relative to
+    # the largest of the row once more for the reference; then v_exp_f32 (one unit) and the sum of Lk terms
+    size = Q.abs() @ K.abs().transpose(2, 3) * abs(scale)       # a size: of either sign of scale
+    finite = torch.where(seen[:, None] & torch.isfinite(S), bias.abs() + raw.abs(), 0.0)
+    es = U32 * ((D + 4) * size + 4 * finite)
+    es = es + es.amax(3, keepdim=True) if Lk else es
+    ep = 2 * es + (Lk + 8) * U32
+    aV = V.abs()
+    tol_o = (P * (ep + u_op) + a_p) @ aV + (Lk + 4) * U32 * (P @ aV) + u * O.abs()
+    back = lambda x: x.permute(0, 2, 1, 3)
+    if g is None:
+        return back(O), back(tol_o)
+    Gr = g.double().permute(0, 2, 1, 3)
+    dP = Gr @ V.transpose(2, 3)
+    dl = (Gr * O).sum(3, keepdim=True)
+    dS = P * (dP - dl)
+    gv, go = Gr.abs() @ aV.transpose(2, 3), (Gr.abs() * (O.abs() + tol_o)).sum(3, keepdim=True)
+    # the row sum takes the kernel's own output (its error counts) rounded to the type and its remainder, rounded again
+    e_dl = (Gr.abs() * tol_o).sum(3, keepdim=True) if u_op == 0 else \
+        (Gr.abs() * ((P * (ep + u_op) + a_p) @ aV + (Lk + 4) * U32 * (P @ aV))).sum(3, keepdim=True)
+    e_dl = e_dl + (D * U32 + 2 * u_op * u_op) * go
+    e_dS = P * ep * (dP - dl).abs() + P * ((D + 2) * U32 * gv + e_dl + 2 * U32 * (dP.abs() + dl.abs()))
+    e_op = e_dS + u_op * dS.abs() + a_ds                            # as an operand of the next product
+    aK, aQ, aG = K.abs(), Q.abs(), Gr.abs()
+    share = lambda x: x.view(B, Hkv, G, Lk, D).sum(2).permute(0, 2, 1, 3)
+    n_q = (Lq * G + 4) * U32
+    dQ, tQ = scale * dS @ K, abs(scale) * (e_op + (Lk + 4) * U32 * dS.abs()) @ aK
+    dK, tK = share(scale * dS.transpose(2, 3) @ Q), share(abs(scale) * (e_op + n_q * dS.abs()).transpose(2, 3) @ aQ)
+    dV, tV = share(P.transpose(2, 3) @ Gr), share((P * (ep + u_op + n_q) + a_p).transpose(2, 3) @ aG)
+    nb = table.shape[0]
+    by = lambda x: torch.zeros((nb, H), dtype=torch.float64, device=dev).index_add_(
+        0, bucket.expand(B, Lq, Lk).reshape(-1), x.permute(0, 2, 3, 1).reshape(-1, H))
+    dT, tT = by(dS), by(e_dS + 2 * 128 * U32 * dS.abs())
+    out = [(back(O), back(tol_o))] + [(x, t + u * x.abs()) for x, t in ((back(dQ), back(tQ)), (dK, tK), (dV, tV))]
+    return out + [(dT, tT + half_step(table.dtype) * dT.abs())]
+
+
+def inside(got, want, tol, what):
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), what
+    over = (got.double() - want).abs() - tol - 1e-30
+    # subnormal results of a 16-bit type are rounded to its smallest step
+    over = over - (torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps)
+    assert over.max().item() <= 0 if over.numel() else True, "%s: %.3g over, of %.3g" % (what, over.max().item(), want.abs().max().item())
+
+
+def run_case(ops, t, B, Lq, Lk, H, Hkv, D, width=0, causal=False, q_offset=0, kv_len=None, masked=False, table_t=None, scale=None,
+             train=True, spread=1.0, seed=0, buckets=None, max_len=None):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    T = TYPES[t]
+    rnd = lambda *s: (torch.randn(*s, generator=gen, device=DEV) * spread).to(T)
+    q, k, v, g = rnd(B, Lq, H, D), rnd(B, Lk, Hkv, D), rnd(B, Lk, Hkv, D), rnd(B, Lq, H, D)
+    if buckets is None:
+        if width:
+            buckets = ops.grid_buckets(-(-(max_len or max(Lq, Lk)) // width), width, device=DEV)
+        else:
+            buckets = ops.sequence_buckets(max_len or max(Lq, Lk, 1), 16, 64, bidirectional=not causal, device=DEV)
+    table = torch.randn(buckets.num_buckets, H, generator=gen, device=DEV).to(TYPES[table_t] if table_t else T)
+    lens = torch.tensor(kv_len if kv_len is not None else [Lk] * B, dtype=torch.int32, device=DEV)
+    kpm = None
+    if masked:
+        kpm = torch.rand(B, Lk, generator=gen, device=DEV) < 0.4
+        kpm[0] = True                                           # a whole sequence without keys
+    off = lens - Lq if q_offset == "end" else torch.tensor(q_offset if isinstance(q_offset, list) else [q_offset] * B, device=DEV)
+    # what is hidden by length or mask holds anything
+    hidden = torch.arange(Lk, device=DEV)[None] >= lens.long()[:, None].clamp(max=Lk)
+    if kpm is not None:
+        hidden = hidden | kpm
+    k, v = k.masked_fill(hidden[:, :, None, None], math.nan), v.masked_fill(hidden[:, :, None, None], math.inf)
+    leaves = [x.requires_grad_(train) for x in (q, k, v, table)]
+    arg = torch.tensor(q_offset, dtype=torch.int32, device=DEV) if isinstance(q_offset, list) else q_offset
+    out = ops.bias_attention(*leaves, buckets, causal=causal, q_offset=arg, kv_len=lens if kv_len is not None else None,
+                             key_padding_mask=kpm, scale=scale)
+    assert out.dtype == T and out.shape == (B, Lq, H, D)
+    sc = 1 / math.sqrt(D) if scale is None else scale
+    with torch.no_grad():
+        want = reference(q, k, v, table, buckets.cells, width, buckets.max_len, causal, off, lens.clamp(0, Lk), kpm, sc, g if train else None)
+    if not train:
+        inside(out, *want, "out")
+        return
+    grads = torch.autograd.grad(out, leaves, g)
+    again = ops.bias_attention(*leaves, buckets, causal=causal, q_offset=arg, kv_len=lens if kv_len is not None else None,
+                               key_padding_mask=kpm, scale=scale)
+    for name, x, y, (w, tol), leaf in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads), (again, *torch.autograd.grad(again, leaves, g)), want,
+                                          [q, q, k, v, table]):
+        assert x.dtype == leaf.dtype
+        inside(x.detach(), w, tol, name)
+        assert torch.equal(x, y), name + " differs from run to run"
+
+
+SIZES = [
+    # B, Lq, Lk, H, Hkv, D, width
+    (1, 1, 1, 1, 1, 32, 0),
+    (2, 1, 70, 4, 4, 64, 0),
+    (1, 5, 3, 2, 1, 128, 0),
+    (2, 33, 65, 2, 2, 32, 0),
+    (1, 129, 200, 6, 2, 64, 0),
+    (2, 257, 257, 3, 3, 128, 0),
+    (2, 256, 256, 8, 8, 32, 16),
+    (1, 35, 35, 2, 1, 64, 7),
+    (3, 150, 150, 4, 4, 32, 25),
+    (1, 64, 64, 2, 2, 32, 1),
+    (8, 130, 130, 3, 1, 64, 13),
+]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", SIZES)
+def test_forward_and_gradients(ops, t, size):
+    B, Lq, Lk, H, Hkv, D, width = size
+    run_case(ops, t, B, Lq, Lk, H, Hkv, D, width=width, seed=sum(size))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [(1, 1, 1, 2, 1, 64), (2, 130, 130, 4, 2, 64), (1, 300, 300, 2, 2, 128), (2, 190, 190, 2, 1, 32)])
+def test_causal(ops, t, size):
+    run_case(ops, t, *size, causal=True, seed=3)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("width", [0, 9])
+def test_padding_hides_keys_and_whole_rows(ops, t, width):
+    run_case(ops, t, 3, 90, 90, 4, 2, 64, width=width, masked=True, seed=4)
+    run_case(ops, t, 4, 90, 90, 4, 2, 32, width=width, kv_len=[90, 64, 1, 0], seed=5)
+    run_case(ops, t, 4, 90, 90, 2, 2, 32, width=width, kv_len=[-7, 33, 1000, 65], masked=True, seed=6)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_positions(ops, t, causal):
+    run_case(ops, t, 2, 40, 100, 2, 2, 32, causal=causal, q_offset=60, seed=7)
+    run_case(ops, t, 3, 20, 100, 4, 1, 64, causal=causal, q_offset="end", kv_len=[100, 57, 20], seed=8)
+    # fewer keys than queries: the first queries stand before position 0 and see nothing
+    run_case(ops, t, 2, 20, 100, 2, 1, 64, causal=causal, q_offset="end", kv_len=[7, 100], seed=9)
+    # positions from a tensor, some of them outside of the buckets
+    run_case(ops, t, 3, 40, 100, 2, 2, 32, causal=causal, q_offset=[0, 95, -10], seed=10)
+    run_case(ops, t, 2, 12, 60, 2, 2, 32, width=6, causal=causal, q_offset=[30, 48], seed=11)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [(2, 1, 1000, 8, 2, 64), (1, 1, 4099, 4, 4, 128), (3, 4, 513, 8, 1, 32), (1, 3, 64, 40, 1, 64),
+                                  (1, 2, 2000, 6, 2, 128), (2, 1, 129, 33, 1, 32)])
+def test_few_queries_over_a_cache(ops, t, size):
+    B, Lq, Lk = size[:3]
+    lens = [Lk, max(Lq, Lk // 3), Lq][:B]
+    run_case(ops, t, *size, causal=True, q_offset="end", kv_len=lens, train=False, seed=12)
+    run_case(ops, t, *size, causal=True, q_offset="end", kv_len=lens, seed=12)
+    run_case(ops, t, *size, masked=B > 1, train=False, seed=13, max_len=Lk + 100)
+
+
+@pytest.mark.parametrize("t,table_t", [("bf16", "f32"), ("f16", "f32"), ("f32", "bf16"), ("f32", "f16")])
+def test_table_of_another_type(ops, t, table_t):
+    run_case(ops, t, 2, 100, 100, 4, 2, 64, table_t=table_t, seed=14)
+    run_case(ops, t, 2, 96, 96, 2, 2, 32, width=8, table_t=table_t, seed=15)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_scale_and_spread(ops, t):
+    run_case(ops, t, 1, 70, 70, 2, 2, 32, scale=1.0, seed=16)
+    run_case(ops, t, 1, 70, 70, 2, 2, 32, scale=0.0, seed=17)
+    run_case(ops, t, 1, 70, 70, 2, 2, 64, scale=-0.3, seed=18)
+
+
+def test_empty(ops):
+    b = ops.sequence_buckets(8, 16, 64, device=DEV)
+    table = torch.zeros(16, 2, device=DEV, requires_grad=True)
+    z = lambda B, L, H=2: torch.ones(B, L, H, 32, device=DEV, requires_grad=True)
+    for B, Lq, Lk in ((0, 4, 4), (2, 0, 4), (2, 4, 0), (0, 0, 0)):
+        q, k, v = z(B, Lq), z(B, Lk), z(B, Lk)
+        out = ops.bias_attention(q, k, v, table, b)
+        assert out.shape == (B, Lq, 2, 32) and not out.any()
+        for g, x in zip(torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out)), (q, k, v, table)):
+            assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_bias_that_masks(ops, t):
+    """-inf in the table hides; the type's lowest value does not, and a row of nothing else is averaged."""
+    T = TYPES[t]
+    b = ops.sequence_buckets(40, 8, 16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(T)
+    q, k, v, g = (rnd(1, 40, 2, 32).requires_grad_() for _ in range(4))
+    for low in (-math.inf, torch.finfo(T).min):
+        table = rnd(8, 2)
+        table[:, 1] = low                                   # head 1: every bucket
+        table[2:5, 0] = low
+        table.requires_grad_()
+        out = ops.bias_attention(q, k, v, table, b)
+        got = (out, *torch.autograd.grad(out, (q, k, v, table), g))
+        p = torch.arange(40, device=DEV)
+        bucket = b.cells[0].long()[(p[None] - p[:, None]) + 39]
+        leaf = [x.detach().double().requires_grad_() for x in (q, k, v, table)]
+        S = torch.einsum("bihd,bjhd->bhij", leaf[0], leaf[1]) / math.sqrt(32) + leaf[3][bucket].permute(2, 0, 1)[None]
+        if low == -math.inf:
+            S = S[:, :1]
+            want = torch.einsum("bhij,bjhd->bihd", S.softmax(3), leaf[2][:, :, :1])
+            assert not out[:, :, 1].any()
+        else:
+            if t != "f16":
+                S = torch.cat([S[:, :1], S[:, 1:] * 0], 1)     # in 32 bits the scores vanish beside the lowest value
+            want = torch.einsum("bhij,bjhd->bihd", S.softmax(3), leaf[2])
+        n = want.shape[2]
+        ref = (want, *torch.autograd.grad(want, leaf, g.detach().double()[:, :, :n]))
+        # f16: scores of 16 bits' range, -65504 +- 10 in 32 bits; a score then has 2^-9 steps, a probability 2^-8 of error
+        tol = {"f32": 2e-5, "bf16": 4e-2, "f16": 4e-2}[t]
+        for x, y, name in zip(got, ref, ("out", "dq", "dk", "dv", "dtable")):
+            assert torch.isfinite(x).all(), name
+            head = lambda z, i: z[:, i:i + 1] if name == "dtable" else z[:, :, i:i + 1]
+            heads = [0, 1] if n == 2 else [0]
+            if n == 1:
+                assert not head(x, 1).any(), name              # hidden altogether: nothing comes of it
+            elif t != "f16" and name not in ("out", "dv"):
+                heads = [0]                                    # constant scores have no counterpart in the reference's gradient
+            for i in heads:
+                y_i = torch.nan_to_num(head(y, i))
+                assert (head(x, i).double() - y_i).abs().max() <= tol * y_i.abs().max().clamp(min=1.0), (name, i)
+
+
+def test_lowest_value_everywhere_gives_the_mean(ops):
+    b = ops.sequence_buckets(100, 8, 16, device=DEV)
+    q, k, v = (torch.randn(1, 100, 1, 32, device=DEV).requires_grad_() for _ in range(3))
+    table = torch.full((8, 1), torch.finfo(torch.float32).min, device=DEV)
+    out = ops.bias_attention(q, k, v, table, b)
+    assert (out.double() - v.detach().double().mean(1, keepdim=True)).abs().max() < 100 * U32 * 5
+    dv, = torch.autograd.grad(out, v, torch.ones_like(out))
+    # every key gets 1 / 100 of each of 100 rows: 100 roundings of the sum, two of the probability
+    assert (dv.double() - 1).abs().max() < 110 * U32
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_strides(ops, t):
+    """Column windows of a packed projection, other orders of dimensions, odd alignments, expanded keys."""
+    T = TYPES[t]
+    B, L, H, D = 2, 70, 4, 32
+    b = ops.sequence_buckets(L, 8, 16, device=DEV)
+    table = torch.randn(8, H, device=DEV).to(T)
+    base = torch.randn(3, B, L, H, D, device=DEV).to(T)
+    want = ops.bias_attention(*base, table, b)
+    packed = base.permute(1, 2, 0, 3, 4).reshape(B, L, 3 * H * D)
+    win = [packed[:, :, i * H * D:(i + 1) * H * D].view(B, L, H, D) for i in range(3)]
+    assert not win[1].is_contiguous() and torch.equal(ops.bias_attention(*win, table, b), want)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in base]
+    assert torch.equal(ops.bias_attention(*heads_first, table, b), want)
+    room = torch.zeros(B, L, H * D + 1, device=DEV, dtype=T)
+    odd = []
+    for x in base:
+        r = room.clone()
+        r[:, :, 1:] = x.reshape(B, L, H * D)
+        odd.append(r[:, :, 1:].view(B, L, H, D) if False else r[:, :, 1:].unflatten(2, (H, D)))
+    assert odd[0].data_ptr() % 16 and torch.equal(ops.bias_attention(*odd, table, b), want)
+    assert torch.equal(ops.bias_attention(*base, table.t().contiguous().t(), b), want)
+    one = base[:, :1].contiguous()
+    k1, v1 = (one[i].detach().requires_grad_() for i in (1, 2))
+    wide = ops.bias_attention(base[0], k1.expand(B, -1, -1, -1), v1.expand(B, -1, -1, -1), table, b)
+    copied = [one[i].repeat(B, 1, 1, 1).requires_grad_() for i in (1, 2)]
+    assert torch.equal(wide, ops.bias_attention(base[0], *copied, table, b))
+    g = torch.randn(B, L, H, D, device=DEV).to(T)
+    dk, = torch.autograd.grad(wide, k1, g)
+    dc, = torch.autograd.grad(ops.bias_attention(base[0], *copied, table, b), copied[0], g)
+    assert torch.equal(dk, dc.sum(0, keepdim=True))
+    # a gradient that is not dense, and gradients of one input only
+    q = base[0].clone().requires_grad_()
+    out = ops.bias_attention(q, base[1], base[2], table, b)
+    gt = g.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(torch.autograd.grad(out, q, gt, retain_graph=True)[0], torch.autograd.grad(out, q, g)[0])
+
+
+def test_gradients_against_differences(ops):
+    torch.manual_seed(0)
+    b = ops.grid_buckets(4, 5, device=DEV)
+    q, k, v = (torch.randn(2, 20, 2, 32, device=DEV) for _ in range(3))
+    table = torch.randn(b.num_buckets, 2, device=DEV)
+    g = torch.randn(2, 20, 2, 32, device=DEV)
+    leaves = [x.requires_grad_() for x in (q, k, v, table)]
+    grads = torch.autograd.grad(ops.bias_attention(*leaves, b), leaves, g)
+    h = 2.0 ** -6
+    for i, (x, dx) in enumerate(zip(leaves, grads)):
+        d = torch.randn_like(x)
+        d = d / d.norm()
+        f = lambda s: (ops.bias_attention(*[y.detach() + s * d if n == i else y.detach() for n, y in enumerate(leaves)], b).double() * g).sum()
+        slope = (8 * (f(h) - f(-h)) - (f(2 * h) - f(-2 * h))) / (12 * h)
+        # fourth order: h^4 = 6e-8; the outputs' rounding, 1600 terms of about 10 U32 sqrt(1600) / h = 1.5e-3
+        assert abs(slope - (dx.double() * d).sum()) < 2e-3, i
+
+
+def test_gradients_wanted_of_some(ops):
+    b = ops.sequence_buckets(50, 8, 16, device=DEV)
+    base = [torch.randn(1, 50, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(3)] + [torch.randn(8, 2, device=DEV)]
+    g = torch.randn_like(base[0])
+    full = [x.clone().requires_grad_() for x in base]
+    want = torch.autograd.grad(ops.bias_attention(*full, b), full, g)
+    for i in range(4):
+        some = [x.clone().requires_grad_(n == i) for n, x in enumerate(base)]
+        got, = torch.autograd.grad(ops.bias_attention(*some, b), [some[i]], g)
+        assert torch.equal(got, want[i]), i
+
+
+def test_two_streams_and_no_grad(ops):
+    b = ops.sequence_buckets(300, 16, 64, device=DEV)
+    table = torch.randn(16, 4, device=DEV)
+    xs = [[torch.randn(2, 300, 4, 32, device=DEV) for _ in range(3)] for _ in range(2)]
+    want = [ops.bias_attention(*x, table, b) for x in xs]
+    s = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for st, x in zip(s, xs):
+        with torch.cuda.stream(st):
+            got.append(ops.bias_attention(*x, table, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("Lq,q_offset", [(1, "end"), (90, 0)])
+def test_graph_replays(ops, Lq, q_offset):
+    """Captured forward and backward, replayed on changed inputs and lengths between eager calls."""
+    b = ops.sequence_buckets(700, 16, 64, bidirectional=False, device=DEV)
+    B, Lk, H, D = 2, 700 if Lq == 1 else 90, 4, 64
+    mk = lambda *s: torch.randn(*s, device=DEV, dtype=torch.bfloat16)
+    q, k, v, g = mk(B, Lq, H, D), mk(B, Lk, 2, D), mk(B, Lk, 2, D), mk(B, Lq, H, D)
+    table = torch.randn(16, H, device=DEV)
+    lens = torch.tensor([Lk, Lk // 2], dtype=torch.int32, device=DEV)
+
+    def step():
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, table)]
+        out = ops.bias_attention(*leaves, b, causal=True, q_offset=q_offset, kv_len=lens)
+        return (out.detach(), *torch.autograd.grad(out, leaves, g))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in (Lk, 3, 41, Lk - 1):
+        for x in (q, k, v, g):
+            x.copy_(mk(*x.shape))
+        lens.copy_(torch.tensor([n, Lk], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(held, step()):
+            assert torch.equal(a, c)
+
+
+def test_long_cache_behind_32_bits(ops):
+    """Rows more than 2^31 elements into the cache."""
+    B, Lk, H, D = 1, 300, 2, 64
+    stride = (1 << 23) + 64                     # 300 rows of 8.4 M elements: 5 GB
+    room = torch.empty((Lk * stride,), dtype=torch.bfloat16, device=DEV)
+    k = room.as_strided((B, Lk, H, D), (0, stride, D, 1))
+    v = room[4096:].as_strided((B, Lk, H, D), (0, stride, D, 1))
+    small = [torch.randn(B, Lk, H, D, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    k.copy_(small[0])
+    v.copy_(small[1])
+    b = ops.sequence_buckets(Lk, 16, 64, device=DEV)
+    table = torch.randn(16, H, device=DEV)
+    for Lq in (1, 200):
+        q = torch.randn(B, Lq, H, D, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        a, c = ops.bias_attention(q, k, v, table, b), ops.bias_attention(q, *small, table, b)
+        assert torch.equal(a, c)
+        g = torch.randn_like(a)
+        assert torch.equal(torch.autograd.grad(a, q, g)[0], torch.autograd.grad(c, q, g)[0])
+
+
+def test_refusals(ops):
+    b = ops.sequence_buckets(64, 16, 64, device=DEV)
+    x = lambda *s, t=torch.float32: torch.zeros(*s, device=DEV, dtype=t)
+    q, k, tab = x(2, 8, 4, 32), x(2, 16, 2, 32), x(16, 4)
+    call = ops.bias_attention
+    bad = [
+        ((q.cpu(), k, k, tab, b), {}), ((q.double(), k.double(), k.double(), tab, b), {}), ((q, k.half(), k.half(), tab, b), {}),
+        ((x(2, 8, 4, 48), x(2, 16, 2, 48), x(2, 16, 2, 48), tab, b), {}), ((q, x(2, 16, 3, 32), x(2, 16, 3, 32), tab, b), {}),
+        ((q, k, x(2, 17, 2, 32), tab, b), {}), ((q, x(3, 16, 2, 32), x(3, 16, 2, 32), tab, b), {}), ((q[0], k[0], k[0], tab, b), {}),
+        ((q, k, k, x(15, 4), b), {}), ((q, k, k, x(16, 2), b), {}), ((q, k, k, tab.long(), b), {}),
+        ((q, x(2, 65, 2, 32), x(2, 65, 2, 32), tab, b), {}), ((q, k, k, tab, b), {"q_offset": 57}), ((q, k, k, tab, b), {"q_offset": -1}),
+        ((q, k, k, tab, b), {"q_offset": "start"}), ((q, k, k, tab, b), {"q_offset": x(2)}), ((q, k, k, tab, b), {"kv_len": x(3).int()}),
+        ((q, k, k, tab, b), {"kv_len": x(2).long()}), ((q, k, k, tab, b), {"key_padding_mask": x(2, 15).bool()}),
+        ((q, k, k, tab, b), {"key_padding_mask": x(2, 16)}),
+        ((q, k, k, tab, ops.sequence_buckets(64, 16, 64, device="cpu")), {}),
+    ]
+    for args, kw in bad:
+        with pytest.raises(RuntimeError, match="spot_amd"):
+            call(*args, **kw)
+    out = call(q.requires_grad_(), k, k, tab, b)
+    first, = torch.autograd.grad(out.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()

@@ -1,0 +1,274 @@
+"""Top logits and the distillation loss against their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from spot_amd import lib, ops as _ops
+    lib.load()
+    return _ops
+
+
+def ordered(x, k):
+    """Places by value, equal values by place, NaN first."""
+    key = torch.nan_to_num(x.double(), nan=math.inf, posinf=1e300, neginf=-math.inf)
+    at = torch.sort(key, dim=-1, descending=True, stable=True).indices[..., :k]
+    return x.gather(-1, at), at.int()
+
+
+def check_top(ops, x, k):
+    values, at = ops.top_logits(x, k)
+    want_v, want_at = ordered(x, k)
+    assert values.dtype == x.dtype and at.dtype == torch.int32 and values.shape == x.shape[:-1] + (k,)
+    assert torch.equal(at, want_at)
+    assert torch.equal(values.nan_to_num(nan=7.0), want_v.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,V,k", [(1, 1, 1), (3, 2, 2), (5, 7, 3), (2, 128, 128), (32, 1024, 16), (7, 625, 1), (3, 2040, 128),
+                                   (4, 2049, 50), (2, 8191, 64), (600, 5000, 17), (1, 32760, 128), (2, 32761, 128), (3, 100003, 8),
+                                   (1, 262144, 128), (1, 1048576, 100)])
+def test_top_logits(ops, t, N, V, k):
+    g = torch.Generator(device=DEV).manual_seed(N + V + k)
+    check_top(ops, (torch.randn(N, V, generator=g, device=DEV) * 3).to(TYPES[t]), k)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_top_logits_ties_and_special_values(ops, t):
+    T = TYPES[t]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for V, k in ((3000, 100), (40000, 128), (130, 128)):
+        check_top(ops, torch.zeros(3, V, device=DEV, dtype=T), k)                                       # all equal
+        check_top(ops, torch.randint(0, 3, (3, V), generator=g, device=DEV).to(T), k)                   # three values
+        check_top(ops, -torch.randint(0, 2, (3, V), generator=g, device=DEV).to(T) * 0.0, k)            # both zeros
+        x = torch.randn(4, V, generator=g, device=DEV).to(T)
+        x[0, ::3] = -math.inf
+        x[1, 5:20] = math.inf
+        x[2, 7:90:2] = math.nan
+        x[2, 8] = -math.nan
+        x[3] = -math.inf
+        check_top(ops, x, k)
+        x = torch.full((2, V), -1.0, device=DEV, dtype=T)
+        x[:, V // 2] = -0.0
+        x[:, V - 1] = 0.0
+        check_top(ops, x, min(k, 3))
+        rising = torch.arange(V, device=DEV).to(T)[None]
+        check_top(ops, rising, k)
+        check_top(ops, rising.flip(1), k)
+    tiny = torch.finfo(T).smallest_normal * torch.finfo(T).eps
+    check_top(ops, torch.arange(-40, 41, device=DEV).double().mul(tiny)[torch.randperm(81, generator=g, device=DEV)].to(T)[None], 60)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_top_logits_views(ops, t):
+    g = torch.Generator(device=DEV).manual_seed(2)
+    big = torch.randn(6, 5, 3001, generator=g, device=DEV).to(TYPES[t])
+    check_top(ops, big, 9)
+    check_top(ops, big[:, 2], 9)
+    check_top(ops, big[:, :, 1:], 9)
+    check_top(ops, big[:, :, ::2], 9)
+    check_top(ops, big.transpose(0, 1), 9)
+    check_top(ops, big[0, 0], 9)
+    check_top(ops, big[:1, :1].expand(4, 2, -1), 9)
+    v, at = ops.top_logits(big[:0], 4)
+    assert v.shape == (0, 5, 4) and at.shape == (0, 5, 4)
+
+
+def distill64(student, values, at, T, g=None):
+    """(loss, gradient) in 64 bits and how far the kernels may be off."""
+    V = student.shape[-1]
+    u = torch.finfo(student.dtype).eps / 2
+    x, t = student.double() / T, values.double() / T
+    here = (at >= 0) & (at < V) & (values != -math.inf)
+    some = here.any(1, keepdim=True)
+    place = at.long().clamp(0, V - 1)
+    t = t.masked_fill(~here, -math.inf)
+    logp = (t - torch.logsumexp(t, 1, keepdim=True)).masked_fill(~here, 0)
+    p = logp.exp().masked_fill(~here, 0)
+    logq = torch.log_softmax(x, 1)
+    term = torch.where(p > 0, p * (logp - logq.gather(1, place)), 0.0)
+    loss = torch.where(some[:, 0], T * T * term.sum(1), 0.0)
+    # exponents: one rounding of x / T log2 e against the row's reference, in units of the distance to it; the row's
+    # sum: V / 256 terms in a thread and 256 threads; p: k terms
+    far = lambda z, top: ((z - top).abs() + 4).nan_to_num(nan=0.0, posinf=0.0)
+    top = x.amax(1, keepdim=True)
+    eq = U32 * (4 * far(x, top) + 2 * top.abs() + V / 256 + 40)
+    tt = t.amax(1, keepdim=True)
+    et = U32 * (4 * far(t.nan_to_num(neginf=0.0), tt.nan_to_num(neginf=0.0)) + 8 * t.abs().nan_to_num(posinf=0.0) + 140)
+    big = eq.amax(1)
+    tol = T * T * ((p * (et * (1 + (logp - logq.gather(1, place)).abs().nan_to_num(posinf=0.0)) + eq.gather(1, place))).sum(1) + big +
+                   140 * U32 * term.abs().sum(1)) + U32 * loss.abs()
+    if g is None:
+        return loss, tol
+    scatter = lambda z: torch.zeros_like(x).scatter_add_(1, place, torch.where(here, z, 0.0))
+    dx = torch.where(some, (logq.exp() - scatter(p)) * (T * g.double()[:, None]), 0.0)
+    # an exponential below 2^-126 is zero: off by up to 2^-126 before the factor T g (the sum's reciprocal is at most 1)
+    tol_dx = ((logq.exp() * 2 * eq + scatter(p * (2 * et + 130 * U32))) * (T * g.double().abs()[:, None])) + (u + 4 * U32) * dx.abs()
+    tol_dx = tol_dx + 2.0 ** -126 * T * g.double().abs()[:, None]
+    return loss, tol, dx, tol_dx
+
+
+def check_distill(ops, student, values, at, T=1.0, seed=0):
+    g = torch.randn(student.shape[:-1], generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+    leaf = student.detach().requires_grad_()
+    loss = ops.top_logit_distillation(leaf, values, at, T)
+    dx, = torch.autograd.grad(loss, leaf, g)
+    again, = torch.autograd.grad(ops.top_logit_distillation(leaf, values, at, T), leaf, g)
+    assert torch.equal(dx, again) and dx.dtype == student.dtype and loss.dtype == torch.float32 and loss.shape == student.shape[:-1]
+    V, k = student.shape[-1], values.shape[-1]
+    want, tol, wdx, tdx = distill64(student.reshape(-1, V), values.reshape(-1, k), at.reshape(-1, k), T, g.reshape(-1))
+    off = (loss.detach().double().reshape(-1) - want).abs() - tol
+    assert off.numel() == 0 or off.max() <= 0, off.max()
+    off = (dx.double().reshape(-1, V) - wdx).abs() - tdx - torch.finfo(dx.dtype).smallest_normal * torch.finfo(dx.dtype).eps
+    assert off.numel() == 0 or off.max() <= 0, off.max()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,V,k,T", [(1, 1, 1, 1.0), (3, 2, 2, 1.0), (5, 7, 3, 0.5), (32, 1024, 16, 2.0), (9, 625, 128, 1.0),
+                                     (2, 8191, 64, 3.0), (700, 4097, 5, 1.0), (3, 100003, 8, 2.0), (1, 262144, 128, 1.0),
+                                     (5, 131073, 128, 4.0)])
+def test_distillation(ops, t, N, V, k, T):
+    gen = torch.Generator(device=DEV).manual_seed(N + V + k)
+    teacher = torch.randn(N, V, generator=gen, device=DEV) * 3
+    student = (teacher + torch.randn(N, V, generator=gen, device=DEV)).to(TYPES[t])
+    values, at = ops.top_logits(teacher.to(TYPES[t]), min(k, V))
+    check_distill(ops, student, values, at, T)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_distillation_absent_double_and_extreme_entries(ops, t):
+    T = TYPES[t]
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    for V in (300, 9001):
+        student = torch.randn(8, V, generator=gen, device=DEV).to(T)
+        values = torch.randn(8, 6, generator=gen, device=DEV)                 # a teacher of another type
+        at = torch.randint(0, V, (8, 6), generator=gen, device=DEV, dtype=torch.int32)
+        at[0] = -1                                                            # no entry at all
+        values[1] = -math.inf
+        at[2, 3:] = -1                                                        # a short row
+        at[3] = 17                                                            # one place, six times
+        at[4, 2:4] = at[4, 0]
+        at[5] = torch.tensor([V, V + 1, 2 ** 31 - 1, -2 ** 31, 0, V - 1])     # out of range: absent
+        values[6, 0] = torch.finfo(torch.float32).min
+        values[6, 1] = 80.0
+        student[7, ::2] = -math.inf
+        at[7] = torch.tensor([1, 3, 5, 7, 9, 11])
+        check_distill(ops, student, values, at)
+        student = student.nan_to_num(neginf=0.0) * 40                         # far apart: most probabilities vanish
+        check_distill(ops, student, values, at, T=0.7)
+    # a row without entries has zero gradient, whatever the student holds
+    student = torch.full((2, 500), math.nan, device=DEV).requires_grad_()
+    loss = ops.top_logit_distillation(student, torch.zeros(2, 3, device=DEV), torch.full((2, 3), -1, dtype=torch.int32, device=DEV))
+    assert not loss.any() and not torch.autograd.grad(loss.sum(), student)[0].any()
+    # an entry where the student has -inf: infinite loss, finite gradient
+    student = torch.zeros(1, 10, device=DEV)
+    student[0, 3] = -math.inf
+    student.requires_grad_()
+    loss = ops.top_logit_distillation(student, torch.zeros(1, 2, device=DEV), torch.tensor([[3, 4]], dtype=torch.int32, device=DEV))
+    dx, = torch.autograd.grad(loss.sum(), student)
+    assert loss.item() == math.inf and torch.isfinite(dx).all() and abs(dx[0, 3].item() + 0.5) < 1e-6
+
+
+def test_distillation_views_and_empty(ops):
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    for T in (torch.float32, torch.bfloat16):
+        big = torch.randn(4, 3, 2003, generator=gen, device=DEV).to(T)
+        for x in (big, big[:, 1], big[:, :, 1:], big[:, :, ::2], big.transpose(0, 1), big[0, 0][None]):
+            values, at = ops.top_logits(x, 5)
+            check_distill(ops, x, values, at, 1.5)
+    e = torch.zeros(0, 9, device=DEV, requires_grad=True)
+    loss = ops.top_logit_distillation(e, torch.zeros(0, 2, device=DEV), torch.zeros(0, 2, dtype=torch.int32, device=DEV))
+    assert loss.shape == (0,) and torch.autograd.grad(loss.sum(), e)[0].shape == (0, 9)
+
+
+def test_distillation_against_differences(ops):
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn(3, 50, generator=gen, device=DEV)
+    values, at = ops.top_logits(torch.randn(3, 50, generator=gen, device=DEV), 6)
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(ops.top_logit_distillation(leaf, values, at, 1.5).sum(), leaf)
+    d = torch.randn(3, 50, generator=gen, device=DEV)
+    d = d / d.norm()
+    h = 2.0 ** -4
+    f = lambda s: ops.top_logit_distillation(x + s * d, values, at, 1.5).double().sum()
+    slope = (8 * (f(h) - f(-h)) - (f(2 * h) - f(-2 * h))) / (12 * h)
+    # fourth order: h^4 / 30 of the fifth derivative, below 1e-5; rounding of losses of size 3: 20 U32 * 10 / h = 2e-4
+    assert abs(slope - (dx.double() * d).sum()) < 3e-4
+
+
+def test_graph_replays(ops):
+    x, teacher = torch.randn(3, 50000, device=DEV), torch.randn(3, 50000, device=DEV)
+    g = torch.rand(3, device=DEV)
+
+    def step():
+        values, at = ops.top_logits(teacher, 20)
+        leaf = x.detach().requires_grad_()
+        loss = ops.top_logit_distillation(leaf, values, at, 2.0)
+        return values, at, loss.detach(), torch.autograd.grad(loss, leaf, g)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(4):
+        x.normal_()
+        teacher.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_refusals(ops):
+    x = torch.zeros(4, 100, device=DEV)
+    v, at = torch.zeros(4, 3, device=DEV), torch.zeros(4, 3, dtype=torch.int32, device=DEV)
+    for bad in ((x.cpu(), 3), (x.double(), 3), (x, 0), (x, 101), (x, -1), (torch.zeros(2, 500, device=DEV), 129), (x[:, :0], 1),
+                (torch.zeros((), device=DEV), 1), (torch.zeros(1, (1 << 20) + 1, device=DEV), 1)):
+        with pytest.raises(RuntimeError, match="spot"):
+            ops.top_logits(*bad)
+    for bad in ((x.cpu(), v, at), (x, v.cpu(), at), (x, v, at.long()), (x, v.double(), at), (x, v[:3], at[:3]), (x, v, at[:, :2]),
+                (x, v[:, :0], at[:, :0]), (x, torch.zeros(4, 129, device=DEV), torch.zeros(4, 129, dtype=torch.int32, device=DEV)),
+                (x, v, at, 0.0), (x, v, at, -1.0), (x, v, at, math.inf), (x, v, at, math.nan), (x.long(), v, at)):
+        with pytest.raises(RuntimeError, match="spot"):
+            ops.top_logit_distillation(*bad)
+
+
+def test_student_learns_positions_from_a_teachers_top_places(ops):
+    """The operators as they are used together: biased attention over a token map gives each clip a score map, the
+    teacher's best places are its target; the gradients of all inputs against 64 bits."""
+    torch.manual_seed(0)
+    B, side, H, D, k = 3, 12, 4, 32, 10
+    L = side * side
+    buckets = ops.grid_buckets(side, side, device=DEV)
+    q, kk, v, w = (torch.randn(B, L, H, D, device=DEV) for _ in range(4))
+    table = torch.randn(buckets.num_buckets, H, device=DEV)
+    teacher = torch.randn(B, L, device=DEV) * 3
+    leaves = [x.requires_grad_() for x in (q, kk, v, table)]
+    score = (ops.bias_attention(*leaves, buckets) * w).sum((2, 3)) / math.sqrt(H * D)
+    loss = ops.top_logit_distillation(score, *ops.top_logits(teacher, k), 2.0).mean()
+    grads = torch.autograd.grad(loss, leaves)
+    deep = [x.detach().double().requires_grad_() for x in leaves]
+    p = torch.arange(L, device=DEV)
+    bucket = (p[None] // side - p[:, None] // side + side - 1) * (2 * side - 1) + p[None] % side - p[:, None] % side + side - 1
+    heads = lambda x: x.permute(0, 2, 1, 3)
+    S = heads(deep[0]) @ heads(deep[1]).transpose(2, 3) / math.sqrt(D) + deep[3][bucket].permute(2, 0, 1)
+    s64 = (heads(S.softmax(3) @ heads(deep[2])) * w.double()).sum((2, 3)) / math.sqrt(H * D)
+    tv, ta = torch.topk(teacher.double(), k, dim=1)
+    logp = torch.log_softmax(tv / 2, 1)
+    l64 = (4 * (logp.exp() * (logp - torch.log_softmax(s64 / 2, 1).gather(1, ta))).sum(1)).mean()
+    # losses of about 5: score roundings of 500 U32 relative to sums of 128 terms of size 1
+    assert abs(loss.item() - l64.item()) < 1e-4
+    for a, b in zip(grads, torch.autograd.grad(l64, deep)):
+        assert (a.double() - b).norm() <= 1e-4 * b.norm()
