@@ -616,10 +616,12 @@ int spot_clip_grad_norm_f32(float* grads, long n, float max_norm, float* norm_ou
  * included; keys hidden by causal alone have to be finite.  A query without a visible key has output and gradients 0.
  *
  * Forward: writes out, and for a backward pass stats [B, H, Lq, 2] floats (NULL: none) and out_lo (NULL: none; the
- * rounding error of a 16-bit out, from which the backward takes rowsum(out * d_out) to 32-bit precision).
+ * rounding error of a 16-bit out, from which the backward takes rowsum(out * d_out) to 32-bit precision).  ws:
+ * spot_bias_attention_fwd_ws_bytes bytes, 16-byte aligned (0 bytes: may be NULL).
  * Backward: reads what the forward read and wrote, and d_out; writes dq, dk and dv (both NULL: not wanted) and dtable
  * (table_dtype, [num_buckets, H]; NULL: not wanted).  cell_order int [cells]: the cells sorted by bucket; cell_start
  * int [num_buckets + 1]: where each bucket's begin in it.  ws: spot_bias_attention_bwd_ws_bytes bytes, 16-byte aligned.
+ * The sizes depend on the dimensions alone.
  * No atomics between workgroups: the same inputs give the same bits. */
 #define SPOT_BIAS_ATTN_MAX_LEN 1048576
 typedef struct spot_bias_attn_desc {
@@ -639,6 +641,7 @@ typedef struct spot_bias_attn_desc {
     int num_buckets, max_len, width, causal, q_offset_mode, q_offset;
     float scale;
 } spot_bias_attn_desc;
+int spot_bias_attention_fwd_ws_bytes(const spot_bias_attn_desc* desc /* host */, long* bytes /* host */);
 int spot_bias_attention_fwd(const spot_bias_attn_desc* desc /* host */, hipStream_t stream);
 int spot_bias_attention_bwd_ws_bytes(const spot_bias_attn_desc* desc /* host */, long* bytes /* host */);
 int spot_bias_attention_bwd(const spot_bias_attn_desc* desc /* host */, hipStream_t stream);

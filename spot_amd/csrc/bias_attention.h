@@ -41,6 +41,8 @@ struct Args {               // strides in elements; out, d_out, dq, dk, dv are d
     long q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
     int B, H, Hkv, G, Lq, Lk, N, width, nb, causal, off_mode, off, table_type;
     float scale, c;         // c = scale * log2 e
+    int heads, queries, tiles, splits;      // few_kernel: heads and queries of a tile of 32 rows, tiles, key ranges
+    float *few_o, *few_ml;                  // its partial results if splits > 1
 };
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
@@ -316,6 +318,250 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
         st[0] = m == -INFINITY ? 0.f : m;
         st[1] = inv * up<T>();
     }
+}
+
+// --- forward for few rows -------------------------------------------------------------------------------------------
+// A tile is 32 rows: `heads` query heads of one key/value head for `queries` queries each, so that every key and value
+// is read once for all of them (one new token: its heads).  A workgroup's four waves take 32-key tiles in turn and join
+// at the end; where the tiles are few the keys are cut in `splits` ranges, one workgroup each, joined by merge_kernel.
+// Keys go from memory to operand registers (a lane's row), values through the wave's own LDS, transposed; the next tile
+// is in flight while this one is worked on.  No barrier until the end.
+constexpr int FT = 32;      // keys per tile
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+struct FewRow { int i, head, last, px, p; bool ok; };
+__device__ __forceinline__ FewRow few_row(const Args& a, const Seq& s, int kvh, int tile, int r) {
+    // tiles: query blocks, then blocks of 32 heads where a key/value head has more than that
+    const int qb = (a.Lq + a.queries - 1) / a.queries, gi = r % a.heads, g = tile / qb * a.heads + gi;
+    FewRow f;
+    f.i = (tile % qb) * a.queries + r / a.heads;
+    f.head = kvh * a.G + g;
+    f.ok = r < a.heads * a.queries && f.i < a.Lq && g < a.G;
+    f.last = f.ok ? last_key(a, s, f.i) : -1;
+    f.p = s.off + f.i;
+    f.px = a.width ? ((f.p % a.width) + a.width) % a.width : 0;
+    return f;
+}
+template <class T> __device__ __forceinline__ void few_store(const Args& a, int b, const FewRow& f, int D, int d, const float* x,
+                                                             float inv) {
+    typename Vec<T>::v4 hi, rem;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = x[e] * inv;
+        hi[e] = (T)y;
+        rem[e] = (T)(y - (float)hi[e]);
+    }
+    const long at = (((long)b * a.Lq + f.i) * a.H + f.head) * D + d;
+    *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + at) = hi;
+    if (a.out_lo) *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out_lo) + at) = rem;
+}
+template <class T> __device__ __forceinline__ void few_stats(const Args& a, int b, const FewRow& f, float m, float inv) {
+    float* st = a.stats + (((long)b * a.H + f.head) * a.Lq + f.i) * 2;
+    st[0] = m == -INFINITY ? 0.f : m;
+    st[1] = inv * up<T>();
+}
+
+template <class T, int D> struct FewLds {
+    static constexpr int CP = FT + Vec<T>::PAD, V = D * CP;                              // elements of a wave's values
+    static constexpr int JOIN = 4 * 32 * 33 * 4 + 4 * 32 * 2 * 4;                        // bytes of the waves' join
+    static constexpr int BYTES = 4 * V * (int)sizeof(T) > JOIN ? 4 * V * (int)sizeof(T) : JOIN;
+};
+// floats of a wave's bias window, per class
+__host__ __device__ __forceinline__ int few_window(int heads, int queries) { return heads * (FT - 1 + queries); }
+
+template <class T, int D, bool MAP>
+__global__ __launch_bounds__(256) void few_kernel(const Args a) {
+    typedef FewLds<T, D> L;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int unit, rest;
+    place(a.B * a.Hkv, a.tiles * a.splits, unit, rest);
+    const int b = unit / a.Hkv, kvh = unit % a.Hkv, tile = rest / a.splits, split = rest % a.splits;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
+    const Seq s = sequence(a, b);
+    const FewRow f = few_row(a, s, kvh, tile, col);
+    T* sv = reinterpret_cast<T*>(lds) + w * L::V;
+    const int per = FT - 1 + a.queries, window = a.heads * per;
+    float* win = reinterpret_cast<float*>(lds + L::BYTES) + w * window * (MAP ? 2 : 1);
+    const int i0 = (tile % ((a.Lq + a.queries - 1) / a.queries)) * a.queries, g0 = f.head - kvh * a.G - col % a.heads;
+    const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
+    const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
+
+    typename Vec<T>::v8 qf[D / 16], kf[D / 16];
+    {
+        const T* qr = static_cast<const T*>(a.q) + b * a.q_b + (long)f.i * a.q_l + f.head * a.q_h;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) qf[c] = frag_or_zero(qr + 16 * c + 8 * h, f.ok);
+    }
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
+    float m = -INFINITY, sum = 0.f;
+
+    int end = a.causal ? min(s.len, s.off + min(i0 + a.queries, a.Lq)) : s.len;
+    const int all = (max(end, 0) + FT - 1) / FT;
+    const int t_begin = (int)((long)all * split / a.splits), t_end = (int)((long)all * (split + 1) / a.splits);
+
+    typename Vec<T>::v4 vr[D / 32][4];
+    unsigned live = 0, next_live = 0;
+    auto load = [&](int t) {
+        const int k0 = t * FT;
+        const int key = k0 + col;
+        bool ok = t < t_end && key < s.len;
+        if (ok && a.kpm) ok = a.kpm[(long)b * a.Lk + key] == 0;
+        next_live = (unsigned)__ballot(ok);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) kf[c] = frag_or_zero(kb + key * a.k_l + 16 * c + 8 * h, ok);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+            const int id = l + 64 * x, dg = id % (D / 4), g = id / (D / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                vr[x][j] = typename Vec<T>::v4{};
+                if ((next_live >> (4 * g + j)) & 1)
+                    vr[x][j] = *reinterpret_cast<const typename Vec<T>::v4*>(vb + (long)(k0 + 4 * g + j) * a.v_l + 4 * dg);
+            }
+        }
+    };
+    load(t_begin + w);
+    for (int t = t_begin + w; t < t_end; t += 4) {
+        const int k0 = t * FT;
+        live = next_live;
+        // offsets of a head's window: key - query from k0 - (p0 + queries - 1) on
+        for (int z = l; z < window; z += 64) {
+            const int gi = z / per, d = k0 - (s.off + i0 + a.queries - 1) + z % per, head = min(kvh * a.G + g0 + gi, a.H - 1);
+            win[z] = bias_at(a, 0, d, head);
+            if (MAP) win[window + z] = bias_at(a, 1, d, head);
+        }
+        f32x16 sc = {};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) mma(kf[c], qf[c], sc);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+            const int id = l + 64 * x, dg = id % (D / 4), g = id / (D / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<typename Vec<T>::v4*>(sv + (4 * dg + j) * L::CP + 4 * perm_group(g)) =
+                    typename Vec<T>::v4{vr[x][0][j], vr[x][1][j], vr[x][2][j], vr[x][3][j]};
+        }
+        load(t + 4);
+        wave_fence();
+        const int at = (col % a.heads) * per + a.queries - 1 - col / a.heads + 4 * h;     // rows past the last have no key
+        const unsigned lv = live >> (4 * h);
+        float mx = m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int j = 8 * (e >> 2) + (e & 3), key = k0 + j + 4 * h;
+            float bias = 0.f;
+            if (f.ok) {
+                bias = win[at + j];
+                if (MAP && key % a.width < f.px) bias = win[window + at + j];
+            }
+            sc[e] = ((lv >> j) & 1) && key <= f.last ? fmaf(sc[e], a.c, bias) : -INFINITY;
+            mx = fmaxf(mx, sc[e]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx != m)) {
+            const float x = __builtin_amdgcn_exp2f(m - ref);
+            sum *= x;
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) o[u] *= x;
+            m = mx;
+        }
+        const float low = ref - Vec<T>::SHIFT;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(sc[e] - low);
+            sum += sc[e];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const typename Vec<T>::v8 pf = acc_frag<T>(sc, c);
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) mma(frag<T>(sv + (32 * u + col) * L::CP + 16 * c + 8 * h), pf, o[u]);
+        }
+        wave_fence();
+    }
+    sum += __shfl_xor(sum, 32);
+
+    // the four waves' results: [wave][channel][row] and (m, sum) [wave][row]
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(lds);
+    float* ml = red + 4 * 32 * 33;
+    if (h == 0) {
+        ml[(w * 32 + col) * 2] = m;
+        ml[(w * 32 + col) * 2 + 1] = sum;
+    }
+    __syncthreads();
+    const int r = threadIdx.x & 31, d4 = (threadIdx.x >> 5) * 4;
+    auto joint = [&](int row, float& top, float& total) {
+        top = fmaxf(fmaxf(ml[row * 2], ml[(32 + row) * 2]), fmaxf(ml[(64 + row) * 2], ml[(96 + row) * 2]));
+        const float ref = top == -INFINITY ? 0.f : top;
+        total = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) total += ml[(32 * x + row) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(32 * x + row) * 2] - ref);
+        return ref;
+    };
+    float top, total;
+    const float mine = __builtin_amdgcn_exp2f(m - joint(col, top, total));
+    joint(r, top, total);
+    const FewRow fr = few_row(a, s, kvh, tile, r);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const long part = ((long)unit * a.tiles + tile) * a.splits + split;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) red[(w * 32 + acc_row(e, h)) * 33 + col] = o[u][e] * mine;
+        __syncthreads();
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = (red[(d4 + e) * 33 + r] + red[(32 + d4 + e) * 33 + r]) + (red[(64 + d4 + e) * 33 + r] + red[(96 + d4 + e) * 33 + r]);
+        if (fr.ok) {
+            if (a.splits == 1) few_store<T>(a, b, fr, D, 32 * u + d4, x, inv);
+            else *reinterpret_cast<float4*>(a.few_o + (part * 32 + r) * D + 32 * u + d4) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        __syncthreads();
+    }
+    if (fr.ok && d4 == 0) {
+        if (a.splits > 1) {
+            a.few_ml[(part * 32 + r) * 2] = top;
+            a.few_ml[(part * 32 + r) * 2 + 1] = total;
+        } else if (a.stats) {
+            few_stats<T>(a, b, fr, top, inv);
+        }
+    }
+}
+
+// One workgroup per tile: eight threads a row, the ranges in their order.
+template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(const Args a) {
+    const int unit = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, b = unit / a.Hkv, kvh = unit % a.Hkv;
+    const int r = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);
+    const Seq s = sequence(a, b);
+    const FewRow f = few_row(a, s, kvh, tile, r);
+    if (!f.ok) return;
+    const long part = ((long)unit * a.tiles + tile) * a.splits;
+    float top = -INFINITY, total = 0.f, x[D / 8];
+    for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.few_ml[((part + z) * 32 + r) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int e = 0; e < D / 8; ++e) x[e] = 0.f;
+    for (int z = 0; z < a.splits; ++z) {
+        const long at = (part + z) * 32 + r;
+        const float y = __builtin_amdgcn_exp2f(a.few_ml[at * 2] - ref);
+        total += a.few_ml[at * 2 + 1] * y;
+#pragma unroll
+        for (int e = 0; e < D / 8; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(a.few_o + at * D + d0 + e);
+            x[e] += v.x * y; x[e + 1] += v.y * y; x[e + 2] += v.z * y; x[e + 3] += v.w * y;
+        }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < D / 8; e += 4) few_store<T>(a, b, f, D, d0 + e, x + e, inv);
+    if (a.stats && d0 == 0) few_stats<T>(a, b, f, top, inv);
 }
 
 // --- dQ and the sums along the offsets ------------------------------------------------------------------------------
@@ -597,13 +843,16 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
 }
 
 // What the host part launches, one set per element type.
-enum { FWD, DQ, DKV };
+enum { FWD, FEW, MERGE, DQ, DKV };
 int launch_f32(int what, int D, const Args& a, unsigned grid, hipStream_t stream);
 int launch_bf16(int what, int D, const Args& a, unsigned grid, hipStream_t stream);
 int launch_f16(int what, int D, const Args& a, unsigned grid, hipStream_t stream);
 
 template <class T, int D, bool MAP> void launch_one(int what, const Args& a, unsigned grid, hipStream_t stream) {
     if (what == FWD) fwd_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
+    else if (what == FEW)
+        few_kernel<T, D, MAP><<<grid, 256, FewLds<T, D>::BYTES + 16 * few_window(a.heads, a.queries) * (MAP ? 2 : 1), stream>>>(a);
+    else if (what == MERGE) merge_kernel<T, D><<<grid, 256, 0, stream>>>(a);
     else if (what == DQ) dq_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
     else dkv_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
 }

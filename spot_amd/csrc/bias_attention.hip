@@ -62,6 +62,29 @@ static Layout layout(const spot_bias_attn_desc& d) {
     return l;
 }
 
+// The forward's kernel.  few_kernel reads keys once for all heads that share them and cuts the keys between its waves and
+// workgroups; fwd_kernel reads them once per 128 queries.  The former is taken for up to 32 rows per key/value head, and
+// where the latter's workgroups would not fill the 256 CUs.
+struct Few { bool use; int heads, queries, tiles, splits; long o, ml; };
+static Few few(const spot_bias_attn_desc& d) {
+    Few f = {};
+    const int G = d.H / d.Hkv;
+    f.use = (long)d.Lq * G <= 32 || (long)d.B * d.H * ((d.Lq + BM - 1) / BM) < 256;
+    f.heads = G < 32 ? G : 32;
+    f.queries = 32 / f.heads;
+    f.tiles = ((d.Lq + f.queries - 1) / f.queries) * ((G + f.heads - 1) / f.heads);
+    // about four workgroups per CU, each with a few tiles for every wave
+    const long units = (long)d.B * d.Hkv * f.tiles, most = d.Lk / (4 * FT * 2);
+    long splits = units ? 1024 / units : 1;
+    if (splits > most) splits = most;
+    f.splits = splits < 1 ? 1 : (int)splits;
+    if (f.splits > 1) {
+        f.o = units * f.splits * 32 * d.head_dim * 4;
+        f.ml = units * f.splits * 32 * 2 * 4;
+    }
+    return f;
+}
+
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 static int check(const spot_bias_attn_desc* d, bool backward) {
@@ -125,8 +148,26 @@ extern "C" int spot_bias_attention_fwd(const spot_bias_attn_desc* desc, hipStrea
     if (const int rc = check(desc, false)) return rc;
     const spot_bias_attn_desc& d = *desc;
     if (d.B == 0 || d.Lq == 0) return SPOT_OK;
-    const Args a = arguments(d);
-    return launch_any(d.dtype, FWD, d.head_dim, a, (unsigned)d.B * d.H * ((d.Lq + BM - 1) / BM), stream);
+    Args a = arguments(d);
+    const Few f = few(d);
+    if (!f.use) return launch_any(d.dtype, FWD, d.head_dim, a, (unsigned)d.B * d.H * ((d.Lq + BM - 1) / BM), stream);
+    SPOT_CHECK_ARG(f.splits == 1 || (d.ws && aligned16(d.ws) && d.ws_bytes >= f.o + f.ml),
+                   "spot_bias_attention_fwd: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", f.o + f.ml, d.ws_bytes);
+    a.heads = f.heads; a.queries = f.queries; a.tiles = f.tiles; a.splits = f.splits;
+    a.few_o = static_cast<float*>(d.ws);
+    a.few_ml = a.few_o + f.o / 4;
+    const unsigned tiles = (unsigned)d.B * d.Hkv * f.tiles;
+    const int rc = launch_any(d.dtype, FEW, d.head_dim, a, tiles * f.splits, stream);
+    return rc || f.splits == 1 ? rc : launch_any(d.dtype, MERGE, d.head_dim, a, tiles, stream);
+}
+
+extern "C" int spot_bias_attention_fwd_ws_bytes(const spot_bias_attn_desc* desc, long* bytes) {
+    using namespace ba;
+    if (const int rc = check(desc, false)) return rc;
+    SPOT_CHECK_ARG(bytes != nullptr, "spot_bias_attention_fwd_ws_bytes: null pointer");
+    const Few f = few(*desc);
+    *bytes = f.use && desc->Lq > 0 ? f.o + f.ml : 0;
+    return SPOT_OK;
 }
 
 extern "C" int spot_bias_attention_bwd_ws_bytes(const spot_bias_attn_desc* desc, long* bytes) {

@@ -131,6 +131,7 @@ SIGNATURES = {
     "spot_dropout_f32": [vp, vp, i64, i32, f32, C.c_uint, vp],
     "spot_layernorm_fwd_f32": [vp, vp, vp, vp, vp, vp, i64, i32, f32, vp],
     "spot_batchnorm_stats_f32": [vp, vp, i32, i32, i32, vp],
+    "spot_bias_attention_fwd_ws_bytes": [C.POINTER(BiasAttnDesc), C.POINTER(i64)],
     "spot_bias_attention_fwd": [C.POINTER(BiasAttnDesc), vp],
     "spot_bias_attention_bwd_ws_bytes": [C.POINTER(BiasAttnDesc), C.POINTER(i64)],
     "spot_bias_attention_bwd": [C.POINTER(BiasAttnDesc), vp],

@@ -2141,6 +2141,12 @@ def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_p
         d.k_stride_h = d.v_stride_h = 0
     lib.keep(q, k, v, out, out_lo, stats, table, buckets.cells, off_t, kv_len, kpm)
     with _on(q):
+        need = C.c_long(0)
+        lib.check(lib.load().spot_bias_attention_fwd_ws_bytes(C.byref(d), C.byref(need)), "spot_bias_attention_fwd")
+        if need.value:
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=q.device)
+            lib.keep(ws)
+            d.ws, d.ws_bytes = ws.data_ptr(), need.value
         lib.call("spot_bias_attention_fwd", C.byref(d), _st())
     return out, out_lo, stats, d, (q, k, v, table, off_t, kv_len, kpm)
 
@@ -2171,7 +2177,7 @@ class BiasAttentionFn(_Fn):
             setattr(d, name, None if t is None else t.data_ptr())
         with _on(q):
             need = C.c_long(0)
-            lib.call("spot_bias_attention_bwd_ws_bytes", C.byref(d), C.byref(need))
+            lib.check(lib.load().spot_bias_attention_bwd_ws_bytes(C.byref(d), C.byref(need)), "spot_bias_attention_bwd")
             ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
             d.ws, d.ws_bytes = ws.data_ptr(), need.value
             lib.call("spot_bias_attention_bwd", C.byref(d), _st())
@@ -2225,7 +2231,7 @@ def _logit_rows(x, name):
 
 def _ws(query, device, *args):
     need = C.c_long(0)
-    lib.call(query, *args, C.byref(need))
+    lib.check(getattr(lib.load(), query)(*args, C.byref(need)), query)      # answers at once, also while launches are collected
     return (torch.empty((need.value,), dtype=torch.uint8, device=device) if need.value else None), need.value
 
 
