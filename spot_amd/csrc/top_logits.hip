@@ -39,17 +39,20 @@ template <class T> __device__ __forceinline__ int order_key(T x) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// One workgroup takes a piece of a row, held in registers.
-//   1. The k-th largest of the 256 threads' maxima is a bound that at least k elements reach, and few more do: for
-//      values in random places about 256 ln(256 / (256 - k)), 74 for k = 64.
-//   2. What reaches it goes to a list in LDS; an element's rank is how many of the list stand before it (greater, or
-//      equal at a lower place), and the first k are written at their rank.
-//   3. Only if the list overflows (many equal values) the k-th value is found by bisection over the keys, and among
-//      its equals the last place by bisection over the places.
+// One workgroup takes a piece of a row.
+//   1. Streams it once, 16 bytes a load, and keeps the maximum of each load (and whether there is a NaN).
+//   2. A bound that the maxima of at least k threads reach, from bisection over the 256 of them: at least k elements
+//      reach it and few more do - for values in random places about 256 ln(256 / (256 - k)), 74 for k = 64.
+//   3. The loads whose maximum reaches it (about as many) are read again, and what reaches it goes to a list in LDS; an
+//      element's rank is how many of the list stand before it (greater, or equal at a lower place), and the first k are
+//      written at their rank.
+//   4. Only if a list overflows (many equal values) or the piece holds a NaN, the k-th value is found by bisection over
+//      the order of all elements, and among its equals the last place by bisection over the places.
 // Rows too long for one workgroup, or too few to fill the card, are cut in pieces; a second launch of the same kernel
 // takes the pieces' candidates, whose order is that of the places among equals.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int LIST = 1024;
+constexpr int LIST = 1280;           // 127 threads' first loads of 8 elements, and the piece's ends, fit
+constexpr int HITS = 1024;
 
 __device__ __forceinline__ int block_sum(int v, int* red) {
 #pragma unroll
@@ -65,116 +68,144 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ x, long l
                                                  const int* __restrict__ places, T* __restrict__ values, int* __restrict__ indices) {
     constexpr int VE = Vec16<T>::N;
     __shared__ __attribute__((aligned(16))) int s_max[NT];
-    __shared__ int s_key[LIST], s_at[LIST];
-    __shared__ int s_count, s_bound, red[4];
+    __shared__ __attribute__((aligned(16))) int2 s_list[LIST];      // (order key, place)
+    __shared__ int s_hit[HITS];
+    __shared__ int s_count, s_hits, s_nan, red[4];
     const long row = blockIdx.x / pieces;
-    const int piece = blockIdx.x % pieces;
+    const int piece = blockIdx.x % pieces, tid = threadIdx.x;
     const int begin = (int)((long)V * piece / pieces), n = (int)((long)V * (piece + 1) / pieces) - begin;
     const T* xr = x + row * ld + begin;
-    const int skew = skew_of(xr);
+    // [0, head) and [head + nv VE, n) are the ends before the first and behind the last 16-byte border
+    const int skew = skew_of(xr), head = min(skew ? VE - skew : 0, n), nv = (n - head) / VE;
+    const T* xv = xr + head;
+    if (tid == 0) s_count = s_hits = s_nan = 0;
 
-    typename Vec16<T>::v r[NV];
+    float top[NV], most = -INFINITY;
+    unsigned odd = 0;                                               // largest magnitude, as a whole number
 #pragma unroll
-    for (int i = 0; i < NV; ++i) r[i] = load_vec(xr, n, (i * NT + (int)threadIdx.x) * VE - skew, (T)0.f);
-    int top = (int)0x80000000;
+    for (int i = 0; i < NV; ++i) {
+        const int j = i * NT + tid;
+        top[i] = -INFINITY;
+        if (j < nv) {
+            const typename Vec16<T>::v v = *reinterpret_cast<const typename Vec16<T>::v*>(xv + (long)j * VE);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const int e = (i * NT + threadIdx.x) * VE - skew + j;
-            if ((unsigned)e < (unsigned)n) top = max(top, order_key(r[i][j]));
-        }
-    s_max[threadIdx.x] = top;
-    if (threadIdx.x == 0) s_count = 0;
-    __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < NT; i += 4) {
-        const int4 o = *reinterpret_cast<const int4*>(s_max + i);
-        rank += (o.x > top || (o.x == top && i < (int)threadIdx.x)) + (o.y > top || (o.y == top && i + 1 < (int)threadIdx.x)) +
-                (o.z > top || (o.z == top && i + 2 < (int)threadIdx.x)) + (o.w > top || (o.w == top && i + 3 < (int)threadIdx.x));
-    }
-    if (rank == k - 1) s_bound = top;
-    __syncthreads();
-    int bound = s_bound;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const int e = (i * NT + threadIdx.x) * VE - skew + j, key = order_key(r[i][j]);
-            if ((unsigned)e < (unsigned)n && key >= bound) {
-                const int at = atomicAdd(&s_count, 1);
-                if (at < LIST) {
-                    s_key[at] = key;
-                    s_at[at] = e;
-                }
+            for (int e = 0; e < VE; ++e) top[i] = fmaxf(top[i], (float)v[e]);
+            const uint4 u = *reinterpret_cast<const uint4*>(&v);
+            if (sizeof(T) == 4) {
+                odd = max(max(odd, max(u.x & 0x7fffffffu, u.y & 0x7fffffffu)), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu));
+            } else {
+                typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                auto pair = [](unsigned z) { z &= 0x7fff7fffu; return *reinterpret_cast<const u16x2*>(&z); };
+                u16x2 q = __builtin_elementwise_max(__builtin_elementwise_max(pair(u.x), pair(u.y)),
+                                                    __builtin_elementwise_max(pair(u.z), pair(u.w)));
+                q = __builtin_elementwise_max(q, *reinterpret_cast<const u16x2*>(&odd));
+                odd = *reinterpret_cast<const unsigned*>(&q);
             }
         }
+        most = fmaxf(most, top[i]);
+    }
+    const unsigned inf = sizeof(T) == 4 ? 0x7f800000u : (float)T(1) == 1.f && sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool has_nan = sizeof(T) == 4 ? odd > inf : (odd & 0xffff) > inf || (odd >> 16) > inf;
+    // one element of the ends for each of the first threads
+    const int end_at = tid < head ? tid : tid >= VE && tid - VE < n - head - nv * VE ? head + nv * VE + tid - VE : -1;
+    T end_x = (T)-INFINITY;
+    if (end_at >= 0) {
+        end_x = xr[end_at];
+        has_nan = has_nan || (float)end_x != (float)end_x;
+    }
+    s_max[tid] = order_key(most);
+    __syncthreads();
+    if (has_nan) s_nan = 1;
+
+    // a wave holds all 256 maxima; lo: at least k of them reach it
+    const int4 mine = *reinterpret_cast<const int4*>(s_max + 4 * (tid & 63));
+    int lo = min(min(mine.x, mine.y), min(mine.z, mine.w)), hi = max(max(mine.x, mine.y), max(mine.z, mine.w));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    for (int step = 0; step < 16 && hi > lo; ++step) {
+        const int mid = (int)(((long)lo + hi + 1) >> 1);
+        const int c = __popcll(__ballot(mine.x >= mid)) + __popcll(__ballot(mine.y >= mid)) + __popcll(__ballot(mine.z >= mid)) +
+                      __popcll(__ballot(mine.w >= mid));
+        if (c >= k) lo = mid; else hi = mid - 1;
+    }
+    const int bound = lo;
+    auto append = [&](T v, int at) {
+        const int key = order_key(v);
+        if (key < bound) return;
+        const int c = atomicAdd(&s_count, 1);
+        if (c < LIST) s_list[c] = make_int2(key, at);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = i * NT + tid;
+        if (j < nv && order_key(top[i]) >= bound) {
+            const int c = atomicAdd(&s_hits, 1);
+            if (c < HITS) s_hit[c] = j;
+        }
+    }
+    if (end_at >= 0) append(end_x, end_at);
+    __syncthreads();
+    const int hits = s_hits;
+    for (int z = tid; z < min(hits, HITS) * VE; z += NT) {
+        const int at = head + s_hit[z / VE] * VE + z % VE;
+        append(xr[at], at);
+    }
     __syncthreads();
     int count = s_count;
-    if (count > LIST) {
-        // the largest key that k elements reach: bound reaches it, lo holds that invariant
+    if (s_nan || hits > HITS || count > LIST) {
+        // the largest key that k elements reach
         auto reach = [&](long key) {
             int c = 0;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    const int e = (i * NT + threadIdx.x) * VE - skew + j;
-                    c += (unsigned)e < (unsigned)n && order_key(r[i][j]) >= key;
-                }
+            for (int e = tid; e < n; e += NT) c += order_key(xr[e]) >= key;
             return block_sum(c, red);
         };
-        long lo = bound, hi = 0x80000000L;              // reach(lo) >= k > reach(hi)
-        while (hi - lo > 1) {
-            const long mid = (lo + hi) >> 1;
-            if (reach(mid) >= k) lo = mid; else hi = mid;
+        long low = -0x80000000L, high = 0x80000000L;    // reach(low) >= k > reach(high)
+        while (high - low > 1) {
+            const long mid = (low + high) >> 1;
+            if (reach(mid) >= k) low = mid; else high = mid;
         }
-        const int kth = (int)lo, left = k - reach(hi);  // how many of those equal to the k-th are taken
+        const int kth = (int)low, left = k - reach(high);       // how many of those equal to the k-th are taken
         int first = -1, last = n - 1;                   // of them, up to `last` at least `left`, up to `first` fewer
         while (last - first > 1) {
             const int mid = (first + last) >> 1;
             int c = 0;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    const int e = (i * NT + threadIdx.x) * VE - skew + j;
-                    c += (unsigned)e <= (unsigned)mid && e < n && order_key(r[i][j]) == kth;
-                }
+            for (int e = tid; e <= mid; e += NT) c += order_key(xr[e]) == kth;
             if (block_sum(c, red) >= left) last = mid; else first = mid;
         }
         __syncthreads();
-        if (threadIdx.x == 0) s_count = 0;
+        if (tid == 0) s_count = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const int e = (i * NT + threadIdx.x) * VE - skew + j, key = order_key(r[i][j]);
-                if ((unsigned)e < (unsigned)n && (key > kth || (key == kth && e <= last))) {
-                    const int at = atomicAdd(&s_count, 1);
-                    s_key[at] = key;
-                    s_at[at] = e;
-                }
-            }
+        for (int e = tid; e < n; e += NT) {
+            const int key = order_key(xr[e]);
+            if (key > kth || (key == kth && e <= last)) s_list[atomicAdd(&s_count, 1)] = make_int2(key, e);     // k of them
+        }
         __syncthreads();
         count = s_count;
     }
     const long out = (long)blockIdx.x * k;
-    for (int c = threadIdx.x; c < count; c += NT) {
-        const int key = s_key[c], at = s_at[c];
+    for (int c = tid; c < count; c += NT) {
+        const int2 own = s_list[c];
         int before = 0;
-        for (int i = 0; i < count; ++i) before += s_key[i] > key || (s_key[i] == key && s_at[i] < at);
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const int2 o = s_list[i];
+            before += o.x > own.x || (o.x == own.x && o.y < own.y);
+        }
         if (before < k) {
-            values[out + before] = xr[at];
-            indices[out + before] = places ? places[row * V + at] : begin + at;
+            values[out + before] = xr[own.y];
+            indices[out + before] = places ? places[row * V + own.y] : begin + own.y;
         }
     }
 }
 
-template <class T> constexpr int capacity(int nv) { return (nv * NT - 1) * Vec16<T>::N; }   // whatever the skew is
+template <class T> constexpr int capacity(int nv) { return nv * NT * Vec16<T>::N; }
 
-// Pieces per row: what the registers of a workgroup hold at most, and about 512 workgroups where the rows are few (two
+// Pieces per row: what the maxima of a workgroup's loads cover at most, and about 512 workgroups where the rows are few (two
 // per CU), but no piece under 4096 elements, where a workgroup's fixed work is longer than its loads.
 template <class T> int top_pieces(int N, int V, int k) {
     const long most = capacity<T>(16);
