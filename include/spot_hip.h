@@ -608,9 +608,9 @@ int spot_clip_grad_norm_f32(float* grads, long n, float max_norm, float* norm_ou
  * Positions: key j stands at j, query i of sequence b at offset_b + i, where offset_b is q_offset (q_offset_mode 0),
  * q_offsets[b] (1) or kv_len[b] - Lq (2: the queries are the last of the keys).  A query whose position is negative or
  * not below max_len sees no key.
- * Buckets: the offset delta = key - query of a pair, and on a map of `width` > 0 columns the class
- * [key % width < query % width], select cells[class][delta + max_len - 1], an entry of 0 .. num_buckets - 1; cells is
- * int [width > 0 ? 2 : 1][2 max_len - 1].  table [num_buckets, H] of table_dtype.
+ * Buckets: u(p) = p, or on a map of `width` > 0 columns u(p) = p / width * (2 width - 1) + p % width, so that
+ * u(key) - u(query) stands for one offset (of places; of rows and columns).  cells[u(key) - u(query) + u(max_len - 1)]
+ * is its bucket, 0 .. num_buckets - 1; cells is int [2 u(max_len - 1) + 1].  table [num_buckets, H] of table_dtype.
  * Hidden keys: j >= kv_len[b] (NULL: none; clamped to 0 .. Lk), bytes of key_padding_mask [B, Lk] that are not zero
  * (NULL: none), and with causal those behind the query.  What kv_len and the mask hide may hold anything, NaN
  * included; keys hidden by causal alone have to be finite.  A query without a visible key has output and gradients 0.
@@ -624,6 +624,7 @@ int spot_clip_grad_norm_f32(float* grads, long n, float max_norm, float* norm_ou
  * The sizes depend on the dimensions alone.
  * No atomics between workgroups: the same inputs give the same bits. */
 #define SPOT_BIAS_ATTN_MAX_LEN 1048576
+#define SPOT_BIAS_ATTN_MAX_WIDTH 512
 typedef struct spot_bias_attn_desc {
     const void *q, *k, *v;
     void *out, *out_lo;

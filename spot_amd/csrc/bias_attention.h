@@ -9,16 +9,17 @@
 // or eight v_mfma_f32_32x32x2_f32, which read the same fragments (lane l: 8 consecutive reduction indices
 // 8 (l / 32) + 0..7 of row / column l % 32; the instruction only needs both operands to agree which index sits where).
 // The accumulator of a score tile (element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32) then is an
-// operand of the next product as it stands, if the other operand is stored with the middle two of every four groups of
-// four reduction indices exchanged (perm_group): no score ever passes through LDS.
+// operand of the next product as it stands, if the other operand takes its reduction indices in that order: no score
+// ever passes through LDS.  That other operand is a tile's column; ds_read_b64_tr_b16 reads it from the row-major tile
+// (four rows of 16 columns per 16 lanes), in f32 single words do.
 //
-// Bias.  For a pair the offset delta = j - p fixes the bucket, on a map of `width` columns together with the class
-// [x_j < x_p] (the offset wraps around a row or does not): a tile of queries x keys meets at most rows + columns - 1
-// offsets, so the tile's window of biases is looked up once per tile into LDS and read from there per element.
+// Bias.  Position p of a sequence has the coordinate u(p) = p, on a map of W columns u(p) = p / W (2 W - 1) + p % W, so
+// that u(key) - u(query) stands for one offset in either; `bias` is the table spread out by that difference, per head
+// and times log2 e.  A tile of queries x keys meets a window of it, which goes to LDS with the tile.
 //
-// Statistics.  Row maximum and reciprocal row sum are kept apart: as one number (their log-sum-exp) a row of scores
-// near the type's lowest value would lose the sum.  A row that sees no key has maximum 0 and reciprocal 0: its output
-// and gradients are zero.
+// Statistics.  A row's reference (its maximum or a little less) and reciprocal sum are kept apart: as one number (their
+// log-sum-exp) a row of scores near the type's lowest value would lose the sum.  A row that sees no key has reference 0
+// and reciprocal 0: its output and gradients are zero.
 #pragma once
 #include <float.h>
 
@@ -30,16 +31,18 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int BM = 128;     // queries per workgroup of the forward and dQ kernels: 32 per wave
 constexpr int BN = 64;      // keys per LDS tile there
 constexpr int KB = 128;     // keys per workgroup of the dK / dV kernel: 32 per wave
-constexpr int QB = 32;      // queries per LDS tile there
+constexpr int MAXW = 512;   // columns of a map
+constexpr int PADB = 64;    // entries behind the last of a head's spread-out biases
 
 struct Args {               // strides in elements; out, d_out, dq, dk, dv are dense [B, L, heads, D]
     const void *q, *k, *v, *d_out, *table;
     void *out, *out_lo, *dq, *dk, *dv;
-    float *stats, *delta, *part;
+    float *stats, *delta, *part, *bias;
     const int *cells, *q_offsets, *kv_len;
     const unsigned char* kpm;
     long q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
     int B, H, Hkv, G, Lq, Lk, N, width, nb, causal, off_mode, off, table_type;
+    int ncells, pitch, window;  // 2 u(N - 1) + 1; floats of a head's biases; window of a workgroup's tile
     float scale, c;         // c = scale * log2 e
     int heads, queries, tiles, splits;      // few_kernel: heads and queries of a tile of 32 rows, tiles, key ranges
     float *few_o, *few_ml;                  // its partial results if splits > 1
@@ -52,11 +55,14 @@ template <class T> struct Vec {
     typedef T v8 __attribute__((ext_vector_type(8)));
     typedef T v4 __attribute__((ext_vector_type(4)));
     // probabilities become operands times 2^SHIFT: a half float is subnormal from 2^-14 on, and the rows of a thousand
-    // keys hold little else; 2^12 of the row's largest still is far from its end
+    // keys hold little else
     static constexpr int SHIFT = 0;
+    // a row's reference may fall behind its maximum by 2^LAG before the sums are scaled again
+    static constexpr int LAG = 8;
     static constexpr int PAD = 16 / sizeof(T);      // LDS rows are padded by 16 bytes: eight lanes' 16-byte reads meet all banks
 };
 template <> constexpr int Vec<_Float16>::SHIFT = 12;
+template <> constexpr int Vec<_Float16>::LAG = 3;   // 2^15 is a half float
 template <class T> constexpr float up() { return (float)(1 << Vec<T>::SHIFT); }
 template <class T> constexpr float down() { return 1.f / (1 << Vec<T>::SHIFT); }
 
@@ -70,8 +76,6 @@ __device__ __forceinline__ void mma(const Vec<float>::v8& a, const Vec<float>::v
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
 }
-
-__device__ __forceinline__ int perm_group(int g) { return (g & ~3) | ((g & 1) << 1) | ((g >> 1) & 1); }
 __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
 
 // accumulator elements 8 s .. 8 s + 7 as an operand: rounded to T (the matrix instructions of the 16-bit types take
@@ -82,6 +86,38 @@ template <class T> __device__ __forceinline__ typename Vec<T>::v8 acc_frag(const
     for (int j = 0; j < 8; ++j) f[j] = (T)a[8 * s + j];
     return f;
 }
+template <class T> __device__ __forceinline__ typename Vec<T>::v8 frag(const T* p) {
+    return *reinterpret_cast<const typename Vec<T>::v8*>(p);
+}
+template <class T> __device__ __forceinline__ typename Vec<T>::v8 frag_or_zero(const T* p, bool ok) {
+    typename Vec<T>::v8 z = {};
+    return ok ? *reinterpret_cast<const typename Vec<T>::v8*>(p) : z;
+}
+
+// Column c0 + l % 32 of a row-major LDS tile of pitch P, rows r0 + acc_row(0 .. 7, l / 32), as an operand.
+template <class T, int P> struct ColFrag {
+    const T* p;             // what this lane addresses for r0 = c0 = 0
+    __device__ __forceinline__ explicit ColFrag(const T* tile) {
+        const int l = threadIdx.x & 63;
+        if (sizeof(T) == 4) p = tile + 4 * (l >> 5) * P + (l & 31);
+        else p = tile + (4 * (l >> 5) + ((l & 15) >> 2)) * P + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+    }
+    __device__ __forceinline__ typename Vec<T>::v8 operator()(int r0, int c0) const {
+        typename Vec<T>::v8 f;
+        const T* x = p + r0 * P + c0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = x[(8 * (j >> 2) + (j & 3)) * P];
+        } else {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) s4 lds_s4;
+            const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)x), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(x + 8 * P));
+            f = __builtin_bit_cast(typename Vec<T>::v8, (s8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        return f;
+    }
+};
 
 // --- one sequence's positions -------------------------------------------------------------------------------------
 struct Seq { int len, off; };
@@ -96,6 +132,13 @@ __device__ __forceinline__ int last_key(const Args& a, const Seq& s, int i) {
     const int p = s.off + i;
     return i >= a.Lq || p < 0 || p >= a.N ? -1 : a.causal ? p : 0x7fffffff;
 }
+template <bool MAP> __device__ __forceinline__ int coord(const Args& a, int p) {
+    return MAP ? p / a.width * (2 * a.width - 1) + p % a.width : p;
+}
+// end of the keys that the workgroup of queries q0 .. q0 + BM - 1 has to see
+__device__ __forceinline__ int key_end(const Args& a, const Seq& s, int q0) {
+    return a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
+}
 // bit l: key k0 + l is no padding
 __device__ __forceinline__ unsigned long long live_keys(const Args& a, const Seq& s, int b, int k0) {
     const int key = k0 + (threadIdx.x & 63);
@@ -105,12 +148,11 @@ __device__ __forceinline__ unsigned long long live_keys(const Args& a, const Seq
 }
 
 // --- bias ---------------------------------------------------------------------------------------------------------
-// log2 e * table[bucket of (offset delta, class cls)][head].  Scores live in the log2 domain; a finite entry stays
-// finite there (the type's lowest value as a mask must not turn into -inf, which hides a key altogether).
-__device__ __forceinline__ float bias_at(const Args& a, int cls, int delta, int head) {
-    const int i = delta + a.N - 1, n = 2 * a.N - 1;
-    if ((unsigned)i >= (unsigned)n) return 0.f;
-    const int bucket = a.cells[cls * n + i];
+// log2 e * table[cells[i]][head].  Scores live in the log2 domain; a finite entry stays finite there (the type's lowest
+// value as a mask must not turn into -inf, which hides a key altogether).
+__device__ __forceinline__ float bias_at(const Args& a, int i, int head) {
+    if ((unsigned)i >= (unsigned)a.ncells) return 0.f;
+    const int bucket = a.cells[i];
     if ((unsigned)bucket >= (unsigned)a.nb) return 0.f;
     const long at = (long)bucket * a.H + head;
     const float t = a.table_type == F32 ? static_cast<const float*>(a.table)[at]
@@ -120,56 +162,53 @@ __device__ __forceinline__ float bias_at(const Args& a, int cls, int delta, int 
     return fabsf(t) <= FLT_MAX ? fminf(fmaxf(r, -FLT_MAX), FLT_MAX) : r;
 }
 
-// --- LDS tiles ----------------------------------------------------------------------------------------------------
-// ROWS x D elements in blocks of 4 x 4 per thread, stored row-major (pitch D + PAD) and / or transposed (pitch
-// ROWS + PAD, groups of four rows in perm_group order).  Rows whose bit in `live` is not set are zero: what padding
-// holds (infinities, NaN) does not reach a product.
+// Window of a head's biases from cell i0 on, by 256 threads; the first 512 entries travel in registers while the tile
+// before is worked on, what a very wide map needs beyond is read when it is stored.
+struct Window {
+    float r[2];
+    int i0;
+    __device__ __forceinline__ static float at(const Args& a, const float* bias, int i) {
+        return (unsigned)i < (unsigned)a.ncells ? bias[i] : 0.f;
+    }
+    __device__ __forceinline__ void load(const Args& a, const float* bias, int from, int n) {
+        i0 = from;
+        r[0] = at(a, bias, from + (int)threadIdx.x);
+        if (n > 256) r[1] = at(a, bias, from + 256 + (int)threadIdx.x);
+    }
+    __device__ __forceinline__ void store(const Args& a, const float* bias, float* lds, int n) const {
+        if ((int)threadIdx.x < n) lds[threadIdx.x] = r[0];
+        if (n > 256 && (int)threadIdx.x + 256 < n) lds[threadIdx.x + 256] = r[1];
+        for (int t = 512 + threadIdx.x; t < n; t += 256) lds[t] = at(a, bias, i0 + t);
+    }
+};
+// entries of a window: keys and queries in a row, u's range on a map
+constexpr int window_span(int n, int width) { return n - 1 + (width ? ((n - 1) / width + 1) * (width - 1) : 0); }
+constexpr int window_of(int keys, int queries, int width) { return window_span(keys, width) + window_span(queries, width) + 1; }
+template <bool MAP> struct WindowLds { static constexpr int N = MAP ? 1280 : BM + BN; };
+static_assert(window_of(64, 128, MAXW) <= 1280 && window_of(64, 128, 127) <= 1280, "a tile's window has to fit");
+
+// --- LDS tiles: ROWS x D elements, row-major, 16 bytes a load.  Rows whose bit in `live` is not set are zero: what
+// padding holds (infinities, NaN) does not reach a product.
 template <class T, int D, int ROWS> struct Tile {
-    typedef typename Vec<T>::v4 v4;
-    static constexpr int BLOCKS = ROWS * D / 16, NB = (BLOCKS + 255) / 256;
-    static constexpr int RP = D + Vec<T>::PAD, CP = ROWS + Vec<T>::PAD;
-    static constexpr int ROW_ELEMS = ROWS * RP, COL_ELEMS = D * CP;
-    v4 r[NB][4];
+    static constexpr int P = D + Vec<T>::PAD, ELEMS = ROWS * P;
+    static constexpr int VE = 16 / sizeof(T), VR = D / VE, VECS = ROWS * VR, NV = (VECS + 255) / 256;
+    uint4 r[NV];
     __device__ __forceinline__ void load(const T* base, long stride, unsigned long long live) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, dg = id % (D / 4), g = id / (D / 4);
-            if (BLOCKS % 256 != 0 && id >= BLOCKS) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = 4 * g + j;
-                r[i][j] = v4{};
-                if ((live >> row) & 1) r[i][j] = *reinterpret_cast<const v4*>(base + row * stride + 4 * dg);
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int id = threadIdx.x + 256 * i, row = id / VR, c = id % VR;
+            r[i] = make_uint4(0, 0, 0, 0);
+            if ((VECS % 256 == 0 || id < VECS) && ((live >> row) & 1)) r[i] = *reinterpret_cast<const uint4*>(base + row * stride + c * VE);
         }
     }
-    __device__ __forceinline__ void rows(T* lds) const {
+    __device__ __forceinline__ void store(T* lds) const {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, dg = id % (D / 4), g = id / (D / 4);
-            if (BLOCKS % 256 != 0 && id >= BLOCKS) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<v4*>(lds + (4 * g + j) * RP + 4 * dg) = r[i][j];
-        }
-    }
-    __device__ __forceinline__ void cols(T* lds) const {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, dg = id % (D / 4), g = id / (D / 4);
-            if (BLOCKS % 256 != 0 && id >= BLOCKS) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<v4*>(lds + (4 * dg + j) * CP + 4 * perm_group(g)) = v4{r[i][0][j], r[i][1][j], r[i][2][j], r[i][3][j]};
+        for (int i = 0; i < NV; ++i) {
+            const int id = threadIdx.x + 256 * i;
+            if (VECS % 256 == 0 || id < VECS) *reinterpret_cast<uint4*>(lds + id / VR * P + id % VR * VE) = r[i];
         }
     }
 };
-template <class T> __device__ __forceinline__ typename Vec<T>::v8 frag(const T* p) {
-    return *reinterpret_cast<const typename Vec<T>::v8*>(p);
-}
-template <class T> __device__ __forceinline__ typename Vec<T>::v8 frag_or_zero(const T* p, bool ok) {
-    typename Vec<T>::v8 z = {};
-    return ok ? *reinterpret_cast<const typename Vec<T>::v8*>(p) : z;
-}
 
 // Workgroup -> (sequence, key/value head, rest).  Consecutive workgroups go to the eight XCDs in turn; where the number
 // of key/value heads allows it, all workgroups that read the same keys and values share one XCD's L2.
@@ -184,16 +223,62 @@ __device__ __forceinline__ void place(int units, int per_unit, int& unit, int& r
     }
 }
 
+// The softmax step of a lane's row: the scores of NT tiles become 2^(s - reference + SHIFT), the sums are scaled where
+// the reference moves.
+template <class T, int NT, int NO>
+__device__ __forceinline__ void softmax_step(f32x16* sc, float& m, float& sum, f32x16* o) {
+    float mx = sc[0][0];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m + Vec<T>::LAG)) {
+        const float to = fmaxf(mx, m), f = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < NO; ++t) o[t] *= f;
+        m = to;
+    }
+    const float low = (m == -INFINITY ? 0.f : m) - Vec<T>::SHIFT;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sc[u][e] = __builtin_amdgcn_exp2f(sc[u][e] - low);
+            part[e & 3] += sc[u][e];
+        }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+template <class T> __device__ __forceinline__ void store_out(const Args& a, long at, const float* x, float inv) {
+    typename Vec<T>::v4 hi, rem;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = x[e] * inv;
+        hi[e] = (T)y;
+        rem[e] = (T)(y - (float)hi[e]);
+    }
+    *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + at) = hi;
+    if (a.out_lo) *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out_lo) + at) = rem;
+}
+template <class T> __device__ __forceinline__ void store_stats(const Args& a, int b, int head, int i, float m, float inv) {
+    float* st = a.stats + (((long)b * a.H + head) * a.Lq + i) * 2;
+    st[0] = m == -INFINITY ? 0.f : m;
+    st[1] = inv * up<T>();
+}
+
 // --- forward ------------------------------------------------------------------------------------------------------
-// One workgroup: 128 queries of one head, 32 per wave; keys stream through LDS in tiles of 64.  Queries sit on the
-// lanes (S^T = K Q^T), so running maximum and sum are one number per lane.
+// One workgroup: 128 queries of one head, 32 per wave; keys stream through LDS in tiles of 64, the next one in flight in
+// registers.  Queries sit on the lanes (S^T = K Q^T), so reference and sum are one number per lane.
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
+__global__ __launch_bounds__(256, 2) void fwd_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
-    __shared__ __attribute__((aligned(16))) T sk[KT::ROW_ELEMS];
-    __shared__ __attribute__((aligned(16))) T sv[KT::COL_ELEMS];
-    __shared__ float sb[MAP ? 2 : 1][BM + BN];
-    __shared__ __attribute__((aligned(16))) int sx[BN];
+    __shared__ __attribute__((aligned(16))) T sk[KT::ELEMS];
+    __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
+    __shared__ float sb[WindowLds<MAP>::N];
+    __shared__ __attribute__((aligned(16))) int su[BN];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
     place(a.B * a.Hkv, a.G * nq, unit, rest);
@@ -202,10 +287,11 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
-    const int last = last_key(a, s, i), p = s.off + i;
-    const int px = MAP ? ((p % a.width) + a.width) % a.width : 0;
+    const int last = last_key(a, s, i);
+    const int u_hi = coord<MAP>(a, max(s.off + q0 + BM - 1, 0)), lane_u = u_hi - coord<MAP>(a, max(s.off + i, 0));
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
+    const float* bias = a.bias + (long)head * a.pitch;
 
     typename Vec<T>::v8 qf[D / 16];
     {
@@ -218,42 +304,49 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
     for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, sum = 0.f;
 
-    const int k_end = a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
+    const int k_end = key_end(a, s, q0);
+    const ColFrag<T, KT::P> vcol(sv);
+    KT tk, tv;
+    Window tw;
+    unsigned long long next = 0;
+    auto load = [&](int k0) {
+        next = live_keys(a, s, b, k0);
+        tk.load(kb + k0 * a.k_l, a.k_l, next);
+        tv.load(vb + k0 * a.v_l, a.v_l, next);
+        tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
+    };
+    if (k_end > 0) load(0);
     for (int k0 = 0; k0 < k_end; k0 += BN) {
-        const unsigned long long live = live_keys(a, s, b, k0);
-        KT tk, tv;
-        tk.load(kb + k0 * a.k_l, a.k_l, live);
-        tv.load(vb + k0 * a.v_l, a.v_l, live);
+        const unsigned long long live = next;
         __syncthreads();
-        tk.rows(sk);
-        tv.cols(sv);
-        const int d0 = k0 - (s.off + q0 + BM - 1);
-        for (int t = threadIdx.x; t < BM + BN - 1; t += 256) {
-            sb[0][t] = bias_at(a, 0, d0 + t, head);
-            if (MAP) sb[MAP ? 1 : 0][t] = bias_at(a, 1, d0 + t, head);
-        }
-        if (MAP && threadIdx.x < BN) sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
+        tk.store(sk);
+        tv.store(sv);
+        tw.store(a, bias, sb, a.window);
+        if (MAP && threadIdx.x < BN) su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
         __syncthreads();
+        if (k0 + BN < k_end) load(k0 + BN);
 
         f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) mma(frag<T>(sk + (32 * u + col) * KT::RP + 16 * c + 8 * h), qf[c], sc[u]);
-
-        const int lane_b = BM - 1 - (32 * w + col) + 4 * h;
-        const bool masked = live != ~0ull || __any(last < k0 + BN - 1);
-        float mx = m;
+            for (int u = 0; u < 2; ++u) mma(frag<T>(sk + (32 * u + col) * KT::P + 16 * c + 8 * h), qf[c], sc[u]);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = 32 * u + 8 * (e >> 2) + (e & 3);       // + 4 h
-                float bias = sb[0][lane_b + j];
-                if (MAP && sx[j + 4 * h] < px) bias = sb[MAP ? 1 : 0][lane_b + j];
-                sc[u][e] = fmaf(sc[u][e], a.c, bias);
+            for (int g = 0; g < 4; ++g) {
+                const int j = 32 * u + 8 * g;                        // + 4 h + 0 .. 3
+                int4 x = {lane_u + 4 * h + j, lane_u + 4 * h + j + 1, lane_u + 4 * h + j + 2, lane_u + 4 * h + j + 3};
+                if (MAP) {
+                    const int4 y = *reinterpret_cast<const int4*>(su + j + 4 * h);
+                    x = {lane_u + y.x, lane_u + y.y, lane_u + y.z, lane_u + y.w};
+                }
+                sc[u][4 * g] = fmaf(sc[u][4 * g], a.c, sb[x.x]);
+                sc[u][4 * g + 1] = fmaf(sc[u][4 * g + 1], a.c, sb[x.y]);
+                sc[u][4 * g + 2] = fmaf(sc[u][4 * g + 2], a.c, sb[x.z]);
+                sc[u][4 * g + 3] = fmaf(sc[u][4 * g + 3], a.c, sb[x.w]);
             }
-        if (masked) {
+        if (live != ~0ull || __any(last < k0 + BN - 1)) {
             const unsigned long long lv = live >> (4 * h);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -263,75 +356,43 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
                     if (!((lv >> j) & 1) || k0 + j + 4 * h > last) sc[u][e] = -INFINITY;
                 }
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx != m)) {
-            const float f = __builtin_amdgcn_exp2f(m - ref);
-            sum *= f;
-#pragma unroll
-            for (int t = 0; t < D / 32; ++t) o[t] *= f;
-            m = mx;
-        }
-        const float low = ref - Vec<T>::SHIFT;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[u][e] = __builtin_amdgcn_exp2f(sc[u][e] - low);
-                sum += sc[u][e];
-            }
+        softmax_step<T, 2, D / 32>(sc, m, sum, o);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const typename Vec<T>::v8 pf = acc_frag<T>(sc[u], c);
 #pragma unroll
-                for (int t = 0; t < D / 32; ++t) mma(frag<T>(sv + (32 * t + col) * KT::CP + 32 * u + 16 * c + 8 * h), pf, o[t]);
+                for (int t = 0; t < D / 32; ++t) mma(vcol(32 * u + 16 * c, 32 * t), pf, o[t]);
             }
     }
     sum += __shfl_xor(sum, 32);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (i >= a.Lq) return;
-    const long row = ((long)b * a.Lq + i) * a.H + head;
-    T* out = static_cast<T*>(a.out) + row * D;
-    T* lo = a.out_lo ? static_cast<T*>(a.out_lo) + row * D : nullptr;
+    const long row = (((long)b * a.Lq + i) * a.H + head) * D;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            typename Vec<T>::v4 hi, rem;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = o[t][4 * g + e] * inv;
-                hi[e] = (T)x;
-                rem[e] = (T)(x - (float)hi[e]);
-            }
-            *reinterpret_cast<typename Vec<T>::v4*>(out + 32 * t + 8 * g + 4 * h) = hi;
-            if (lo) *reinterpret_cast<typename Vec<T>::v4*>(lo + 32 * t + 8 * g + 4 * h) = rem;
+            const float x[4] = {o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+            store_out<T>(a, row + 32 * t + 8 * g + 4 * h, x, inv);
         }
-    if (a.stats && h == 0) {
-        float* st = a.stats + (((long)b * a.H + head) * a.Lq + i) * 2;
-        st[0] = m == -INFINITY ? 0.f : m;
-        st[1] = inv * up<T>();
-    }
+    if (a.stats && h == 0) store_stats<T>(a, b, head, i, m, inv);
 }
 
 // --- forward for few rows -------------------------------------------------------------------------------------------
 // A tile is 32 rows: `heads` query heads of one key/value head for `queries` queries each, so that every key and value
 // is read once for all of them (one new token: its heads).  A workgroup's four waves take 32-key tiles in turn and join
 // at the end; where the tiles are few the keys are cut in `splits` ranges, one workgroup each, joined by merge_kernel.
-// Keys go from memory to operand registers (a lane's row), values through the wave's own LDS, transposed; the next tile
-// is in flight while this one is worked on.  No barrier until the end.
+// Keys go from memory to operand registers (a lane's row), values through the wave's own LDS; the next tile is in flight
+// while this one is worked on.  No barrier until the end.  The biases come from memory (first-level cache): spread out
+// if there are many tiles, else (a.bias NULL) by bucket, which saves the launch that spreads them.
 constexpr int FT = 32;      // keys per tile
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-struct FewRow { int i, head, last, px, p; bool ok; };
+struct FewRow { int i, head, last, p; bool ok; };
 __device__ __forceinline__ FewRow few_row(const Args& a, const Seq& s, int kvh, int tile, int r) {
     // tiles: query blocks, then blocks of 32 heads where a key/value head has more than that
     const int qb = (a.Lq + a.queries - 1) / a.queries, gi = r % a.heads, g = tile / qb * a.heads + gi;
@@ -340,41 +401,21 @@ __device__ __forceinline__ FewRow few_row(const Args& a, const Seq& s, int kvh, 
     f.head = kvh * a.G + g;
     f.ok = r < a.heads * a.queries && f.i < a.Lq && g < a.G;
     f.last = f.ok ? last_key(a, s, f.i) : -1;
-    f.p = s.off + f.i;
-    f.px = a.width ? ((f.p % a.width) + a.width) % a.width : 0;
+    f.p = min(max(s.off + f.i, 0), a.N - 1);
     return f;
-}
-template <class T> __device__ __forceinline__ void few_store(const Args& a, int b, const FewRow& f, int D, int d, const float* x,
-                                                             float inv) {
-    typename Vec<T>::v4 hi, rem;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float y = x[e] * inv;
-        hi[e] = (T)y;
-        rem[e] = (T)(y - (float)hi[e]);
-    }
-    const long at = (((long)b * a.Lq + f.i) * a.H + f.head) * D + d;
-    *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + at) = hi;
-    if (a.out_lo) *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out_lo) + at) = rem;
-}
-template <class T> __device__ __forceinline__ void few_stats(const Args& a, int b, const FewRow& f, float m, float inv) {
-    float* st = a.stats + (((long)b * a.H + f.head) * a.Lq + f.i) * 2;
-    st[0] = m == -INFINITY ? 0.f : m;
-    st[1] = inv * up<T>();
 }
 
 template <class T, int D> struct FewLds {
-    static constexpr int CP = FT + Vec<T>::PAD, V = D * CP;                              // elements of a wave's values
+    static constexpr int P = D + Vec<T>::PAD, V = FT * P;                                // elements of a wave's values
     static constexpr int JOIN = 4 * 32 * 33 * 4 + 4 * 32 * 2 * 4;                        // bytes of the waves' join
     static constexpr int BYTES = 4 * V * (int)sizeof(T) > JOIN ? 4 * V * (int)sizeof(T) : JOIN;
 };
-// floats of a wave's bias window, per class
-__host__ __device__ __forceinline__ int few_window(int heads, int queries) { return heads * (FT - 1 + queries); }
 
 template <class T, int D, bool MAP>
 __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     typedef FewLds<T, D> L;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ __attribute__((aligned(16))) char lds[L::BYTES];
+    __shared__ __attribute__((aligned(16))) int s_u[4][FT];
     int unit, rest;
     place(a.B * a.Hkv, a.tiles * a.splits, unit, rest);
     const int b = unit / a.Hkv, kvh = unit % a.Hkv, tile = rest / a.splits, split = rest % a.splits;
@@ -382,11 +423,12 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     const Seq s = sequence(a, b);
     const FewRow f = few_row(a, s, kvh, tile, col);
     T* sv = reinterpret_cast<T*>(lds) + w * L::V;
-    const int per = FT - 1 + a.queries, window = a.heads * per;
-    float* win = reinterpret_cast<float*>(lds + L::BYTES) + w * window * (MAP ? 2 : 1);
-    const int i0 = (tile % ((a.Lq + a.queries - 1) / a.queries)) * a.queries, g0 = f.head - kvh * a.G - col % a.heads;
+    const int i0 = (tile % ((a.Lq + a.queries - 1) / a.queries)) * a.queries;
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
+    const int head = f.ok ? f.head : 0, cell0 = a.ncells / 2 - coord<MAP>(a, f.p);
+    const float* bias = a.bias ? a.bias + (long)head * a.pitch + cell0 : nullptr;
+    const ColFrag<T, L::P> vcol(sv);
 
     typename Vec<T>::v8 qf[D / 16], kf[D / 16];
     {
@@ -399,88 +441,80 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, sum = 0.f;
 
-    int end = a.causal ? min(s.len, s.off + min(i0 + a.queries, a.Lq)) : s.len;
+    const int end = a.causal ? min(s.len, s.off + min(i0 + a.queries, a.Lq)) : s.len;
     const int all = (max(end, 0) + FT - 1) / FT;
     const int t_begin = (int)((long)all * split / a.splits), t_end = (int)((long)all * (split + 1) / a.splits);
 
-    typename Vec<T>::v4 vr[D / 32][4];
+    constexpr int VE = 16 / sizeof(T), VR = D / VE, NV = FT * VR / 64;
+    uint4 vr[NV];
+    float br[16];
     unsigned live = 0, next_live = 0;
-    auto load = [&](int t) {
+    auto load_bias = [&](int t) {
         const int k0 = t * FT;
-        const int key = k0 + col;
-        bool ok = t < t_end && key < s.len;
+        if (MAP) {
+            wave_fence();
+            if (l < FT) s_u[w][l] = coord<MAP>(a, k0 + l);
+            wave_fence();
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            int4 x = {k0 + 8 * g + 4 * h, k0 + 8 * g + 4 * h + 1, k0 + 8 * g + 4 * h + 2, k0 + 8 * g + 4 * h + 3};
+            if (MAP) x = *reinterpret_cast<const int4*>(&s_u[w][8 * g + 4 * h]);
+            if (bias) {
+                // keys past the last lie in the biases' padding
+                br[4 * g] = bias[x.x]; br[4 * g + 1] = bias[x.y]; br[4 * g + 2] = bias[x.z]; br[4 * g + 3] = bias[x.w];
+            } else {
+                br[4 * g] = bias_at(a, cell0 + x.x, head); br[4 * g + 1] = bias_at(a, cell0 + x.y, head);
+                br[4 * g + 2] = bias_at(a, cell0 + x.z, head); br[4 * g + 3] = bias_at(a, cell0 + x.w, head);
+            }
+        }
+    };
+    auto load = [&](int t) {
+        const int k0 = t * FT, key = k0 + col;
+        bool ok = key < s.len;
         if (ok && a.kpm) ok = a.kpm[(long)b * a.Lk + key] == 0;
         next_live = (unsigned)__ballot(ok);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) kf[c] = frag_or_zero(kb + key * a.k_l + 16 * c + 8 * h, ok);
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-            const int id = l + 64 * x, dg = id % (D / 4), g = id / (D / 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                vr[x][j] = typename Vec<T>::v4{};
-                if ((next_live >> (4 * g + j)) & 1)
-                    vr[x][j] = *reinterpret_cast<const typename Vec<T>::v4*>(vb + (long)(k0 + 4 * g + j) * a.v_l + 4 * dg);
-            }
+        for (int x = 0; x < NV; ++x) {
+            const int id = l + 64 * x, row = id / VR;
+            vr[x] = make_uint4(0, 0, 0, 0);
+            if ((next_live >> row) & 1) vr[x] = *reinterpret_cast<const uint4*>(vb + (long)(k0 + row) * a.v_l + id % VR * VE);
         }
     };
-    load(t_begin + w);
+    if (t_begin + w < t_end) {
+        load_bias(t_begin + w);
+        load(t_begin + w);
+    }
     for (int t = t_begin + w; t < t_end; t += 4) {
         const int k0 = t * FT;
         live = next_live;
-        // offsets of a head's window: key - query from k0 - (p0 + queries - 1) on
-        for (int z = l; z < window; z += 64) {
-            const int gi = z / per, d = k0 - (s.off + i0 + a.queries - 1) + z % per, head = min(kvh * a.G + g0 + gi, a.H - 1);
-            win[z] = bias_at(a, 0, d, head);
-            if (MAP) win[window + z] = bias_at(a, 1, d, head);
+        f32x16 sc[1] = {f32x16{}};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) mma(kf[c], qf[c], sc[0]);
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+            const int id = l + 64 * x;
+            *reinterpret_cast<uint4*>(sv + id / VR * L::P + id % VR * VE) = vr[x];
         }
-        f32x16 sc = {};
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) mma(kf[c], qf[c], sc);
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-            const int id = l + 64 * x, dg = id % (D / 4), g = id / (D / 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<typename Vec<T>::v4*>(sv + (4 * dg + j) * L::CP + 4 * perm_group(g)) =
-                    typename Vec<T>::v4{vr[x][0][j], vr[x][1][j], vr[x][2][j], vr[x][3][j]};
-        }
-        load(t + 4);
-        wave_fence();
-        const int at = (col % a.heads) * per + a.queries - 1 - col / a.heads + 4 * h;     // rows past the last have no key
         const unsigned lv = live >> (4 * h);
-        float mx = m;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int j = 8 * (e >> 2) + (e & 3), key = k0 + j + 4 * h;
-            float bias = 0.f;
-            if (f.ok) {
-                bias = win[at + j];
-                if (MAP && key % a.width < f.px) bias = win[window + at + j];
-            }
-            sc[e] = ((lv >> j) & 1) && key <= f.last ? fmaf(sc[e], a.c, bias) : -INFINITY;
-            mx = fmaxf(mx, sc[e]);
+            const int j = 8 * (e >> 2) + (e & 3);
+            sc[0][e] = ((lv >> j) & 1) && k0 + j + 4 * h <= f.last ? fmaf(sc[0][e], a.c, br[e]) : -INFINITY;
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx != m)) {
-            const float x = __builtin_amdgcn_exp2f(m - ref);
-            sum *= x;
-#pragma unroll
-            for (int u = 0; u < D / 32; ++u) o[u] *= x;
-            m = mx;
+        if (t + 4 < t_end) {
+            load_bias(t + 4);
+            load(t + 4);
         }
-        const float low = ref - Vec<T>::SHIFT;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            sc[e] = __builtin_amdgcn_exp2f(sc[e] - low);
-            sum += sc[e];
-        }
+        softmax_step<T, 1, D / 32>(sc, m, sum, o);
+        wave_fence();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const typename Vec<T>::v8 pf = acc_frag<T>(sc, c);
+            const typename Vec<T>::v8 pf = acc_frag<T>(sc[0], c);
 #pragma unroll
-            for (int u = 0; u < D / 32; ++u) mma(frag<T>(sv + (32 * u + col) * L::CP + 16 * c + 8 * h), pf, o[u]);
+            for (int u = 0; u < D / 32; ++u) mma(vcol(16 * c, 32 * u), pf, o[u]);
         }
         wave_fence();
     }
@@ -520,7 +554,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
         for (int e = 0; e < 4; ++e)
             x[e] = (red[(d4 + e) * 33 + r] + red[(32 + d4 + e) * 33 + r]) + (red[(64 + d4 + e) * 33 + r] + red[(96 + d4 + e) * 33 + r]);
         if (fr.ok) {
-            if (a.splits == 1) few_store<T>(a, b, fr, D, 32 * u + d4, x, inv);
+            if (a.splits == 1) store_out<T>(a, (((long)b * a.Lq + fr.i) * a.H + fr.head) * D + 32 * u + d4, x, inv);
             else *reinterpret_cast<float4*>(a.few_o + (part * 32 + r) * D + 32 * u + d4) = make_float4(x[0], x[1], x[2], x[3]);
         }
         __syncthreads();
@@ -530,7 +564,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
             a.few_ml[(part * 32 + r) * 2] = top;
             a.few_ml[(part * 32 + r) * 2 + 1] = total;
         } else if (a.stats) {
-            few_stats<T>(a, b, fr, top, inv);
+            store_stats<T>(a, b, fr.head, fr.i, top, inv);
         }
     }
 }
@@ -560,26 +594,48 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int e = 0; e < D / 8; e += 4) few_store<T>(a, b, f, D, d0 + e, x + e, inv);
-    if (a.stats && d0 == 0) few_stats<T>(a, b, f, top, inv);
+    for (int e = 0; e < D / 8; e += 4) store_out<T>(a, (((long)b * a.Lq + f.i) * a.H + f.head) * D + d0 + e, x + e, inv);
+    if (a.stats && d0 == 0) store_stats<T>(a, b, f.head, f.i, top, inv);
 }
 
 // --- dQ and the sums along the offsets ------------------------------------------------------------------------------
-// The forward's split.  A wave adds dS into its own LDS window of offsets, one window per half of the wave: in one
-// instruction a half's 32 lanes hold 32 queries and one key, i.e. 32 different offsets, so no two lanes meet and the
-// sums have one order.  After each key tile the windows join the workgroup's running sums in wave order; offsets that
-// no later tile meets are written out.
+// The forward's split.  The table's gradient is the sum of dS along each offset key - query: a wave writes a 32x32 tile
+// of dS to its own LDS, row k turned by k places, so that a column holds one offset before the turn's end and one behind
+// it (t places back, and 32 - t on), and 64 lanes sum the 32 columns' halves.  The next key tile of the same wave goes on
+// with the latter at the same lanes: 32 finished sums are written per tile.  (LDS float additions by atomics, one per
+// element, took 145 cycles per wave instruction and 60 % of the kernel.)  On a map an offset stands for two different
+// column offsets, inside a row and around its end: two sets of sums.
+__device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 32; }
+__device__ __forceinline__ void offset_sums(const f32x16& x, float* lds, float& carry, float* out) {
+    const int l = threadIdx.x & 63, col = l & 31, h = l >> 5;
+    // element e of half h is row acc_row(e, h); physical rows 2 e + h: the halves write and read different banks
+#pragma unroll
+    for (int e = 0; e < 16; ++e) lds[(2 * e + h) * 32 + ((col - acc_row(e, h)) & 31)] = x[e];
+    wave_fence();
+    float before = 0.f, behind = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float v = lds[(2 * e + h) * 32 + col];
+        const bool wraps = acc_row(e, h) + col >= 32;
+        before += wraps ? 0.f : v;
+        behind += wraps ? v : 0.f;
+    }
+    wave_fence();
+    before += __shfl_xor(before, 32);
+    behind += __shfl_xor(behind, 32);
+    if (h == 0) out[31 - col] = before + carry;
+    carry = behind;
+}
+
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256) void dq_kernel(const Args a) {
+__global__ __launch_bounds__(256, 2) void dq_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
     constexpr int CLS = MAP ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) T sk[KT::ROW_ELEMS];
-    __shared__ __attribute__((aligned(16))) T skt[KT::COL_ELEMS];
-    __shared__ __attribute__((aligned(16))) T sv[KT::ROW_ELEMS];
-    __shared__ float sb[CLS][BM + BN];
-    __shared__ __attribute__((aligned(16))) int sx[BN];
-    __shared__ float win[4][2][CLS][96];
-    __shared__ float ring[CLS][256];
+    __shared__ __attribute__((aligned(16))) T sk[KT::ELEMS];
+    __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
+    __shared__ float sb[WindowLds<MAP>::N];
+    __shared__ __attribute__((aligned(16))) int su[BN], sx[BN];
+    __shared__ float turned[4][32 * 32];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
     place(a.B * a.Hkv, a.G * nq, unit, rest);
@@ -588,11 +644,15 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a) {
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
-    const int last = last_key(a, s, i), p = s.off + i;
-    const int px = MAP ? ((p % a.width) + a.width) % a.width : 0;
+    const int last = last_key(a, s, i);
+    const int u_hi = coord<MAP>(a, max(s.off + q0 + BM - 1, 0)), lane_u = u_hi - coord<MAP>(a, max(s.off + i, 0));
+    const int px = MAP ? max(s.off + i, 0) % a.width : 0;
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
+    const float* bias = a.bias + (long)head * a.pitch;
     const bool want = a.part != nullptr;
+    const int pitch = sum_pitch(a.Lk);
+    float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
 
     typename Vec<T>::v8 qf[D / 16], gf[D / 16];
     float m = 0.f, inv = 0.f, delta = 0.f;
@@ -624,94 +684,93 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a) {
     f32x16 dq[D / 32];
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) dq[t] = f32x16{};
-    if (want) {
-        for (int t = threadIdx.x; t < 4 * 2 * CLS * 96; t += 256) (&win[0][0][0][0])[t] = 0.f;
-        for (int t = threadIdx.x; t < CLS * 256; t += 256) (&ring[0][0])[t] = 0.f;
-    }
-    const int span = a.Lk + BM;                 // offsets of a workgroup, as a = j + BM - 1 - (query in workgroup)
-    float* part = want ? a.part + (((long)b * a.H + head) * nq + qblk) * CLS * span : nullptr;
-    int flushed = 0;
+    float carry[CLS] = {};
 
-    const int k_end = a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
+    const int k_end = key_end(a, s, q0);
+    const ColFrag<T, KT::P> kcol(sk);
+    KT tk, tv;
+    Window tw;
+    unsigned long long next = 0;
+    auto load = [&](int k0) {
+        next = live_keys(a, s, b, k0);
+        tk.load(kb + k0 * a.k_l, a.k_l, next);
+        tv.load(vb + k0 * a.v_l, a.v_l, next);
+        tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
+    };
+    if (k_end > 0) load(0);
     for (int k0 = 0; k0 < k_end; k0 += BN) {
-        const unsigned long long live = live_keys(a, s, b, k0);
-        KT tk, tv;
-        tk.load(kb + k0 * a.k_l, a.k_l, live);
-        tv.load(vb + k0 * a.v_l, a.v_l, live);
+        const unsigned long long live = next;
         __syncthreads();
-        tk.rows(sk);
-        tk.cols(skt);
-        tv.rows(sv);
-        const int d0 = k0 - (s.off + q0 + BM - 1);
-        for (int t = threadIdx.x; t < BM + BN - 1; t += 256) {
-            sb[0][t] = bias_at(a, 0, d0 + t, head);
-            if (MAP) sb[CLS - 1][t] = bias_at(a, 1, d0 + t, head);
+        tk.store(sk);
+        tv.store(sv);
+        tw.store(a, bias, sb, a.window);
+        if (MAP && threadIdx.x < BN) {
+            su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
+            sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
         }
-        if (MAP && threadIdx.x < BN) sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
         __syncthreads();
+        if (k0 + BN < k_end) load(k0 + BN);
 
-        const int lane_b = BM - 1 - (32 * w + col) + 4 * h;
         const unsigned long long lv = live >> (4 * h);
+        const bool masked = live != ~0ull || __any(last < k0 + BN - 1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
-                mma(frag<T>(sk + (32 * u + col) * KT::RP + 16 * c + 8 * h), qf[c], sc);
-                mma(frag<T>(sv + (32 * u + col) * KT::RP + 16 * c + 8 * h), gf[c], dp);
+                mma(frag<T>(sk + (32 * u + col) * KT::P + 16 * c + 8 * h), qf[c], sc);
+                mma(frag<T>(sv + (32 * u + col) * KT::P + 16 * c + 8 * h), gf[c], dp);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = 32 * u + 8 * (e >> 2) + (e & 3);
-                const bool far = MAP && sx[j + 4 * h] < px;
-                const float bias = sb[far ? CLS - 1 : 0][lane_b + j];
-                float pr = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, bias) - m) * inv;
-                if (!((lv >> j) & 1) || k0 + j + 4 * h > last) pr = 0.f;
-                dp[e] = pr * (dp[e] - delta);
-                if (want) atomicAdd(&win[w][h][far ? CLS - 1 : 0][j + 4 * h - col + 31], dp[e]);
+            for (int g = 0; g < 4; ++g) {
+                const int j = 32 * u + 8 * g;
+                int4 y = {};
+                if (MAP) y = *reinterpret_cast<const int4*>(su + j + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = lane_u + (MAP ? (e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w) : j + 4 * h + e);
+                    sc[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sc[4 * g + e], a.c, sb[at]) - m) * inv;
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 32 * u + 8 * (e >> 2) + (e & 3);
+                    if (!((lv >> j) & 1) || k0 + j + 4 * h > last) sc[e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = sc[e] * (dp[e] - delta);
+            if (want) {
+                if (MAP) {
+                    f32x16 around = {}, inside = dp;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int4 x = *reinterpret_cast<const int4*>(sx + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w) < px) {
+                                around[4 * g + e] = dp[4 * g + e];
+                                inside[4 * g + e] = 0.f;
+                            }
+                    }
+                    offset_sums(inside, turned[w], carry[0], part + k0 + 32 * u);
+                    offset_sums(around, turned[w], carry[CLS - 1], part + (CLS - 1) * pitch + k0 + 32 * u);
+                } else {
+                    offset_sums(dp, turned[w], carry[0], part + k0 + 32 * u);
+                }
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const typename Vec<T>::v8 df = acc_frag<T>(dp, c);
 #pragma unroll
-                for (int t = 0; t < D / 32; ++t) mma(frag<T>(skt + (32 * t + col) * KT::CP + 32 * u + 16 * c + 8 * h), df, dq[t]);
+                for (int t = 0; t < D / 32; ++t) mma(kcol(32 * u + 16 * c, 32 * t), df, dq[t]);
             }
         }
-        if (want) {
-            __syncthreads();
-            const int t = threadIdx.x;
-            if (t < BM + BN - 1) {
-#pragma unroll
-                for (int cls = 0; cls < CLS; ++cls) {
-                    float add = 0.f;
-#pragma unroll
-                    for (int ww = 0; ww < 4; ++ww) {
-                        const int at = t - 96 + 32 * ww;
-                        if (at >= 0 && at < 95) {
-                            add += win[ww][0][cls][at] + win[ww][1][cls][at];
-                        }
-                    }
-                    const int slot = (k0 + t) & 255;
-                    const float r = ring[cls][slot] + add;
-                    if (t < BN) {
-                        part[(long)cls * span + k0 + t] = r;
-                        ring[cls][slot] = 0.f;
-                    } else {
-                        ring[cls][slot] = r;
-                    }
-                }
-            }
-            __syncthreads();
-            for (int z = threadIdx.x; z < 4 * 2 * CLS * 96; z += 256) (&win[0][0][0][0])[z] = 0.f;
-            flushed = k0 + BN;
-        }
     }
-    if (want) {
-        __syncthreads();
-        for (int t = flushed + threadIdx.x; t < span; t += 256)
+    if (want && k_end > 0 && h == 0)
 #pragma unroll
-            for (int cls = 0; cls < CLS; ++cls) part[(long)cls * span + t] = t < flushed + BM - 1 ? ring[cls][t & 255] : 0.f;
-    }
+        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + 31 - col] = carry[cls];
     if (i >= a.Lq) return;
     T* out = static_cast<T*>(a.dq) + (((long)b * a.Lq + i) * a.H + head) * D;
 #pragma unroll
@@ -730,15 +789,14 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a) {
 // that share it stream through LDS, so the sums over those heads stay in the accumulators (no atomics, one order).
 // Keys sit on the lanes (S = Q K^T), P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
+__global__ __launch_bounds__(256, 2) void dkv_kernel(const Args a) {
+    constexpr int QB = D == 128 ? 32 : 64;      // queries per LDS tile
     typedef Tile<T, D, QB> QT;
-    __shared__ __attribute__((aligned(16))) T sq[QT::ROW_ELEMS];
-    __shared__ __attribute__((aligned(16))) T sqt[QT::COL_ELEMS];
-    __shared__ __attribute__((aligned(16))) T sg[QT::ROW_ELEMS];
-    __shared__ __attribute__((aligned(16))) T sgt[QT::COL_ELEMS];
-    __shared__ float sb[MAP ? 2 : 1][KB + QB];
+    __shared__ __attribute__((aligned(16))) T sq[QT::ELEMS];
+    __shared__ __attribute__((aligned(16))) T sg[QT::ELEMS];
+    __shared__ float sb[WindowLds<MAP>::N];
     __shared__ __attribute__((aligned(16))) float sm[QB], si[QB], sd[QB];
-    __shared__ __attribute__((aligned(16))) int sl[QB], sx[QB];
+    __shared__ __attribute__((aligned(16))) int sl[QB], su[QB];
     const int nk = (a.Lk + KB - 1) / KB;
     int unit, rest;
     place(a.B * a.Hkv, nk, unit, rest);
@@ -747,7 +805,7 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
     const Seq s = sequence(a, b);
     const int key = k0 + 32 * w + col;
     const bool alive = key < s.len && !(a.kpm && a.kpm[(long)b * a.Lk + key]);
-    const int kx = MAP ? key % a.width : 0;
+    const int u_lo = coord<MAP>(a, k0), lane_u = coord<MAP>(a, key) - u_lo;
 
     typename Vec<T>::v8 kf[D / 16], vf[D / 16];
     {
@@ -762,63 +820,93 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
     f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) dk[t] = dv[t] = f32x16{};
+    const ColFrag<T, QT::P> qcol(sq), gcol(sg);
 
     const int i_begin = k0 >= s.len ? a.Lq : a.causal ? max(0, (k0 - s.off) / QB * QB) : 0;
-    for (int g = 0; g < a.G; ++g) {
-        const int head = kvh * a.G + g;
-        const T* qb = static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h;
-        const T* gb = static_cast<const T*>(a.d_out) + ((long)b * a.Lq * a.H + head) * D;
-        for (int i0 = i_begin; i0 < a.Lq; i0 += QB) {
-            const unsigned long long rows = a.Lq - i0 >= QB ? 0xffffffffull : (1ull << (a.Lq - i0)) - 1;
-            QT tq, tg;
-            tq.load(qb + (long)i0 * a.q_l, a.q_l, rows);
-            tg.load(gb + (long)i0 * a.H * D, (long)a.H * D, rows);
-            __syncthreads();
-            tq.rows(sq);
-            tq.cols(sqt);
-            tg.rows(sg);
-            tg.cols(sgt);
-            const int d0 = k0 - (s.off + i0 + QB - 1);
-            for (int t = threadIdx.x; t < KB + QB - 1; t += 256) {
-                sb[0][t] = bias_at(a, 0, d0 + t, head);
-                if (MAP) sb[MAP ? 1 : 0][t] = bias_at(a, 1, d0 + t, head);
-            }
-            if (threadIdx.x < QB) {
-                const int t = threadIdx.x, i = i0 + t, p = s.off + i;
-                const long st = ((long)b * a.H + head) * a.Lq + i;
-                const bool ok = i < a.Lq;
-                sm[t] = ok ? a.stats[2 * st] : 0.f;
-                si[t] = ok ? a.stats[2 * st + 1] * up<T>() : 0.f;
-                sd[t] = ok ? a.delta[st] * down<T>() : 0.f;
-                sl[t] = last_key(a, s, i);
-                if (MAP) sx[t] = ((p % a.width) + a.width) % a.width;
-            }
-            __syncthreads();
-
+    const int blocks = i_begin < a.Lq ? (a.Lq - i_begin + QB - 1) / QB : 0, steps = blocks * a.G;
+    QT tq, tg;
+    Window tw;
+    float rm = 0.f, ri = 0.f, rd = 0.f;
+    int rl = -1, ru = 0;
+    // step n: query block n % blocks of head n / blocks
+    auto load = [&](int n) {
+        const int head = kvh * a.G + n / blocks, i0 = i_begin + n % blocks * QB;
+        const unsigned long long rows = a.Lq - i0 >= 64 ? ~0ull : (1ull << (a.Lq - i0)) - 1;
+        tq.load(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, rows);
+        tg.load(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, rows);
+        const int u_hi = coord<MAP>(a, max(s.off + i0 + QB - 1, 0));
+        tw.load(a, a.bias + (long)head * a.pitch, u_lo - u_hi + a.ncells / 2, a.window);
+        if (threadIdx.x < QB) {
+            const int i = i0 + threadIdx.x;
+            const long st = ((long)b * a.H + head) * a.Lq + i;
+            const bool ok = i < a.Lq;
+            rm = ok ? a.stats[2 * st] : 0.f;
+            ri = ok ? a.stats[2 * st + 1] * up<T>() : 0.f;
+            rd = ok ? a.delta[st] * down<T>() : 0.f;
+            rl = last_key(a, s, i);
+            ru = u_hi - coord<MAP>(a, max(s.off + i, 0));
+        }
+    };
+    if (steps > 0) load(0);
+    for (int n = 0; n < steps; ++n) {
+        __syncthreads();
+        tq.store(sq);
+        tg.store(sg);
+        tw.store(a, a.bias + (long)(kvh * a.G + n / blocks) * a.pitch, sb, a.window);
+        if (threadIdx.x < QB) {
+            sm[threadIdx.x] = rm;
+            si[threadIdx.x] = ri;
+            sd[threadIdx.x] = rd;
+            sl[threadIdx.x] = rl;
+            su[threadIdx.x] = ru;
+        }
+        __syncthreads();
+        // rows that see not all of this workgroup's keys: behind the last query, out of the buckets, causal
+        const bool masked = __any(!alive) || __any(sl[l & (QB - 1)] < k0 + KB - 1);
+        if (n + 1 < steps) load(n + 1);
+#pragma unroll
+        for (int u = 0; u < QB / 32; ++u) {
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
-                mma(frag<T>(sq + col * QT::RP + 16 * c + 8 * h), kf[c], sc);
-                mma(frag<T>(sg + col * QT::RP + 16 * c + 8 * h), vf[c], dp);
+                mma(frag<T>(sq + (32 * u + col) * QT::P + 16 * c + 8 * h), kf[c], sc);
+                mma(frag<T>(sg + (32 * u + col) * QT::P + 16 * c + 8 * h), vf[c], dp);
             }
-            const int lane_b = 32 * w + col + QB - 1 - 4 * h;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = 8 * (e >> 2) + (e & 3), r = j + 4 * h;
-                const bool far = MAP && kx < sx[r];
-                const float bias = sb[far && MAP ? 1 : 0][lane_b - j];
-                float pr = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, bias) - sm[r]) * si[r];
-                if (!alive || key > sl[r]) pr = 0.f;
-                sc[e] = pr;
-                dp[e] = pr * fmaf(dp[e], down<T>(), -sd[r]);
+            for (int g = 0; g < 4; ++g) {
+                const int r = 32 * u + 8 * g + 4 * h;
+                const float4 m4 = *reinterpret_cast<const float4*>(sm + r), i4 = *reinterpret_cast<const float4*>(si + r);
+                const float4 d4 = *reinterpret_cast<const float4*>(sd + r);
+                const float m_[4] = {m4.x, m4.y, m4.z, m4.w}, i_[4] = {i4.x, i4.y, i4.z, i4.w}, d_[4] = {d4.x, d4.y, d4.z, d4.w};
+                int at[4];
+                if (MAP) {
+                    const int4 y = *reinterpret_cast<const int4*>(su + r);
+                    at[0] = lane_u + y.x; at[1] = lane_u + y.y; at[2] = lane_u + y.z; at[3] = lane_u + y.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) at[e] = lane_u + QB - 1 - r - e;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = 4 * g + e;
+                    sc[x] = __builtin_amdgcn_exp2f(fmaf(sc[x], a.c, sb[at[e]]) - m_[e]) * i_[e];
+                    dp[x] = fmaf(dp[x], down<T>(), -d_[e]);
+                }
             }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!alive || key > sl[32 * u + acc_row(e, h)]) sc[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] *= sc[e];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const typename Vec<T>::v8 pf = acc_frag<T>(sc, c), df = acc_frag<T>(dp, c);
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t) {
-                    mma(frag<T>(sgt + (32 * t + col) * QT::CP + 16 * c + 8 * h), pf, dv[t]);
-                    mma(frag<T>(sqt + (32 * t + col) * QT::CP + 16 * c + 8 * h), df, dk[t]);
+                    mma(gcol(32 * u + 16 * c, 32 * t), pf, dv[t]);
+                    mma(qcol(32 * u + 16 * c, 32 * t), df, dk[t]);
                 }
             }
         }
@@ -850,8 +938,7 @@ int launch_f16(int what, int D, const Args& a, unsigned grid, hipStream_t stream
 
 template <class T, int D, bool MAP> void launch_one(int what, const Args& a, unsigned grid, hipStream_t stream) {
     if (what == FWD) fwd_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
-    else if (what == FEW)
-        few_kernel<T, D, MAP><<<grid, 256, FewLds<T, D>::BYTES + 16 * few_window(a.heads, a.queries) * (MAP ? 2 : 1), stream>>>(a);
+    else if (what == FEW) few_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
     else if (what == MERGE) merge_kernel<T, D><<<grid, 256, 0, stream>>>(a);
     else if (what == DQ) dq_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
     else dkv_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);

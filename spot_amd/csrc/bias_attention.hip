@@ -5,23 +5,44 @@
 
 namespace ba {
 
-// Sums of dS along each (class, offset) cell over sequences and query blocks.  One thread per cell; the partial sums of
-// a workgroup lie at a = delta + BM - 1 + offset_b + BM * block.  At most BM terms are in each partial sum (32 bits);
-// from here on the sums are 64 bits.
-__global__ __launch_bounds__(256) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
-    const int n = 2 * a.N - 1, i = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y, cls = blockIdx.z, ncls = gridDim.z;
-    if (i >= n) return;
-    const int nq = (a.Lq + BM - 1) / BM, span = a.Lk + BM, delta = i - (a.N - 1);
+static_assert(MAXW == SPOT_BIAS_ATTN_MAX_WIDTH, "the windows are made for this width");
+
+// The table spread out by offset, times log2 e: bias[head][u(key) - u(query) + u(N - 1)].
+__global__ __launch_bounds__(256) void spread_kernel(const Args a) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < a.pitch) a.bias[(long)blockIdx.y * a.pitch + i] = i < a.ncells ? bias_at(a, i, blockIdx.y) : 0.f;
+}
+
+// Sums of dS along each offset over sequences and queries.  A wave of the dQ kernel has left its sums for keys
+// - queries = delta at delta + p0 + 31, where p0 is the position of its first query: at most 32 terms each, in 32 bits;
+// from here on the sums are 64 bits.  16 waves per 64 offsets, wave z the blocks z, z + 16, ...
+__global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
+    __shared__ double red[16][64];
+    const int l = threadIdx.x & 63, z = threadIdx.x >> 6, head = blockIdx.y, cls = blockIdx.z, ncls = gridDim.z;
+    const int i = blockIdx.x * 64 + l, delta = i - (a.N - 1);
+    const int nw = (a.Lq + BM - 1) / BM * 4, pitch = sum_pitch(a.Lk);
     double sum = 0.;
     for (int b = 0; b < a.B; ++b) {
         const Seq s = sequence(a, b);
-        const float* part = a.part + (((long)b * a.H + head) * nq * ncls + cls) * span;
-        for (int q = 0; q < nq; ++q) {
-            const int at = delta + BM - 1 + s.off + q * BM;
-            if (at >= 0 && at < span) sum += part[(long)q * ncls * span + at];
+        const float* part = a.part + (((long)b * a.H + head) * nw * ncls + cls) * pitch;
+        for (int w = z; w < nw; w += 16) {
+            const int end = key_end(a, s, w / 4 * BM), at = delta + s.off + 32 * w + 31;
+            if (end > 0 && at >= 0 && at < (end + BN - 1) / BN * BN + 32) sum += part[(long)w * ncls * pitch + at];
         }
     }
-    sums[((long)head * ncls + cls) * n + i] = sum;
+    red[z][l] = sum;
+    __syncthreads();
+    if (z != 0 || i >= 2 * a.N - 1) return;
+    for (int y = 1; y < 16; ++y) sum += red[y][l];
+    // on a map: the cell of this offset inside a row, or around its end; every cell has one such pair
+    int cell = i;
+    if (a.width) {
+        const int W = a.width, x = ((delta % W) + W) % W - (cls ? W : 0), y = (delta - x) / W;
+        if (x <= -W) return;
+        cell = y * (2 * W - 1) + x + a.ncells / 2;
+        if ((unsigned)cell >= (unsigned)a.ncells) return;
+    }
+    sums[(long)head * a.ncells + cell] = sum;
 }
 
 // One wave per (bucket, head): the cells of a bucket stand together in `order`.
@@ -50,22 +71,29 @@ static int launch_any(int dtype, int what, int D, const Args& a, unsigned grid, 
                                                                                : launch_f16(what, D, a, grid, stream);
 }
 
-// Backward workspace in bytes: sums along offsets (64 bits) | delta | partial sums along offsets.
-struct Layout { long sums, delta, part, total; };
+// Backward workspace in bytes: sums by cell (64 bits) | delta | spread-out biases | sums along offsets.
+static long up16(long n) { return (n + 15) & ~15L; }
+static int cells_of(const spot_bias_attn_desc& d) {
+    const int last = d.max_len - 1;
+    return 2 * (d.width ? last / d.width * (2 * d.width - 1) + last % d.width : last) + 1;
+}
+static int pitch_of(const spot_bias_attn_desc& d) { return (cells_of(d) + PADB + (d.width ? window_span(FT, d.width) : 0) + 63) / 64 * 64; }
+struct Layout { long sums, delta, bias, part, total; };
 static Layout layout(const spot_bias_attn_desc& d) {
-    const long cls = d.width > 0 ? 2 : 1, nq = (d.Lq + BM - 1) / BM;
+    const long cls = d.width > 0 ? 2 : 1, nw = (d.Lq + BM - 1) / BM * 4, pitch = ((long)d.Lk + BN - 1) / BN * BN + 32;
     Layout l;
     l.sums = 0;
-    l.delta = d.dtable ? l.sums + 8 * (long)d.H * cls * (2L * d.max_len - 1) : 0;
-    l.part = l.delta + ((4L * d.B * d.H * d.Lq + 15) & ~15L);
-    l.total = l.part + (d.dtable ? 4 * (long)d.B * d.H * nq * cls * ((long)d.Lk + BM) : 0);
+    l.delta = d.dtable ? up16(8 * (long)d.H * cells_of(d)) : 0;
+    l.bias = l.delta + up16(4L * d.B * d.H * d.Lq);
+    l.part = l.bias + 4L * d.H * pitch_of(d);
+    l.total = l.part + (d.dtable ? 4 * (long)d.B * d.H * nw * cls * pitch : 0);
     return l;
 }
 
 // The forward's kernel.  few_kernel reads keys once for all heads that share them and cuts the keys between its waves and
 // workgroups; fwd_kernel reads them once per 128 queries.  The former is taken for up to 32 rows per key/value head, and
 // where the latter's workgroups would not fill the 256 CUs.
-struct Few { bool use; int heads, queries, tiles, splits; long o, ml; };
+struct Few { bool use, spread; int heads, queries, tiles, splits; long o, ml, bias; };
 static Few few(const spot_bias_attn_desc& d) {
     Few f = {};
     const int G = d.H / d.Hkv;
@@ -82,6 +110,9 @@ static Few few(const spot_bias_attn_desc& d) {
         f.o = units * f.splits * 32 * d.head_dim * 4;
         f.ml = units * f.splits * 32 * 2 * 4;
     }
+    // biases by bucket are two dependent loads per score; spread out they are one, after a launch of a few microseconds
+    f.spread = !f.use || d.Lk / (4 * FT * f.splits) >= 4;
+    f.bias = f.spread ? 4L * d.H * pitch_of(d) : 0;
     return f;
 }
 
@@ -98,7 +129,8 @@ static int check(const spot_bias_attn_desc* d, bool backward) {
     SPOT_CHECK_ARG(d->max_len >= 1 && d->max_len <= SPOT_BIAS_ATTN_MAX_LEN && d->Lk <= d->max_len && d->Lq <= SPOT_BIAS_ATTN_MAX_LEN,
                    "spot_bias_attention: max_len %d for %d keys and %d queries (1 to %d, no fewer than the keys)", d->max_len, d->Lk,
                    d->Lq, SPOT_BIAS_ATTN_MAX_LEN);
-    SPOT_CHECK_ARG(d->num_buckets >= 1 && d->width >= 0, "spot_bias_attention: %d buckets, width %d", d->num_buckets, d->width);
+    SPOT_CHECK_ARG(d->num_buckets >= 1 && d->width >= 0 && d->width <= SPOT_BIAS_ATTN_MAX_WIDTH,
+                   "spot_bias_attention: %d buckets, width %d (0 to %d)", d->num_buckets, d->width, SPOT_BIAS_ATTN_MAX_WIDTH);
     SPOT_CHECK_ARG(d->q_offset_mode >= 0 && d->q_offset_mode <= 2 && (d->q_offset_mode != 1 || d->q_offsets),
                    "spot_bias_attention: q_offset_mode %d", d->q_offset_mode);
     SPOT_CHECK_ARG(d->q_offset_mode != 0 || (d->q_offset >= 0 && (long)d->q_offset + d->Lq <= d->max_len),
@@ -137,6 +169,7 @@ static Args arguments(const spot_bias_attn_desc& d) {
     a.v_b = d.v_stride_b; a.v_l = d.v_stride_l; a.v_h = d.v_stride_h;
     a.B = d.B; a.H = d.H; a.Hkv = d.Hkv; a.G = d.H / d.Hkv; a.Lq = d.Lq; a.Lk = d.Lk; a.N = d.max_len; a.width = d.width;
     a.nb = d.num_buckets; a.causal = d.causal != 0; a.off_mode = d.q_offset_mode; a.off = d.q_offset; a.table_type = d.table_dtype;
+    a.ncells = cells_of(d); a.pitch = pitch_of(d); a.window = window_of(BN, BM, d.width);
     a.scale = d.scale; a.c = d.scale * LOG2E;
     return a;
 }
@@ -150,9 +183,15 @@ extern "C" int spot_bias_attention_fwd(const spot_bias_attn_desc* desc, hipStrea
     if (d.B == 0 || d.Lq == 0) return SPOT_OK;
     Args a = arguments(d);
     const Few f = few(d);
+    const long need = f.o + f.ml + f.bias;
+    SPOT_CHECK_ARG(need == 0 || (d.ws && aligned16(d.ws) && d.ws_bytes >= need),
+                   "spot_bias_attention_fwd: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", need, d.ws_bytes);
+    if (f.spread) {
+        a.bias = reinterpret_cast<float*>(static_cast<char*>(d.ws) + f.o + f.ml);
+        spread_kernel<<<dim3((a.pitch + 255) / 256, d.H), 256, 0, stream>>>(a);
+        SPOT_CHECK_LAUNCH("spot_bias_attention_fwd");
+    }
     if (!f.use) return launch_any(d.dtype, FWD, d.head_dim, a, (unsigned)d.B * d.H * ((d.Lq + BM - 1) / BM), stream);
-    SPOT_CHECK_ARG(f.splits == 1 || (d.ws && aligned16(d.ws) && d.ws_bytes >= f.o + f.ml),
-                   "spot_bias_attention_fwd: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", f.o + f.ml, d.ws_bytes);
     a.heads = f.heads; a.queries = f.queries; a.tiles = f.tiles; a.splits = f.splits;
     a.few_o = static_cast<float*>(d.ws);
     a.few_ml = a.few_o + f.o / 4;
@@ -166,7 +205,7 @@ extern "C" int spot_bias_attention_fwd_ws_bytes(const spot_bias_attn_desc* desc,
     if (const int rc = check(desc, false)) return rc;
     SPOT_CHECK_ARG(bytes != nullptr, "spot_bias_attention_fwd_ws_bytes: null pointer");
     const Few f = few(*desc);
-    *bytes = f.use && desc->Lq > 0 ? f.o + f.ml : 0;
+    *bytes = desc->B > 0 && desc->Lq > 0 ? f.o + f.ml + f.bias : 0;
     return SPOT_OK;
 }
 
@@ -188,18 +227,22 @@ extern "C" int spot_bias_attention_bwd(const spot_bias_attn_desc* desc, hipStrea
                    "spot_bias_attention_bwd: a 16-byte aligned workspace of %ld bytes is needed, %ld are given", l.total, d.ws_bytes);
     char* ws = static_cast<char*>(d.ws);
     a.delta = reinterpret_cast<float*>(ws + l.delta);
+    a.bias = reinterpret_cast<float*>(ws + l.bias);
     a.part = d.dtable ? reinterpret_cast<float*>(ws + l.part) : nullptr;
+    double* sums = reinterpret_cast<double*>(ws + l.sums);
+    if (d.B > 0) {
+        spread_kernel<<<dim3((a.pitch + 255) / 256, d.H), 256, 0, stream>>>(a);
+        SPOT_CHECK_LAUNCH("spot_bias_attention_bwd");
+    }
     if (d.B > 0 && d.Lq > 0)
         if (const int rc = launch_any(d.dtype, DQ, d.head_dim, a, (unsigned)d.B * d.H * ((d.Lq + BM - 1) / BM), stream)) return rc;
     if (d.B > 0 && d.dk && d.Lk > 0)
         if (const int rc = launch_any(d.dtype, DKV, d.head_dim, a, (unsigned)d.B * d.Hkv * ((d.Lk + KB - 1) / KB), stream)) return rc;
     if (d.dtable) {
-        const int cls = d.width > 0 ? 2 : 1, n = 2 * d.max_len - 1;
-        double* sums = reinterpret_cast<double*>(ws + l.sums);
-        offset_sums_kernel<<<dim3((n + 255) / 256, d.H, cls), 256, 0, stream>>>(a, sums);
+        offset_sums_kernel<<<dim3((2 * d.max_len - 1 + 63) / 64, d.H, d.width ? 2 : 1), 1024, 0, stream>>>(a, sums);
         SPOT_CHECK_LAUNCH("spot_bias_attention_bwd");
         bucket_sums_kernel<<<dim3((d.num_buckets + 3) / 4, d.H), 256, 0, stream>>>(sums, d.cell_order, d.cell_start, d.dtable,
-                                                                               d.table_dtype, d.num_buckets, d.H, cls * n);
+                                                                               d.table_dtype, d.num_buckets, d.H, a.ncells);
         SPOT_CHECK_LAUNCH("spot_bias_attention_bwd");
     }
     return SPOT_OK;

@@ -1973,28 +1973,31 @@ _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 class RelativeBuckets:
     """Which bucket each relative position of a key to a query has: what bias_attention looks a bias up by.
 
-    ``cells[delta + max_len - 1]`` is the bucket of a key ``delta`` places behind the query (delta < 0: before it), for
-    sequences of up to ``max_len`` positions.  On a map of ``width`` columns (positions row by row) ``cells`` has two
-    rows: the first for keys whose column is not left of the query's, the second for those left of it, so that an entry
-    stands for one (row offset, column offset).  Build it once per model: it also holds, for the gradient, the cells
-    sorted by bucket."""
+    For sequences of up to ``max_len`` positions ``cells[key - query + max_len - 1]`` is the bucket.  On a map of
+    ``width`` columns (up to 512; positions row by row) position p has the coordinate u(p) = p // width * (2 width - 1)
+    + p % width, and cells[u(key) - u(query) + u(max_len - 1)] is the bucket: an entry stands for one (row offset, column
+    offset).  Build it once per model: it also holds, for the gradient, the cells sorted by bucket."""
 
-    def __init__(self, cells, num_buckets, width=0, device="cuda"):
+    def __init__(self, cells, num_buckets, max_len, width=0, device="cuda"):
         cells = torch.as_tensor(cells, dtype=torch.int64, device="cpu")
-        cells = cells.reshape(1, -1) if cells.dim() == 1 else cells
-        if cells.dim() != 2 or cells.shape[0] != (2 if width else 1) or cells.shape[1] % 2 != 1:
-            raise RuntimeError("spot_amd: bucket cells of shape %s: [2 max_len - 1], or with a width [2, 2 max_len - 1]"
-                               % (tuple(cells.shape),))
-        if width < 0 or num_buckets < 1 or int(cells.min()) < 0 or int(cells.max()) >= num_buckets:
-            raise RuntimeError("spot_amd: width %d, bucket cells from %d to %d for %d buckets"
-                               % (width, int(cells.min()), int(cells.max()), num_buckets))
-        self.num_buckets, self.width, self.max_len = int(num_buckets), int(width), (cells.shape[1] + 1) // 2
-        flat = cells.reshape(-1)
+        last = max_len - 1
+        n = 2 * (last // width * (2 * width - 1) + last % width if width > 0 else last) + 1
+        if not 0 <= width <= 512 or not 1 <= max_len <= 1 << 20 or tuple(cells.shape) != (n,):
+            raise RuntimeError("spot_amd: bucket cells of shape %s for %d positions, width %d (0 to 512): [%d]"
+                               % (tuple(cells.shape), max_len, width, n))
+        if num_buckets < 1 or int(cells.min()) < 0 or int(cells.max()) >= num_buckets:
+            raise RuntimeError("spot_amd: bucket cells from %d to %d for %d buckets" % (int(cells.min()), int(cells.max()), num_buckets))
+        self.num_buckets, self.width, self.max_len = int(num_buckets), int(width), int(max_len)
         start = torch.zeros(num_buckets + 1, dtype=torch.int64)
-        start[1:] = torch.bincount(flat, minlength=num_buckets).cumsum(0)
-        self.cells = cells.to(torch.int32).to(device)
-        self.order = torch.argsort(flat, stable=True).to(torch.int32).to(device)
-        self.start = start.to(torch.int32).to(device)
+        start[1:] = torch.bincount(cells, minlength=num_buckets).cumsum(0)
+        # one copy to the device: cells | order | start, each at a border of 16 bytes
+        up = lambda m: (m + 3) // 4 * 4
+        packed = torch.zeros(2 * up(n) + num_buckets + 1, dtype=torch.int32)
+        packed[:n] = cells
+        packed[up(n):up(n) + n] = torch.argsort(cells, stable=True)
+        packed[2 * up(n):] = start
+        packed = packed.to(device)
+        self.cells, self.order, self.start = packed[:n], packed[up(n):up(n) + n], packed[2 * up(n):]
 
 
 def sequence_buckets(max_len, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
@@ -2017,7 +2020,7 @@ def sequence_buckets(max_len, num_buckets=32, max_distance=128, bidirectional=Tr
     d = torch.arange(max_len)
     before = torch.where(d < near, d, near + torch.bucketize(d, torch.tensor(borders, dtype=torch.int64), right=True))
     behind = before + buckets if bidirectional else torch.zeros_like(before)
-    return RelativeBuckets(torch.cat([before.flip(0), behind[1:]]), num_buckets, 0, device)
+    return RelativeBuckets(torch.cat([before.flip(0), behind[1:]]), num_buckets, max_len, 0, device)
 
 
 def grid_buckets(height, width, device="cuda"):
@@ -2025,13 +2028,9 @@ def grid_buckets(height, width, device="cuda"):
     (dy + height - 1) * (2 width - 1) + dx + width - 1."""
     if height < 1 or width < 1:
         raise RuntimeError("spot_amd: grid_buckets of a %d x %d map" % (height, width))
-    n = height * width
-    delta = torch.arange(1 - n, n)
-    dx = torch.stack([delta % width, delta % width - width])
-    dy = torch.div(delta - dx, width, rounding_mode="floor")
-    # offsets that no pair of the map has: any bucket
-    dx, dy = dx.clamp(1 - width, width - 1), dy.clamp(1 - height, height - 1)
-    return RelativeBuckets((dy + height - 1) * (2 * width - 1) + dx + width - 1, (2 * height - 1) * (2 * width - 1), width, device)
+    # u runs over whole rows of 2 width - 1 column offsets, from (1 - height, 1 - width) on: the bucket is the cell
+    n = (2 * height - 1) * (2 * width - 1)
+    return RelativeBuckets(torch.arange(n), n, height * width, width, device)
 
 
 class _on:

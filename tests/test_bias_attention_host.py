@@ -8,7 +8,7 @@ import torch
 def test_sequence_buckets():
     from spot_amd import ops
     b = ops.sequence_buckets(300, 32, 128, device="cpu")
-    cells = b.cells[0].tolist()
+    cells = b.cells.tolist()
     at = lambda d: cells[d + 299]
     assert [at(-n) for n in range(8)] == list(range(8)) and [at(n) for n in range(1, 8)] == [16 + n for n in range(1, 8)]
     # half 16 buckets, 8 of them exact; the others double every two: 8, 11.3, 16, 22.6, 32, 45.3, 64, 90.5
@@ -16,9 +16,9 @@ def test_sequence_buckets():
                       (64, 14), (90, 14), (91, 15), (128, 15), (299, 15)):
         assert at(-n) == bucket and at(n) == 16 + bucket, n
     one = ops.sequence_buckets(300, 32, 128, bidirectional=False, device="cpu")
-    cells = one.cells[0].tolist()
+    cells = one.cells.tolist()
     assert set(cells[300:]) == {0} and cells[299 - 15] == 15 and cells[299 - 16] == 16 and cells[0] == 31
-    assert ops.sequence_buckets(1, 4, 8, device="cpu").cells.shape == (1, 1)
+    assert ops.sequence_buckets(1, 4, 8, device="cpu").cells.shape == (1,)
 
 
 @pytest.mark.parametrize("h,w", [(1, 1), (1, 6), (6, 1), (4, 5), (7, 3)])
@@ -27,11 +27,12 @@ def test_grid_buckets(h, w):
     b = ops.grid_buckets(h, w, device="cpu")
     n = h * w
     assert b.max_len == n and b.width == w and b.num_buckets == (2 * h - 1) * (2 * w - 1)
+    u = lambda p: p // w * (2 * w - 1) + p % w
     for q in range(n):
         for k in range(n):
             dy, dx = k // w - q // w, k % w - q % w
-            assert b.cells[int(dx < 0), k - q + n - 1] == (dy + h - 1) * (2 * w - 1) + dx + w - 1
-    flat = b.cells.reshape(-1)
+            assert b.cells[u(k) - u(q) + u(n - 1)] == (dy + h - 1) * (2 * w - 1) + dx + w - 1
+    flat = b.cells
     assert torch.equal(flat[b.order.long()], flat.sort().values)
     for i in range(b.num_buckets):
         assert (flat[b.order[b.start[i]:b.start[i + 1]].long()] == i).all()
@@ -40,10 +41,11 @@ def test_grid_buckets(h, w):
 
 def test_bucket_plans_refuse():
     from spot_amd import ops
-    for cells, nb, width in (([0, 1], 2, 0), ([0, 2, 1], 2, 0), ([0, -1, 1], 2, 0), ([0, 1, 0], 2, 3), ([[0, 1, 0]], 2, 3),
-                             ([[0, 1, 0]] * 2, 2, 0), ([0], 0, 0), ([[[0]]], 1, 0)):
+    for cells, nb, n, width in (([0, 1], 2, 1, 0), ([0, 2, 1], 2, 2, 0), ([0, -1, 1], 2, 2, 0), ([0, 1, 0], 2, 3, 0), ([[0, 1, 0]], 2, 2, 0),
+                                ([0] * 9, 2, 5, 2), ([0], 0, 1, 0), ([0], 1, 0, 0), ([0], 1, 1, 513), ([0], 1, 1, -1)):
         with pytest.raises(RuntimeError, match="spot_amd"):
-            ops.RelativeBuckets(cells, nb, width, device="cpu")
+            ops.RelativeBuckets(cells, nb, n, width, device="cpu")
+    assert ops.RelativeBuckets([0, 1, 0, 1, 1, 0, 1, 0, 1], 2, 4, 2, device="cpu").cells.tolist() == [0, 1, 0, 1, 1, 0, 1, 0, 1]
     for args in ((0, 32, 128), (10, 2, 128), (10, 32, 8), (10, 0, 128)):
         with pytest.raises(RuntimeError, match="spot_amd"):
             ops.sequence_buckets(*args, device="cpu")
@@ -66,7 +68,7 @@ def _desc(**kw):
 
 @pytest.mark.parametrize("field,value", [
     ("dtype", 3), ("dtype", -1), ("table_dtype", 5), ("head_dim", 48), ("Hkv", 3), ("Hkv", 0), ("B", -1), ("Lk", 33), ("max_len", 0),
-    ("max_len", (1 << 20) + 1), ("num_buckets", 0), ("width", -1), ("q_offset", -1), ("q_offset", 25), ("q_offset_mode", 1),
+    ("max_len", (1 << 20) + 1), ("num_buckets", 0), ("width", -1), ("width", 513), ("q_offset", -1), ("q_offset", 25), ("q_offset_mode", 1),
     ("q_offset_mode", 3), ("q", None), ("k", None), ("out", None), ("table", None), ("cells", None), ("q", 4100), ("v", 4104),
     ("q_stride_l", 130), ("k_stride_b", 2), ("v_stride_h", 1), ("Lq", (1 << 20) + 1)])
 def test_forward_refuses_bad_descriptors(field, value):
@@ -80,9 +82,9 @@ def test_backward_refuses():
     from spot_amd import lib
     l = lib.load()
     n = C.c_long(-1)
-    assert l.spot_bias_attention_bwd_ws_bytes(C.byref(_desc()), C.byref(n)) == 0 and n.value == 4 * 2 * 4 * 8
-    for kw in ({"stats": None}, {"d_out": None}, {"dq": None}, {"dk": None}, {"dtable": 4096}, {"d_out": 4100}, {}, {"ws": 4096, "ws_bytes": 255},
-               {"ws": 4100, "ws_bytes": 256}):
+    assert l.spot_bias_attention_bwd_ws_bytes(C.byref(_desc()), C.byref(n)) == 0 and n.value > 0
+    for kw in ({"stats": None}, {"d_out": None}, {"dq": None}, {"dk": None}, {"dtable": 4096}, {"d_out": 4100}, {}, {"ws": 4096, "ws_bytes": n.value - 1},
+               {"ws": 4100, "ws_bytes": n.value}):
         rc = l.spot_bias_attention_bwd(C.byref(_desc(**kw)), None)
         assert rc < 0 and b"spot_bias_attention" in l.spot_last_error(), kw
     assert l.spot_bias_attention_fwd(None, None) < 0 and l.spot_bias_attention_bwd(None, None) < 0

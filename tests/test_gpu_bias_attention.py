@@ -45,9 +45,9 @@ def reference(q, k, v, table, cells, width, max_len, causal, off, kv_len, kpm, s
     seen = live[:, None] & (p >= 0) & (p < max_len)
     if causal:
         seen = seen & (j <= p)
-    delta = (j - p).clamp(1 - max_len, max_len - 1)
-    cls = (j % width < p % width).long() if width else torch.zeros_like(delta)
-    bucket = cells.long().reshape(-1, 2 * max_len - 1)[cls, delta + max_len - 1]
+    coord = lambda x: torch.div(x, width, rounding_mode="floor") * (2 * width - 1) + x % width if width else x
+    here = p.clamp(0, max_len - 1)
+    bucket = cells.long()[coord(j) - coord(here) + cells.numel() // 2]
     bias = table.double()[bucket].permute(0, 3, 1, 2)
     raw = Q @ K.transpose(2, 3) * scale
     S = (raw + bias).masked_fill(~seen[:, None], -math.inf)
@@ -248,7 +248,7 @@ def test_bias_that_masks(ops, t):
         out = ops.bias_attention(q, k, v, table, b)
         got = (out, *torch.autograd.grad(out, (q, k, v, table), g))
         p = torch.arange(40, device=DEV)
-        bucket = b.cells[0].long()[(p[None] - p[:, None]) + 39]
+        bucket = b.cells.long()[(p[None] - p[:, None]) + 39]
         leaf = [x.detach().double().requires_grad_() for x in (q, k, v, table)]
         S = torch.einsum("bihd,bjhd->bhij", leaf[0], leaf[1]) / math.sqrt(32) + leaf[3][bucket].permute(2, 0, 1)[None]
         if low == -math.inf:
