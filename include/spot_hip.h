@@ -663,7 +663,7 @@ int spot_top_logits(int dtype, const void* logits, long ld, int N, int V, int k,
  * index outside of 0 .. V - 1 or the value -inf are absent; a row without any has loss and gradient 0.  An index that
  * is listed twice counts twice.  student [N, V] of dtype, rows ld elements apart; values [N, k] of values_dtype (0 f32,
  * 1 bf16, 2 f16), indices [N, k].
- * Forward: loss [N], and for the backward norm [N, 2] and p [N, k].  ws: spot_top_distill_ws_bytes bytes, 16-byte
+ * Forward: loss [N], and for the backward norm [N, 2] and p [N, k] (both NULL: no backward follows).  ws: spot_top_distill_ws_bytes bytes, 16-byte
  * aligned.  Backward: d_student [N, V] dense, of the student's dtype, from d_loss [N]. */
 int spot_top_distill_ws_bytes(int dtype, int N, int V, int k, long* bytes /* host */);
 int spot_top_distill_fwd(int dtype, const void* student, long ld, int values_dtype, const void* values, const int* indices, int N,

@@ -30,7 +30,7 @@ namespace ba {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int BM = 128;     // queries per workgroup of the forward and dQ kernels: 32 per wave
 constexpr int BN = 64;      // keys per LDS tile there
-constexpr int KB = 128;     // keys per workgroup of the dK / dV kernel: 32 per wave
+constexpr int KB = 64;      // keys per workgroup of the dK / dV kernel: 32 per pair of waves
 constexpr int MAXW = 512;   // columns of a map
 constexpr int PADB = 64;    // entries behind the last of a head's spread-out biases
 
@@ -49,6 +49,14 @@ struct Args {               // strides in elements; out, d_out, dq, dk, dv are d
 };
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
+enum { FWD, FEW, MERGE, DQ, DKV };          // kernels
+
+// Waves per SIMD that the registers are cut for: as many as fit without spilling.
+template <class T, int D> constexpr int waves_of(int kernel) {
+    const int words = D * (int)sizeof(T) / 64;      // 1, 2, 4 for 16-bit heads of 32, 64, 128 channels; twice that in f32
+    return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 1 ? 3 : words <= 2 ? 2 : 1)
+                                                                                 : (words <= 1 ? 3 : words <= 2 ? 2 : 1);
+}
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <class T> struct Vec {
@@ -148,8 +156,13 @@ __device__ __forceinline__ unsigned long long live_keys(const Args& a, const Seq
 }
 
 // --- bias ---------------------------------------------------------------------------------------------------------
-// log2 e * table[cells[i]][head].  Scores live in the log2 domain; a finite entry stays finite there (the type's lowest
-// value as a mask must not turn into -inf, which hides a key altogether).
+// Scores live in the log2 domain; a finite entry stays finite there (the type's lowest value as a mask must not turn into
+// -inf, which hides a key altogether).
+__device__ __forceinline__ float log2_bias(float t) {
+    const float r = t * LOG2E;
+    return fabsf(t) <= FLT_MAX ? fminf(fmaxf(r, -FLT_MAX), FLT_MAX) : r;
+}
+// log2 e * table[cells[i]][head]
 __device__ __forceinline__ float bias_at(const Args& a, int i, int head) {
     if ((unsigned)i >= (unsigned)a.ncells) return 0.f;
     const int bucket = a.cells[i];
@@ -158,8 +171,7 @@ __device__ __forceinline__ float bias_at(const Args& a, int i, int head) {
     const float t = a.table_type == F32 ? static_cast<const float*>(a.table)[at]
                   : a.table_type == BF16 ? (float)static_cast<const __bf16*>(a.table)[at]
                                          : (float)static_cast<const _Float16*>(a.table)[at];
-    const float r = t * LOG2E;
-    return fabsf(t) <= FLT_MAX ? fminf(fmaxf(r, -FLT_MAX), FLT_MAX) : r;
+    return log2_bias(t);
 }
 
 // Window of a head's biases from cell i0 on, by 256 threads; the first 512 entries travel in registers while the tile
@@ -211,16 +223,12 @@ template <class T, int D, int ROWS> struct Tile {
 };
 
 // Workgroup -> (sequence, key/value head, rest).  Consecutive workgroups go to the eight XCDs in turn; where the number
-// of key/value heads allows it, all workgroups that read the same keys and values share one XCD's L2.
-__device__ __forceinline__ void place(int units, int per_unit, int& unit, int& rest) {
-    const int id = blockIdx.x;
-    if (units % 8 == 0) {
-        unit = (id >> 3) / per_unit * 8 + (id & 7);
-        rest = (id >> 3) % per_unit;
-    } else {
-        unit = id / per_unit;
-        rest = id % per_unit;
-    }
+// of key/value heads allows it, all workgroups that read the same keys and values share one XCD's L2.  `longest`: the
+// workgroups of small `rest` take longest and start first, whatever their head (causal attention).
+__device__ __forceinline__ void place(int units, int per_unit, bool longest, int& unit, int& rest) {
+    const int id = blockIdx.x, xcds = units % 8 == 0 ? 8 : 1, j = id / xcds, here = units / xcds;
+    unit = (longest ? j % here : j / per_unit) * xcds + id % xcds;
+    rest = longest ? j / here : j % per_unit;
 }
 
 // The softmax step of a lane's row: the scores of NT tiles become 2^(s - reference + SHIFT), the sums are scaled where
@@ -273,7 +281,7 @@ template <class T> __device__ __forceinline__ void store_stats(const Args& a, in
 // One workgroup: 128 queries of one head, 32 per wave; keys stream through LDS in tiles of 64, the next one in flight in
 // registers.  Queries sit on the lanes (S^T = K Q^T), so reference and sum are one number per lane.
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256, 2) void fwd_kernel(const Args a) {
+__global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
     __shared__ __attribute__((aligned(16))) T sk[KT::ELEMS];
     __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
@@ -281,9 +289,9 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const Args a) {
     __shared__ __attribute__((aligned(16))) int su[BN];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
-    place(a.B * a.Hkv, a.G * nq, unit, rest);
-    const int b = unit / a.Hkv, kvh = unit % a.Hkv, head = kvh * a.G + rest / nq;
-    const int q0 = (a.causal ? nq - 1 - rest % nq : rest % nq) * BM;      // causal: the long rows first
+    place(a.B * a.Hkv, a.G * nq, a.causal, unit, rest);
+    const int b = unit / a.Hkv, kvh = unit % a.Hkv, head = kvh * a.G + rest % a.G;
+    const int q0 = (a.causal ? nq - 1 - rest / a.G : rest / a.G) * BM;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
@@ -417,7 +425,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     __shared__ __attribute__((aligned(16))) char lds[L::BYTES];
     __shared__ __attribute__((aligned(16))) int s_u[4][FT];
     int unit, rest;
-    place(a.B * a.Hkv, a.tiles * a.splits, unit, rest);
+    place(a.B * a.Hkv, a.tiles * a.splits, false, unit, rest);
     const int b = unit / a.Hkv, kvh = unit % a.Hkv, tile = rest / a.splits, split = rest % a.splits;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const Seq s = sequence(a, b);
@@ -448,8 +456,11 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     constexpr int VE = 16 / sizeof(T), VR = D / VE, NV = FT * VR / 64;
     uint4 vr[NV];
     float br[16];
+    int cell[16];
     unsigned live = 0, next_live = 0;
-    auto load_bias = [&](int t) {
+    // first: the cells of a tile's scores, and the biases where they are spread out; then the others by their buckets.
+    // Rows and keys that the buckets do not reach are hidden: any entry does for them.
+    auto find_bias = [&](int t) {
         const int k0 = t * FT;
         if (MAP) {
             wave_fence();
@@ -464,9 +475,23 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
                 // keys past the last lie in the biases' padding
                 br[4 * g] = bias[x.x]; br[4 * g + 1] = bias[x.y]; br[4 * g + 2] = bias[x.z]; br[4 * g + 3] = bias[x.w];
             } else {
-                br[4 * g] = bias_at(a, cell0 + x.x, head); br[4 * g + 1] = bias_at(a, cell0 + x.y, head);
-                br[4 * g + 2] = bias_at(a, cell0 + x.z, head); br[4 * g + 3] = bias_at(a, cell0 + x.w, head);
+                cell[4 * g] = a.cells[min(cell0 + x.x, a.ncells - 1)]; cell[4 * g + 1] = a.cells[min(cell0 + x.y, a.ncells - 1)];
+                cell[4 * g + 2] = a.cells[min(cell0 + x.z, a.ncells - 1)]; cell[4 * g + 3] = a.cells[min(cell0 + x.w, a.ncells - 1)];
             }
+        }
+    };
+    auto load_bias = [&]() {
+        if (bias) return;
+        const unsigned top = a.nb - 1;
+        if (a.table_type == F32) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) br[e] = static_cast<const float*>(a.table)[(long)min((unsigned)cell[e], top) * a.H + head];
+        } else if (a.table_type == BF16) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) br[e] = (float)static_cast<const __bf16*>(a.table)[(long)min((unsigned)cell[e], top) * a.H + head];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) br[e] = (float)static_cast<const _Float16*>(a.table)[(long)min((unsigned)cell[e], top) * a.H + head];
         }
     };
     auto load = [&](int t) {
@@ -484,13 +509,18 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
         }
     };
     if (t_begin + w < t_end) {
-        load_bias(t_begin + w);
+        find_bias(t_begin + w);
         load(t_begin + w);
+        load_bias();
     }
     for (int t = t_begin + w; t < t_end; t += 4) {
         const int k0 = t * FT;
         live = next_live;
         f32x16 sc[1] = {f32x16{}};
+        if (!bias) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) br[e] = log2_bias(br[e]);
+        }
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) mma(kf[c], qf[c], sc[0]);
 #pragma unroll
@@ -505,8 +535,9 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
             sc[0][e] = ((lv >> j) & 1) && k0 + j + 4 * h <= f.last ? fmaf(sc[0][e], a.c, br[e]) : -INFINITY;
         }
         if (t + 4 < t_end) {
-            load_bias(t + 4);
+            find_bias(t + 4);
             load(t + 4);
+            load_bias();
         }
         softmax_step<T, 1, D / 32>(sc, m, sum, o);
         wave_fence();
@@ -628,7 +659,7 @@ __device__ __forceinline__ void offset_sums(const f32x16& x, float* lds, float& 
 }
 
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256, 2) void dq_kernel(const Args a) {
+__global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
     constexpr int CLS = MAP ? 2 : 1;
     __shared__ __attribute__((aligned(16))) T sk[KT::ELEMS];
@@ -638,9 +669,9 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a) {
     __shared__ float turned[4][32 * 32];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
-    place(a.B * a.Hkv, a.G * nq, unit, rest);
-    const int b = unit / a.Hkv, kvh = unit % a.Hkv, head = kvh * a.G + rest / nq;
-    const int qblk = a.causal ? nq - 1 - rest % nq : rest % nq, q0 = qblk * BM;
+    place(a.B * a.Hkv, a.G * nq, a.causal, unit, rest);
+    const int b = unit / a.Hkv, kvh = unit % a.Hkv, head = kvh * a.G + rest % a.G;
+    const int qblk = a.causal ? nq - 1 - rest / a.G : rest / a.G, q0 = qblk * BM;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
@@ -785,25 +816,32 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a) {
 }
 
 // --- dK, dV ---------------------------------------------------------------------------------------------------------
-// One workgroup: 128 keys of one key/value head, 32 per wave, their K and V held in registers; the queries of all heads
-// that share it stream through LDS, so the sums over those heads stay in the accumulators (no atomics, one order).
-// Keys sit on the lanes (S = Q K^T), P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers; the queries of all
+// heads that share it stream through LDS 64 at a time, 32 for each wave of a pair, so the sums over those heads stay in
+// the accumulators (no atomics, one order) and the pair joins at the end.  Keys sit on the lanes (S = Q K^T), P and dS
+// are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+template <class T, int D> struct DkvLds {
+    typedef Tile<T, D, 64> QT;
+    static constexpr int TILES = 2 * QT::ELEMS * (int)sizeof(T), JOIN = 2 * 64 * 16 * 4;
+    static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
+};
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256, 2) void dkv_kernel(const Args a) {
-    constexpr int QB = D == 128 ? 32 : 64;      // queries per LDS tile
+__global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const Args a) {
+    constexpr int QB = 64;                      // queries per LDS tile
     typedef Tile<T, D, QB> QT;
-    __shared__ __attribute__((aligned(16))) T sq[QT::ELEMS];
-    __shared__ __attribute__((aligned(16))) T sg[QT::ELEMS];
+    __shared__ __attribute__((aligned(16))) char lds[DkvLds<T, D>::BYTES];
     __shared__ float sb[WindowLds<MAP>::N];
     __shared__ __attribute__((aligned(16))) float sm[QB], si[QB], sd[QB];
     __shared__ __attribute__((aligned(16))) int sl[QB], su[QB];
+    T* sq = reinterpret_cast<T*>(lds);
+    T* sg = sq + QT::ELEMS;
     const int nk = (a.Lk + KB - 1) / KB;
     int unit, rest;
-    place(a.B * a.Hkv, nk, unit, rest);
+    place(a.B * a.Hkv, nk, a.causal, unit, rest);
     const int b = unit / a.Hkv, kvh = unit % a.Hkv, k0 = rest * KB;
-    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5, u = w >> 1;
     const Seq s = sequence(a, b);
-    const int key = k0 + 32 * w + col;
+    const int key = k0 + 32 * (w & 1) + col;
     const bool alive = key < s.len && !(a.kpm && a.kpm[(long)b * a.Lk + key]);
     const int u_lo = coord<MAP>(a, k0), lane_u = coord<MAP>(a, key) - u_lo;
 
@@ -861,77 +899,80 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(const Args a) {
             su[threadIdx.x] = ru;
         }
         __syncthreads();
-        // rows that see not all of this workgroup's keys: behind the last query, out of the buckets, causal
-        const bool masked = __any(!alive) || __any(sl[l & (QB - 1)] < k0 + KB - 1);
         if (n + 1 < steps) load(n + 1);
+        // rows that see not all of this workgroup's keys: behind the last query, out of the buckets, causal
+        const bool masked = __any(!alive) || __any(sl[32 * u + col] < k0 + KB - 1);
+        f32x16 sc = {}, dp = {};
 #pragma unroll
-        for (int u = 0; u < QB / 32; ++u) {
-            f32x16 sc = {}, dp = {};
+        for (int c = 0; c < D / 16; ++c) {
+            mma(frag<T>(sq + (32 * u + col) * QT::P + 16 * c + 8 * h), kf[c], sc);
+            mma(frag<T>(sg + (32 * u + col) * QT::P + 16 * c + 8 * h), vf[c], dp);
+        }
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                mma(frag<T>(sq + (32 * u + col) * QT::P + 16 * c + 8 * h), kf[c], sc);
-                mma(frag<T>(sg + (32 * u + col) * QT::P + 16 * c + 8 * h), vf[c], dp);
+        for (int g = 0; g < 4; ++g) {
+            const int r = 32 * u + 8 * g + 4 * h;
+            const float4 m4 = *reinterpret_cast<const float4*>(sm + r), i4 = *reinterpret_cast<const float4*>(si + r);
+            const float4 d4 = *reinterpret_cast<const float4*>(sd + r);
+            const float m_[4] = {m4.x, m4.y, m4.z, m4.w}, i_[4] = {i4.x, i4.y, i4.z, i4.w}, d_[4] = {d4.x, d4.y, d4.z, d4.w};
+            int at[4];
+            if (MAP) {
+                const int4 y = *reinterpret_cast<const int4*>(su + r);
+                at[0] = lane_u + y.x; at[1] = lane_u + y.y; at[2] = lane_u + y.z; at[3] = lane_u + y.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) at[e] = lane_u + QB - 1 - r - e;
             }
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int r = 32 * u + 8 * g + 4 * h;
-                const float4 m4 = *reinterpret_cast<const float4*>(sm + r), i4 = *reinterpret_cast<const float4*>(si + r);
-                const float4 d4 = *reinterpret_cast<const float4*>(sd + r);
-                const float m_[4] = {m4.x, m4.y, m4.z, m4.w}, i_[4] = {i4.x, i4.y, i4.z, i4.w}, d_[4] = {d4.x, d4.y, d4.z, d4.w};
-                int at[4];
-                if (MAP) {
-                    const int4 y = *reinterpret_cast<const int4*>(su + r);
-                    at[0] = lane_u + y.x; at[1] = lane_u + y.y; at[2] = lane_u + y.z; at[3] = lane_u + y.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) at[e] = lane_u + QB - 1 - r - e;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int x = 4 * g + e;
-                    sc[x] = __builtin_amdgcn_exp2f(fmaf(sc[x], a.c, sb[at[e]]) - m_[e]) * i_[e];
-                    dp[x] = fmaf(dp[x], down<T>(), -d_[e]);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int x = 4 * g + e;
+                sc[x] = __builtin_amdgcn_exp2f(fmaf(sc[x], a.c, sb[at[e]]) - m_[e]) * i_[e];
+                dp[x] = fmaf(dp[x], down<T>(), -d_[e]);
             }
-            if (masked) {
+        }
+        if (masked) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!alive || key > sl[32 * u + acc_row(e, h)]) sc[e] = 0.f;
-            }
+            for (int e = 0; e < 16; ++e)
+                if (!alive || key > sl[32 * u + acc_row(e, h)]) sc[e] = 0.f;
+        }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] *= sc[e];
+        for (int e = 0; e < 16; ++e) dp[e] *= sc[e];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const typename Vec<T>::v8 pf = acc_frag<T>(sc, c), df = acc_frag<T>(dp, c);
+        for (int c = 0; c < 2; ++c) {
+            const typename Vec<T>::v8 pf = acc_frag<T>(sc, c), df = acc_frag<T>(dp, c);
 #pragma unroll
-                for (int t = 0; t < D / 32; ++t) {
-                    mma(gcol(32 * u + 16 * c, 32 * t), pf, dv[t]);
-                    mma(qcol(32 * u + 16 * c, 32 * t), df, dk[t]);
-                }
+            for (int t = 0; t < D / 32; ++t) {
+                mma(gcol(32 * u + 16 * c, 32 * t), pf, dv[t]);
+                mma(qcol(32 * u + 16 * c, 32 * t), df, dk[t]);
             }
         }
     }
-    if (key >= a.Lk) return;
+    // the pair's sums, one 32-channel block at a time: the second wave's go through LDS to the first
+    float* join = reinterpret_cast<float*>(lds) + (w & 1) * 64 * 16 + l;
     const long row = (((long)b * a.Lk + key) * a.Hkv + kvh) * D;
-    T* ok = static_cast<T*>(a.dk) + row;
-    T* ov = static_cast<T*>(a.dv) + row;
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
+    for (int t = 0; t < 2 * (D / 32); ++t) {
+        f32x16& acc = t < D / 32 ? dk[t % (D / 32)] : dv[t % (D / 32)];
+        __syncthreads();
+        if (u == 1) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            typename Vec<T>::v4 x, y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = (T)(dk[t][4 * g + e] * a.scale);
-                y[e] = (T)(dv[t][4 * g + e] * down<T>());
-            }
-            *reinterpret_cast<typename Vec<T>::v4*>(ok + 32 * t + 8 * g + 4 * h) = x;
-            *reinterpret_cast<typename Vec<T>::v4*>(ov + 32 * t + 8 * g + 4 * h) = y;
+            for (int e = 0; e < 16; ++e) join[64 * e] = acc[e];
         }
+        __syncthreads();
+        if (u == 0 && key < a.Lk) {
+            T* out = static_cast<T*>(t < D / 32 ? a.dk : a.dv) + row + 32 * (t % (D / 32)) + 4 * h;
+            const float f = t < D / 32 ? a.scale : down<T>();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                typename Vec<T>::v4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (T)((acc[4 * g + e] + join[64 * (4 * g + e)]) * f);
+                *reinterpret_cast<typename Vec<T>::v4*>(out + 8 * g) = x;
+            }
+        }
+    }
 }
 
 // What the host part launches, one set per element type.
-enum { FWD, FEW, MERGE, DQ, DKV };
 int launch_f32(int what, int D, const Args& a, unsigned grid, hipStream_t stream);
 int launch_bf16(int what, int D, const Args& a, unsigned grid, hipStream_t stream);
 int launch_f16(int what, int D, const Args& a, unsigned grid, hipStream_t stream);

@@ -15,19 +15,26 @@ __global__ __launch_bounds__(256) void spread_kernel(const Args a) {
 
 // Sums of dS along each offset over sequences and queries.  A wave of the dQ kernel has left its sums for keys
 // - queries = delta at delta + p0 + 31, where p0 is the position of its first query: at most 32 terms each, in 32 bits;
-// from here on the sums are 64 bits.  16 waves per 64 offsets, wave z the blocks z, z + 16, ...
+// from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 4, ... and of
+// each the blocks z / 4, ...
 __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
     __shared__ double red[16][64];
     const int l = threadIdx.x & 63, z = threadIdx.x >> 6, head = blockIdx.y, cls = blockIdx.z, ncls = gridDim.z;
     const int i = blockIdx.x * 64 + l, delta = i - (a.N - 1);
     const int nw = (a.Lq + BM - 1) / BM * 4, pitch = sum_pitch(a.Lk);
     double sum = 0.;
-    for (int b = 0; b < a.B; ++b) {
+    const long step = (long)ncls * pitch;
+    for (int b = z & 3; b < a.B; b += 4) {
         const Seq s = sequence(a, b);
+        // where this offset lies in the first wave's sums; a wave further it is 32 further.  Places outside of a wave's
+        // sums are read at their border and not added: loads without a branch overlap.
+        const int at = delta + s.off + 31;
         const float* part = a.part + (((long)b * a.H + head) * nw * ncls + cls) * pitch;
-        for (int w = z; w < nw; w += 16) {
-            const int end = key_end(a, s, w / 4 * BM), at = delta + s.off + 32 * w + 31;
-            if (end > 0 && at >= 0 && at < (end + BN - 1) / BN * BN + 32) sum += part[(long)w * ncls * pitch + at];
+#pragma unroll 8
+        for (int w = z >> 2; w < nw; w += 4) {
+            const int end = key_end(a, s, w / 4 * BM), len = end > 0 ? (end + BN - 1) / BN * BN + 32 : 0, x = at + 32 * w;
+            const float v = part[w * step + min(max(x, 0), pitch - 1)];
+            sum += (unsigned)x < (unsigned)len ? v : 0.f;
         }
     }
     red[z][l] = sum;
@@ -45,21 +52,29 @@ __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double*
     sums[(long)head * a.ncells + cell] = sum;
 }
 
-// One wave per (bucket, head): the cells of a bucket stand together in `order`.
+// LANES threads per (bucket, head): the cells of a bucket stand together in `order`.
+template <int LANES>
 __global__ __launch_bounds__(256) void bucket_sums_kernel(const double* __restrict__ sums, const int* __restrict__ order,
                                                           const int* __restrict__ start, void* __restrict__ dtable,
                                                           int table_type, int nb, int H, int cells) {
-    const int bucket = blockIdx.x * 4 + (threadIdx.x >> 6), head = blockIdx.y;
-    if (bucket >= nb) return;
+    __shared__ double red[4];
+    const int bucket = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, head = blockIdx.y, t = threadIdx.x % LANES;
+    const bool ok = bucket < nb;
     double sum = 0.;
-    const int end = min(start[bucket + 1], cells);
-    for (int z = max(start[bucket], 0) + (threadIdx.x & 63); z < end; z += 64) {
+    const int end = ok ? min(start[bucket + 1], cells) : 0;
+#pragma unroll 4
+    for (int z = (ok ? max(start[bucket], 0) : 0) + t; z < end; z += LANES) {
         const int cell = order[z];
         if ((unsigned)cell < (unsigned)cells) sum += sums[(long)head * cells + cell];
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if ((threadIdx.x & 63) != 0) return;
+    for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        sum = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    if (!ok || t != 0) return;
     const long at = (long)bucket * H + head;
     if (table_type == F32) static_cast<float*>(dtable)[at] = (float)sum;
     else if (table_type == BF16) static_cast<__bf16*>(dtable)[at] = (__bf16)(float)sum;
@@ -241,8 +256,13 @@ extern "C" int spot_bias_attention_bwd(const spot_bias_attn_desc* desc, hipStrea
     if (d.dtable) {
         offset_sums_kernel<<<dim3((2 * d.max_len - 1 + 63) / 64, d.H, d.width ? 2 : 1), 1024, 0, stream>>>(a, sums);
         SPOT_CHECK_LAUNCH("spot_bias_attention_bwd");
-        bucket_sums_kernel<<<dim3((d.num_buckets + 3) / 4, d.H), 256, 0, stream>>>(sums, d.cell_order, d.cell_start, d.dtable,
-                                                                               d.table_dtype, d.num_buckets, d.H, a.ncells);
+        // a map has a cell per bucket, a sequence thousands for the far ones
+        if (a.ncells / d.num_buckets < 16)
+            bucket_sums_kernel<4><<<dim3((d.num_buckets + 63) / 64, d.H), 256, 0, stream>>>(sums, d.cell_order, d.cell_start, d.dtable,
+                                                                                      d.table_dtype, d.num_buckets, d.H, a.ncells);
+        else
+            bucket_sums_kernel<256><<<dim3(d.num_buckets, d.H), 256, 0, stream>>>(sums, d.cell_order, d.cell_start, d.dtable,
+                                                                              d.table_dtype, d.num_buckets, d.H, a.ncells);
         SPOT_CHECK_LAUNCH("spot_bias_attention_bwd");
     }
     return SPOT_OK;

@@ -339,10 +339,11 @@ template <class T> __device__ void row_loss(const Distill& a, long row, Norm z, 
         const float lq = fmaf((float)x[at], a.c, -z.m) - logl;
         if (p != 0.f) term = p * ((t - tn.m - logt) - lq);
     }
-    if (i < a.k) a.p[row * a.k + i] = p;
+    if (i < a.k && a.p) a.p[row * a.k + i] = p;
     const float sum = block_add(term, red_f);
     if (i == 0) {
         a.loss[row] = none ? 0.f : a.T * a.T * LN2 * sum;
+        if (!a.norm) return;
         a.norm[2 * row] = z.m;
         a.norm[2 * row + 1] = none ? 0.f : 1.f / z.l;
     }
@@ -486,7 +487,7 @@ extern "C" int spot_top_distill_fwd(int dtype, const void* student, long ld, int
                    values_dtype);
     SPOT_CHECK_ARG(temperature > 0.f && temperature <= FLT_MAX, "spot_top_distill_fwd: temperature %g", temperature);
     if (N == 0) return SPOT_OK;
-    SPOT_CHECK_ARG(student && values && indices && loss && norm && p, "spot_top_distill_fwd: null pointer");
+    SPOT_CHECK_ARG(student && values && indices && loss && (norm != nullptr) == (p != nullptr), "spot_top_distill_fwd: null pointer");
     Distill a = {};
     a.student = student; a.values = values; a.indices = indices; a.ld = ld; a.N = N; a.V = V; a.k = k;
     a.pieces = distill_pieces(N, V);

@@ -6,7 +6,9 @@ forward and backward kernels together so that the host modules (fusion.py,
 transt.py) read like the reference's nn.Modules.
 """
 import ctypes as C
+import functools
 import math
+import struct
 
 import torch
 
@@ -2038,7 +2040,7 @@ class _on:
     __slots__ = ("guard",)
 
     def __init__(self, t):
-        i = t.device.index
+        i = t.get_device()
         here = _current_device() if _current_device is not None else torch.cuda.current_device()
         self.guard = torch.cuda.device(i) if i != here else None
 
@@ -2052,12 +2054,14 @@ class _on:
 
 
 def _aligned16(t):
-    """t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes, else a copy."""
-    es = t.element_size()
-    if t.data_ptr() % 16 == 0 and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])) \
-            and (t.shape[-1] == 1 or t.stride(-1) == 1):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes, else a copy; and
+    the strides of the others in elements (0 for dimensions of length one, whose stride says nothing)."""
+    es, strides = t.element_size(), t.stride()
+    strides = [x if n > 1 else 0 for n, x in zip(t.shape, strides)]
+    if strides[-1] != 1 or t.data_ptr() % 16 or any(x * es % 16 for x in strides[:-1]):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides[:-1]
 
 
 def _dense16(t):
@@ -2065,27 +2069,26 @@ def _dense16(t):
 
 
 def _check_bias_attention(q, k, v, table, buckets, q_offset, kv_len, key_padding_mask):
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (table, "table")):
+    where, dtype = q.get_device(), q.dtype            # -1: not on a GPU
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (table, "table"), (buckets.cells, "buckets")):
         if not t.is_cuda:
             raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
-        if t.device != q.device:
+        if t.get_device() != where:
             raise RuntimeError("spot_amd: %s is on %s, q on %s" % (name, t.device, q.device))
-        if t.dtype not in _DTYPE_CODE or (name != "table" and t.dtype != q.dtype):
-            raise RuntimeError("spot_amd: %s is %s: q, k and v have one dtype of float32, bfloat16, float16, the table one of these"
-                               % (name, t.dtype))
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise RuntimeError("spot_amd: q %s, k %s, v %s: [B, Lq, H, D] and twice [B, Lk, Hkv, D]"
-                           % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    B, Lq, H, D = q.shape
-    Lk, Hkv = k.shape[1], k.shape[2]
+    if dtype not in _DTYPE_CODE or k.dtype != dtype or v.dtype != dtype or table.dtype not in _DTYPE_CODE:
+        raise RuntimeError("spot_amd: q, k and v have one dtype of float32, bfloat16, float16, the table one of these; got %s, %s, %s, %s"
+                           % (dtype, k.dtype, v.dtype, table.dtype))
+    sq, sk = q.shape, k.shape
+    if len(sq) != 4 or len(sk) != 4 or v.shape != sk or sk[0] != sq[0] or sk[3] != sq[3]:
+        raise RuntimeError("spot_amd: q %s, k %s, v %s: [B, Lq, H, D] and twice [B, Lk, Hkv, D]" % (tuple(sq), tuple(sk), tuple(v.shape)))
+    B, Lq, H, D = sq
+    Lk, Hkv = sk[1], sk[2]
     if D not in (32, 64, 128):
         raise RuntimeError("spot_amd: bias_attention is built for heads of 32, 64 or 128 channels, not %d" % D)
     if Hkv == 0 or H == 0 or H % Hkv:
         raise RuntimeError("spot_amd: %d query heads over %d key/value heads" % (H, Hkv))
-    if tuple(table.shape) != (buckets.num_buckets, H):
+    if table.shape != (buckets.num_buckets, H):
         raise RuntimeError("spot_amd: table %s for %d buckets and %d heads" % (tuple(table.shape), buckets.num_buckets, H))
-    if buckets.cells.device != q.device:
-        raise RuntimeError("spot_amd: buckets are on %s, q on %s" % (buckets.cells.device, q.device))
     if Lk > buckets.max_len:
         raise RuntimeError("spot_amd: %d keys, but the buckets end at %d positions" % (Lk, buckets.max_len))
     if torch.is_tensor(q_offset):
@@ -2108,80 +2111,87 @@ def _check_per_sequence(t, B, q, name):
         raise RuntimeError("spot_amd: %s must be an int32 tensor [%d] on %s" % (name, B, q.device))
 
 
+# the descriptor as one record: 19 pointers, ws_bytes and nine strides, fourteen numbers, scale
+_BIAS_DESC = struct.Struct("@19P10l14if4x")
+
+
+def _bias_desc(pointers, strides, numbers, scale, ws=0, ws_bytes=0):
+    return lib.BiasAttnDesc.from_buffer_copy(_BIAS_DESC.pack(*pointers, ws, ws_bytes, *strides, *numbers, scale))
+
+
+@functools.lru_cache(maxsize=1024)
+def _bias_ws_bytes(query, numbers, with_table):
+    """Workspace of a call of these sizes (the library's answer depends on them alone)."""
+    p = 4096           # the size asks for no data: any address that is not null
+    d = _bias_desc((p,) * 4 + (0,) * 2 + (p,) * 2 + (p if numbers[12] == 1 else 0,) + (0,) * 6 + (p if with_table else 0,) + (p,) * 2, (0,) * 9,
+                   numbers, 1.0)
+    need = C.c_long(0)
+    lib.check(getattr(lib.load(), query)(C.byref(d), C.byref(need)), query)
+    return need.value
+
+
 def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, train):
-    """-> out, out_lo, stats, and the descriptor with the tensors whose addresses it holds."""
-    q, k, v = _aligned16(q), _aligned16(k), _aligned16(v)
+    """-> out, out_lo, stats, (strides, numbers, scale) of the descriptor, and the tensors it addresses."""
+    (q, qs), (k, ks), (v, vs) = _aligned16(q), _aligned16(k), _aligned16(v)
     table = table if table.is_contiguous() else table.contiguous()
-    off_t = q_offset.contiguous() if torch.is_tensor(q_offset) else None
+    B, Lq, H, D = q.shape
+    off_t, mode, off = (q_offset.contiguous(), 1, 0) if torch.is_tensor(q_offset) else (None, 2, 0) if q_offset == "end" else \
+        (None, 0, int(q_offset))
     kv_len = kv_len.contiguous() if kv_len is not None else None
     kpm = key_padding_mask.contiguous() if key_padding_mask is not None else None
-    B, Lq, H, D = q.shape
+    code = _DTYPE_CODE[q.dtype]
+    numbers = (code, _DTYPE_CODE[table.dtype], B, Lq, k.shape[1], H, k.shape[2], D, buckets.num_buckets, buckets.max_len,
+               buckets.width, 1 if causal else 0, mode, off)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    strides = (*qs, *ks, *vs)
     out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    out_lo = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    out_lo = torch.empty_like(out) if train and code else None
     stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device) if train else None
-    ptr = lambda t: None if t is None else t.data_ptr()
-    d = lib.BiasAttnDesc(
-        ptr(q), ptr(k), ptr(v), ptr(out), ptr(out_lo), ptr(stats), ptr(table), ptr(buckets.cells), ptr(off_t), ptr(kv_len), ptr(kpm),
-        None, None, None, None, None, ptr(buckets.order), ptr(buckets.start), None, 0,
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-        _DTYPE_CODE[q.dtype], _DTYPE_CODE[table.dtype], B, Lq, k.shape[1], H, k.shape[2], D, buckets.num_buckets, buckets.max_len,
-        buckets.width, int(bool(causal)), 1 if off_t is not None else 2 if q_offset == "end" else 0,
-        0 if off_t is not None or q_offset == "end" else int(q_offset), 1.0 / math.sqrt(D) if scale is None else float(scale))
-    # strides of dimensions of length one say nothing
-    if B == 1:
-        d.q_stride_b = d.k_stride_b = d.v_stride_b = 0
-    if Lq == 1:
-        d.q_stride_l = 0
-    if k.shape[1] == 1:
-        d.k_stride_l = d.v_stride_l = 0
-    if H == 1:
-        d.q_stride_h = 0
-    if k.shape[2] == 1:
-        d.k_stride_h = d.v_stride_h = 0
-    lib.keep(q, k, v, out, out_lo, stats, table, buckets.cells, off_t, kv_len, kpm)
+    need = _bias_ws_bytes("spot_bias_attention_fwd_ws_bytes", numbers, False)
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+    d = _bias_desc(
+        (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),
+         _a(off_t), _a(kv_len), _a(kpm), 0, 0, 0, 0, 0, 0, 0), strides, numbers, scale, _a(ws), need)
+    lib.keep(q, k, v, out, out_lo, stats, table, buckets.cells, off_t, kv_len, kpm, ws)
     with _on(q):
-        need = C.c_long(0)
-        lib.check(lib.load().spot_bias_attention_fwd_ws_bytes(C.byref(d), C.byref(need)), "spot_bias_attention_fwd")
-        if need.value:
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=q.device)
-            lib.keep(ws)
-            d.ws, d.ws_bytes = ws.data_ptr(), need.value
         lib.call("spot_bias_attention_fwd", C.byref(d), _st())
-    return out, out_lo, stats, d, (q, k, v, table, off_t, kv_len, kpm)
+    return out, out_lo, stats, (strides, numbers, scale), (q, k, v, table, off_t, kv_len, kpm)
+
+
+def _a(t):
+    return 0 if t is None else t.data_ptr()
 
 
 class BiasAttentionFn(_Fn):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale):
         train = _wants(ctx)
-        out, out_lo, stats, d, held = _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, train)
+        out, out_lo, stats, desc, held = _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale, train)
         if train:
             ctx.save_for_backward(*held, out, out_lo, stats)
-            ctx.desc, ctx.buckets = d, buckets
+            ctx.desc, ctx.buckets = desc, buckets
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, table, off_t, kv_len, kpm, out, out_lo, stats = ctx.saved_tensors
+        strides, numbers, scale = ctx.desc
+        buckets, want = ctx.buckets, ctx.needs_input_grad
         dout = _dense16(dout)
         dev = q.device
-        d = lib.BiasAttnDesc.from_buffer_copy(ctx.desc)
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2)) if any(ctx.needs_input_grad[1:3]) else (None, None)
-        dtable = torch.empty(table.shape, dtype=table.dtype, device=dev) if ctx.needs_input_grad[3] else None
-        for name, t in (("q", q), ("k", k), ("v", v), ("table", table), ("out", out), ("out_lo", out_lo), ("stats", stats),
-                        ("q_offsets", off_t), ("kv_len", kv_len), ("key_padding_mask", kpm), ("d_out", dout), ("dq", dq), ("dk", dk),
-                        ("dv", dv), ("dtable", dtable)):
-            setattr(d, name, None if t is None else t.data_ptr())
+        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2)) if want[1] or want[2] else (None, None)
+        dtable = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[3] else None
+        need = _bias_ws_bytes("spot_bias_attention_bwd_ws_bytes", numbers, want[3])
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        d = _bias_desc(
+            (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),
+             _a(off_t), _a(kv_len), _a(kpm), dout.data_ptr(), dq.data_ptr(), _a(dk), _a(dv), _a(dtable), buckets.order.data_ptr(),
+             buckets.start.data_ptr()), strides, numbers, scale, ws.data_ptr(), need)
         with _on(q):
-            need = C.c_long(0)
-            lib.check(lib.load().spot_bias_attention_bwd_ws_bytes(C.byref(d), C.byref(need)), "spot_bias_attention_bwd")
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
-            d.ws, d.ws_bytes = ws.data_ptr(), need.value
             lib.call("spot_bias_attention_bwd", C.byref(d), _st())
-        grads = [g if w else None for g, w in zip((dq, dk, dv, dtable), ctx.needs_input_grad)]
-        return (*grads, None, None, None, None, None, None)
+        return (dq if want[0] else None, dk if want[1] else None, dv if want[2] else None, dtable, None, None, None, None, None, None)
 
 
 def bias_attention(q, k, v, table, buckets, causal=False, q_offset=0, kv_len=None, key_padding_mask=None, scale=None):
@@ -2214,7 +2224,8 @@ def bias_attention(q, k, v, table, buckets, causal=False, q_offset=0, kv_len=Non
 # the teacher's top logits, and distillation from them
 # ---------------------------------------------------------------------------
 def _logit_rows(x, name):
-    """[..., V] as rows [N, V] with a dense last dimension, and their distance in elements (a view where one exists)."""
+    """[..., V] as rows [N, V] with a dense last dimension: that tensor (x itself or a view of it where one exists), N, V
+    and the rows' distance in elements."""
     if not x.is_cuda:
         raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
     if x.dtype not in _DTYPE_CODE:
@@ -2222,16 +2233,21 @@ def _logit_rows(x, name):
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError("spot_amd: %s of shape %s has no logits" % (name, tuple(x.shape)))
     V = x.shape[-1]
-    x2 = x.reshape(-1, V) if x.numel() else x.new_empty((0, V))
-    if V > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < V:
-        x2 = x2.contiguous()
-    return x2, max(x2.stride(0), V) if x2.shape[0] > 1 else V
+    N = x.numel() // V
+    if x.is_contiguous():
+        return x, N, V, V
+    x = x.reshape(N, V)
+    if V > 1 and x.stride(1) != 1 or N > 1 and x.stride(0) < V:
+        x = x.contiguous()
+    return x, N, V, x.stride(0) if N > 1 else V
 
 
-def _ws(query, device, *args):
+@functools.lru_cache(maxsize=1024)
+def _rows_ws_bytes(query, code, N, V, k):
+    """Workspace of a call of these sizes (the library's answer depends on them alone)."""
     need = C.c_long(0)
-    lib.check(getattr(lib.load(), query)(*args, C.byref(need)), query)      # answers at once, also while launches are collected
-    return (torch.empty((need.value,), dtype=torch.uint8, device=device) if need.value else None), need.value
+    lib.check(getattr(lib.load(), query)(code, N, V, k, C.byref(need)), query)
+    return need.value
 
 
 def top_logits(logits, k):
@@ -2239,51 +2255,56 @@ def top_logits(logits, k):
     to 128), largest first; of equal values those with the lowest indices, in their order.  A NaN counts as larger than
     every number.  values [..., k] has the logits' type, indices [..., k] is int32.  No gradient flows through it: it is
     the teacher's side of top_logit_distillation."""
-    x, ld = _logit_rows(logits.detach(), "logits")
-    N, V = x.shape
+    x, N, V, ld = _logit_rows(logits, "logits")
     if not 1 <= k <= min(V, 128):
         raise RuntimeError("spot_amd: top_logits takes 1 to %d of %d logits, not %r" % (min(V, 128), V, k))
-    shape = tuple(logits.shape[:-1]) + (int(k),)
+    k, code = int(k), _DTYPE_CODE[x.dtype]
+    shape = (*logits.shape[:-1], k)
     values = torch.empty(shape, dtype=x.dtype, device=x.device)
     indices = torch.empty(shape, dtype=torch.int32, device=x.device)
     if N:
+        need = _rows_ws_bytes("spot_top_logits_ws_bytes", code, N, V, k)
+        ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
         with _on(x):
-            ws, n = _ws("spot_top_logits_ws_bytes", x.device, _DTYPE_CODE[x.dtype], N, V, int(k))
-            lib.call("spot_top_logits", _DTYPE_CODE[x.dtype], _p(x), ld, N, V, int(k), _p(values), _p(indices), _p(ws), n, _st())
+            lib.call("spot_top_logits", code, _p(x), ld, N, V, k, _p(values), _p(indices), _p(ws), need, _st())
     return values, indices
 
 
 class TopLogitDistillationFn(_Fn):
     @staticmethod
     def forward(ctx, student, values, indices, T):
-        x, ld = _logit_rows(student, "student")
-        N, V = x.shape
-        k = values.shape[-1]
-        f = lambda *s: torch.empty(s, dtype=torch.float32, device=x.device)
-        loss, norm, p = f(*student.shape[:-1]), f(N, 2), f(N, k)
+        x, N, V, ld = _logit_rows(student, "student")
+        k, dev = values.shape[-1], x.device
+        train = _wants(ctx)
+        loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=dev)
+        # a row's reference and reciprocal sum, then its k probabilities, for the backward
+        kept = torch.empty((N * (2 + k),), dtype=torch.float32, device=dev) if train else None
         if N:
+            code = _DTYPE_CODE[x.dtype]
+            need = _rows_ws_bytes("spot_top_distill_ws_bytes", code, N, V, k)
+            ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+            norm = _a(kept)
+            lib.keep(kept)
             with _on(x):
-                code = _DTYPE_CODE[x.dtype]
-                ws, n = _ws("spot_top_distill_ws_bytes", x.device, code, N, V, k)
                 lib.call("spot_top_distill_fwd", code, _p(x), ld, _DTYPE_CODE[values.dtype], _p(values), _p(indices), N, V, k, T,
-                         _p(loss), _p(norm), _p(p), _p(ws), n, _st())
-        if _wants(ctx):
-            ctx.save_for_backward(x, indices, norm, p)
-            ctx.dims = (tuple(student.shape), ld, T)
+                         _p(loss), norm, norm + 8 * N if train else None, _p(ws), need, _st())
+        if train:
+            ctx.save_for_backward(x, indices, kept)
+            ctx.dims = (student.shape, N, V, k, ld, T)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, indices, norm, p = ctx.saved_tensors
-        shape, ld, T = ctx.dims
-        N, V = x.shape
+        x, indices, kept = ctx.saved_tensors
+        shape, N, V, k, ld, T = ctx.dims
         dx = torch.empty(shape, dtype=x.dtype, device=x.device)
         if N:
-            dloss = dloss.to(torch.float32).contiguous()
+            dloss = dloss.contiguous()
+            norm = kept.data_ptr()
             with _on(x):
-                lib.call("spot_top_distill_bwd", _DTYPE_CODE[x.dtype], _p(x), ld, _p(indices), _p(norm), _p(p), _p(dloss), N, V,
-                         p.shape[1], T, _p(dx), _st())
+                lib.call("spot_top_distill_bwd", _DTYPE_CODE[x.dtype], _p(x), ld, _p(indices), norm, norm + 8 * N, _p(dloss), N, V,
+                         k, T, _p(dx), _st())
         return dx, None, None, None
 
 
@@ -2295,12 +2316,13 @@ def top_logit_distillation(student, values, indices, temperature=1.0):
     top_logits gives them (k up to 128).  An entry whose index is outside of 0 .. V - 1 (-1: rows with fewer entries) or
     whose value is -inf is absent; a row without entries has loss 0 and gradient 0.  An index listed twice counts twice.
     -> float32 [...]."""
-    if not (student.is_cuda and values.is_cuda and indices.is_cuda and values.device == indices.device == student.device):
+    if not (student.is_cuda and student.get_device() == values.get_device() == indices.get_device()):
         raise RuntimeError("spot_amd: student, values and indices must live on one GPU (no CPU path exists)")
     if values.dtype not in _DTYPE_CODE or indices.dtype != torch.int32:
         raise RuntimeError("spot_amd: values must be float32, bfloat16 or float16 and indices int32, got %s and %s"
                            % (values.dtype, indices.dtype))
-    if student.dim() == 0 or values.shape != indices.shape or values.dim() != student.dim() or values.shape[:-1] != student.shape[:-1]:
+    shape = student.shape
+    if not shape or values.shape != indices.shape or len(values.shape) != len(shape) or values.shape[:-1] != shape[:-1]:
         raise RuntimeError("spot_amd: student %s, values %s, indices %s: [..., V] and twice [..., k]"
                            % (tuple(student.shape), tuple(values.shape), tuple(indices.shape)))
     if not 1 <= values.shape[-1] <= 128:
@@ -2308,4 +2330,5 @@ def top_logit_distillation(student, values, indices, temperature=1.0):
     T = float(temperature)
     if not 0.0 < T < math.inf:
         raise RuntimeError("spot_amd: temperature %r" % (temperature,))
-    return TopLogitDistillationFn.apply(student, values.detach().contiguous(), indices.contiguous(), T)
+    values = values.detach() if values.requires_grad else values
+    return TopLogitDistillationFn.apply(student, values.contiguous(), indices.contiguous(), T)
