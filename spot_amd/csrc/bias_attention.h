@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
 
 // --- forward for few rows -------------------------------------------------------------------------------------------
 // A tile is 32 rows: `heads` query heads of one key/value head for `queries` queries each, so that every key and value
-// is read once for all of them (one new token: its heads).  A workgroup's four waves take 32-key tiles in turn and join
+// is read once for all of them (one new token: its heads).  A workgroup's waves (eight; four from 128 channels on, in f32 from 64) take 32-key tiles in turn and join
 // at the end; where the tiles are few the keys are cut in `splits` ranges, one workgroup each, joined by merge_kernel.
 // Keys go from memory to operand registers (a lane's row), values through the wave's own LDS; the next tile is in flight
 // while this one is worked on.  No barrier until the end.  The biases come from memory (first-level cache): spread out
@@ -414,16 +414,18 @@ __device__ __forceinline__ FewRow few_row(const Args& a, const Seq& s, int kvh, 
 }
 
 template <class T, int D> struct FewLds {
+    static constexpr int NW = D * (int)sizeof(T) <= 128 ? 8 : 4;                         // waves: eight where 256 registers do
     static constexpr int P = D + Vec<T>::PAD, V = FT * P;                                // elements of a wave's values
-    static constexpr int JOIN = 4 * 32 * 33 * 4 + 4 * 32 * 2 * 4;                        // bytes of the waves' join
-    static constexpr int BYTES = 4 * V * (int)sizeof(T) > JOIN ? 4 * V * (int)sizeof(T) : JOIN;
+    static constexpr int JOIN = NW * 32 * 33 * 4 + NW * 32 * 2 * 4;                      // bytes of the waves' join
+    static constexpr int BYTES = NW * V * (int)sizeof(T) > JOIN ? NW * V * (int)sizeof(T) : JOIN;
 };
 
 template <class T, int D, bool MAP>
-__global__ __launch_bounds__(256) void few_kernel(const Args a) {
+__global__ __launch_bounds__((64 * FewLds<T, D>::NW), (FewLds<T, D>::NW / 4)) void few_kernel(const Args a) {
     typedef FewLds<T, D> L;
+    constexpr int NW = L::NW;
     __shared__ __attribute__((aligned(16))) char lds[L::BYTES];
-    __shared__ __attribute__((aligned(16))) int s_u[4][FT];
+    __shared__ __attribute__((aligned(16))) int s_u[NW][FT];
     int unit, rest;
     place(a.B * a.Hkv, a.tiles * a.splits, false, unit, rest);
     const int b = unit / a.Hkv, kvh = unit % a.Hkv, tile = rest / a.splits, split = rest % a.splits;
@@ -513,7 +515,7 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
         load(t_begin + w);
         load_bias();
     }
-    for (int t = t_begin + w; t < t_end; t += 4) {
+    for (int t = t_begin + w; t < t_end; t += NW) {
         const int k0 = t * FT;
         live = next_live;
         f32x16 sc[1] = {f32x16{}};
@@ -534,9 +536,9 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
             const int j = 8 * (e >> 2) + (e & 3);
             sc[0][e] = ((lv >> j) & 1) && k0 + j + 4 * h <= f.last ? fmaf(sc[0][e], a.c, br[e]) : -INFINITY;
         }
-        if (t + 4 < t_end) {
-            find_bias(t + 4);
-            load(t + 4);
+        if (t + NW < t_end) {
+            find_bias(t + NW);
+            load(t + NW);
             load_bias();
         }
         softmax_step<T, 1, D / 32>(sc, m, sum, o);
@@ -551,28 +553,31 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
     }
     sum += __shfl_xor(sum, 32);
 
-    // the four waves' results: [wave][channel][row] and (m, sum) [wave][row]
+    // the waves' results: [wave][channel][row] and (m, sum) [wave][row]
     __syncthreads();
     float* red = reinterpret_cast<float*>(lds);
-    float* ml = red + 4 * 32 * 33;
+    float* ml = red + NW * 32 * 33;
     if (h == 0) {
         ml[(w * 32 + col) * 2] = m;
         ml[(w * 32 + col) * 2 + 1] = sum;
     }
     __syncthreads();
-    const int r = threadIdx.x & 31, d4 = (threadIdx.x >> 5) * 4;
+    const int r = threadIdx.x & 31, d4 = (threadIdx.x >> 5) * 4;        // the first 256 threads write: eight times four channels
     auto joint = [&](int row, float& top, float& total) {
-        top = fmaxf(fmaxf(ml[row * 2], ml[(32 + row) * 2]), fmaxf(ml[(64 + row) * 2], ml[(96 + row) * 2]));
+        top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) top = fmaxf(top, ml[(32 * x + row) * 2]);
         const float ref = top == -INFINITY ? 0.f : top;
         total = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) total += ml[(32 * x + row) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(32 * x + row) * 2] - ref);
+        for (int x = 0; x < NW; ++x) total += ml[(32 * x + row) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(32 * x + row) * 2] - ref);
         return ref;
     };
     float top, total;
     const float mine = __builtin_amdgcn_exp2f(m - joint(col, top, total));
     joint(r, top, total);
     const FewRow fr = few_row(a, s, kvh, tile, r);
+    const bool writes = fr.ok && d4 < 32;
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const long part = ((long)unit * a.tiles + tile) * a.splits + split;
 #pragma unroll
@@ -580,17 +585,20 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) red[(w * 32 + acc_row(e, h)) * 33 + col] = o[u][e] * mine;
         __syncthreads();
-        float x[4];
+        if (writes) {
+            float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            x[e] = (red[(d4 + e) * 33 + r] + red[(32 + d4 + e) * 33 + r]) + (red[(64 + d4 + e) * 33 + r] + red[(96 + d4 + e) * 33 + r]);
-        if (fr.ok) {
+            for (int e = 0; e < 4; ++e) {
+                x[e] = 0.f;
+#pragma unroll
+                for (int y = 0; y < NW; ++y) x[e] += red[(32 * y + d4 + e) * 33 + r];
+            }
             if (a.splits == 1) store_out<T>(a, (((long)b * a.Lq + fr.i) * a.H + fr.head) * D + 32 * u + d4, x, inv);
             else *reinterpret_cast<float4*>(a.few_o + (part * 32 + r) * D + 32 * u + d4) = make_float4(x[0], x[1], x[2], x[3]);
         }
         __syncthreads();
     }
-    if (fr.ok && d4 == 0) {
+    if (writes && d4 == 0) {
         if (a.splits > 1) {
             a.few_ml[(part * 32 + r) * 2] = top;
             a.few_ml[(part * 32 + r) * 2 + 1] = total;
@@ -979,7 +987,7 @@ int launch_f16(int what, int D, const Args& a, unsigned grid, hipStream_t stream
 
 template <class T, int D, bool MAP> void launch_one(int what, const Args& a, unsigned grid, hipStream_t stream) {
     if (what == FWD) fwd_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
-    else if (what == FEW) few_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
+    else if (what == FEW) few_kernel<T, D, MAP><<<grid, 64 * FewLds<T, D>::NW, 0, stream>>>(a);
     else if (what == MERGE) merge_kernel<T, D><<<grid, 256, 0, stream>>>(a);
     else if (what == DQ) dq_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
     else dkv_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);

@@ -17,19 +17,22 @@ enum { F32 = 0, BF16 = 1, F16 = 2 };
 template <class T> struct Vec16 {
     static constexpr int N = 16 / sizeof(T);
     typedef T v __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));     // at any element
 };
 
-// Elements [j VE - skew, j VE - skew + VE) of a row piece of n elements, where `skew` elements lie between the last
-// 16-byte border and the piece: one 16-byte load inside the piece, single elements at its ends, `fill` outside of it.
-template <class T> __device__ __forceinline__ typename Vec16<T>::v load_vec(const T* x, int n, int e0, T fill) {
-    constexpr int VE = Vec16<T>::N;
-    if (e0 >= 0 && e0 + VE <= n) return *reinterpret_cast<const typename Vec16<T>::v*>(x + e0);
-    typename Vec16<T>::v r;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) r[i] = (unsigned)(e0 + i) < (unsigned)n ? x[e0 + i] : fill;
-    return r;
-}
-template <class T> __device__ __forceinline__ int skew_of(const T* x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+// A row piece of n elements in 16-byte vectors from its first 16-byte border on: `head` elements before, nv vectors, and
+// what is left behind; each of the first 2 N threads has one element of the ends, at `end` (-1: none).
+template <class T> struct Piece {
+    static constexpr int VE = Vec16<T>::N;
+    int head, nv, end;
+    __device__ __forceinline__ Piece(const T* x, int n) {
+        const int skew = (int)(((uintptr_t)x & 15) / sizeof(T)), t = threadIdx.x;
+        head = min(skew ? VE - skew : 0, n);
+        nv = (n - head) / VE;
+        const int tail = head + nv * VE;
+        end = t < head ? t : t >= VE && t - VE < n - tail ? tail + t - VE : -1;
+    }
+};
 
 // Whole number that orders as the value does: -0 and +0 are one value, a NaN is above everything.
 template <class T> __device__ __forceinline__ int order_key(T x) {
@@ -75,39 +78,47 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ x, long l
     const int piece = blockIdx.x % pieces, tid = threadIdx.x;
     const int begin = (int)((long)V * piece / pieces), n = (int)((long)V * (piece + 1) / pieces) - begin;
     const T* xr = x + row * ld + begin;
-    // [0, head) and [head + nv VE, n) are the ends before the first and behind the last 16-byte border
-    const int skew = skew_of(xr), head = min(skew ? VE - skew : 0, n), nv = (n - head) / VE;
+    const Piece<T> part(xr, n);
+    const int head = part.head, nv = part.nv, end_at = part.end;
     const T* xv = xr + head;
     if (tid == 0) s_count = s_hits = s_nan = 0;
 
     float top[NV], most = -INFINITY;
     unsigned odd = 0;                                               // largest magnitude, as a whole number
+    // loads without a branch, so that they overlap; threads behind the last vector read it again and drop it
+    constexpr int BATCH = NV < 8 ? NV : 8;
+    if (nv > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = i * NT + tid;
-        top[i] = -INFINITY;
-        if (j < nv) {
-            const typename Vec16<T>::v v = *reinterpret_cast<const typename Vec16<T>::v*>(xv + (long)j * VE);
+        for (int i0 = 0; i0 < NV; i0 += BATCH) {
+            typename Vec16<T>::v v[BATCH];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) top[i] = fmaxf(top[i], (float)v[e]);
-            const uint4 u = *reinterpret_cast<const uint4*>(&v);
-            if (sizeof(T) == 4) {
-                odd = max(max(odd, max(u.x & 0x7fffffffu, u.y & 0x7fffffffu)), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu));
-            } else {
-                typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-                auto pair = [](unsigned z) { z &= 0x7fff7fffu; return *reinterpret_cast<const u16x2*>(&z); };
-                u16x2 q = __builtin_elementwise_max(__builtin_elementwise_max(pair(u.x), pair(u.y)),
-                                                    __builtin_elementwise_max(pair(u.z), pair(u.w)));
-                q = __builtin_elementwise_max(q, *reinterpret_cast<const u16x2*>(&odd));
-                odd = *reinterpret_cast<const unsigned*>(&q);
+            for (int i = 0; i < BATCH; ++i) v[i] = *reinterpret_cast<const typename Vec16<T>::v*>(xv + (long)min((i0 + i) * NT + tid, nv - 1) * VE);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                float m = (float)v[i][0];
+#pragma unroll
+                for (int e = 1; e < VE; ++e) m = fmaxf(m, (float)v[i][e]);
+                const uint4 u = *reinterpret_cast<const uint4*>(&v[i]);
+                if (sizeof(T) == 4) {
+                    odd = max(max(odd, max(u.x & 0x7fffffffu, u.y & 0x7fffffffu)), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu));
+                } else {
+                    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                    auto pair = [](unsigned z) { z &= 0x7fff7fffu; return *reinterpret_cast<const u16x2*>(&z); };
+                    u16x2 q = __builtin_elementwise_max(__builtin_elementwise_max(pair(u.x), pair(u.y)),
+                                                        __builtin_elementwise_max(pair(u.z), pair(u.w)));
+                    q = __builtin_elementwise_max(q, *reinterpret_cast<const u16x2*>(&odd));
+                    odd = *reinterpret_cast<const unsigned*>(&q);
+                }
+                top[i0 + i] = (i0 + i) * NT + tid < nv ? m : -INFINITY;
+                most = fmaxf(most, top[i0 + i]);
             }
         }
-        most = fmaxf(most, top[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) top[i] = -INFINITY;
     }
     const unsigned inf = sizeof(T) == 4 ? 0x7f800000u : (float)T(1) == 1.f && sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     bool has_nan = sizeof(T) == 4 ? odd > inf : (odd & 0xffff) > inf || (odd >> 16) > inf;
-    // one element of the ends for each of the first threads
-    const int end_at = tid < head ? tid : tid >= VE && tid - VE < n - head - nv * VE ? head + nv * VE + tid - VE : -1;
     T end_x = (T)-INFINITY;
     if (end_at >= 0) {
         end_x = xr[end_at];
@@ -292,24 +303,48 @@ struct Distill {
 };
 
 // (mc, l) over a piece of a row
+template <class T, int NB> __device__ __forceinline__ void norm_step(const typename Vec16<T>::v* v, float c, float& top, Norm& r) {
+    float m = top;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < Vec16<T>::N; ++j) m = fmaxf(m, (float)v[i][j]);
+    if (m > top) {
+        r.l *= __builtin_amdgcn_exp2f(fminf(r.m - m * c, 0.f));     // the first reference is no power to scale by
+        r.m = m * c;
+        top = m;
+    }
+    float l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < Vec16<T>::N; ++j) l[j & 3] += __builtin_amdgcn_exp2f(fmaf((float)v[i][j], c, -r.m));
+    r.l += (l[0] + l[1]) + (l[2] + l[3]);
+}
 template <class T> __device__ __forceinline__ Norm row_norm(const T* x, int n, float c) {
-    constexpr int VE = Vec16<T>::N;
-    const int skew = skew_of(x), nv = (n + skew + VE - 1) / VE;
+    constexpr int VE = Vec16<T>::N, NB = 4;
+    typedef typename Vec16<T>::v V;
+    const Piece<T> part(x, n);
+    const V* xv = reinterpret_cast<const V*>(x + part.head);
     float top = -INFINITY;
     Norm r = {0.f, 0.f};
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        const typename Vec16<T>::v v = load_vec(x, n, i * VE - skew, (T)-INFINITY);
-        float m = top;
+    int i = threadIdx.x;
+    for (; i + (NB - 1) * NT < part.nv; i += NB * NT) {
+        V v[NB];
 #pragma unroll
-        for (int j = 0; j < VE; ++j) m = fmaxf(m, (float)v[j]);
-        if (m > top) {
-            r.l *= __builtin_amdgcn_exp2f(fminf(r.m - m * c, 0.f));     // the first reference is no power to scale by
-            r.m = m * c;
-            top = m;
-        }
+        for (int y = 0; y < NB; ++y) v[y] = xv[i + y * NT];
+        norm_step<T, NB>(v, c, top, r);
+    }
+    for (; i < part.nv; i += NT) {
+        const V v = xv[i];
+        norm_step<T, 1>(&v, c, top, r);
+    }
+    if (part.end >= 0) {
+        V v;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) r.l += __builtin_amdgcn_exp2f(fmaf((float)v[j], c, -r.m));
+        for (int j = 0; j < VE; ++j) v[j] = (T)-INFINITY;
+        v[0] = x[part.end];
+        norm_step<T, 1>(&v, c, top, r);
     }
     if (top == -INFINITY) r.m = -INFINITY;
     return r;
@@ -374,8 +409,10 @@ template <class T> __global__ __launch_bounds__(NT) void distill_bwd_kernel(cons
     constexpr int VE = Vec16<T>::N;
     __shared__ float s_p[KMAX];
     __shared__ int s_at[KMAX];
-    const long row = blockIdx.x / a.pieces;
-    const int piece = blockIdx.x % a.pieces;
+    // last rows first: what the forward read last is still in the last-level cache
+    const unsigned block = gridDim.x - 1 - blockIdx.x;
+    const long row = block / a.pieces;
+    const int piece = block % a.pieces;
     const int begin = (int)((long)a.V * piece / a.pieces), n = (int)((long)a.V * (piece + 1) / a.pieces) - begin;
     const T* x = static_cast<const T*>(a.student) + row * a.ld + begin;
     T* dx = static_cast<T*>(a.d_student) + row * a.V + begin;
@@ -386,26 +423,26 @@ template <class T> __global__ __launch_bounds__(NT) void distill_bwd_kernel(cons
         s_at[i] = a.indices[row * a.k + i];
     }
     const float f = g * inv;
-    const int skew = skew_of(dx), nv = (n + skew + VE - 1) / VE;
-    const bool same = skew_of(x) == skew;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        const int e0 = i * VE - skew;
-        typename Vec16<T>::v v, o;
-        if (same) v = load_vec(x, n, e0, (T)0.f);
-        else {
+    const Piece<T> part(dx, n);
+    const T* xv = x + part.head;
+    T* dv = dx + part.head;
+    auto grad = [&](typename Vec16<T>::v v) {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) v[j] = (unsigned)(e0 + j) < (unsigned)n ? x[e0 + j] : (T)0.f;
-        }
+        for (int j = 0; j < VE; ++j) v[j] = none ? (T)0.f : (T)(f * __builtin_amdgcn_exp2f(fmaf((float)v[j], a.c, -mc)));
+        return v;
+    };
+    constexpr int NB = 4;
+    int i = threadIdx.x;
+    for (; i + (NB - 1) * NT < part.nv; i += NB * NT) {
+        typename Vec16<T>::v v[NB];
 #pragma unroll
-        for (int j = 0; j < VE; ++j) o[j] = none ? (T)0.f : (T)(f * __builtin_amdgcn_exp2f(fmaf((float)v[j], a.c, -mc)));
-        if (e0 >= 0 && e0 + VE <= n) *reinterpret_cast<typename Vec16<T>::v*>(dx + e0) = o;
-        else {
+        for (int y = 0; y < NB; ++y) v[y] = *reinterpret_cast<const typename Vec16<T>::any*>(xv + (long)(i + y * NT) * VE);
 #pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if ((unsigned)(e0 + j) < (unsigned)n) dx[e0 + j] = o[j];
-        }
+        for (int y = 0; y < NB; ++y) *reinterpret_cast<typename Vec16<T>::v*>(dv + (long)(i + y * NT) * VE) = grad(v[y]);
     }
+    for (; i < part.nv; i += NT)
+        *reinterpret_cast<typename Vec16<T>::v*>(dv + (long)i * VE) = grad(*reinterpret_cast<const typename Vec16<T>::any*>(xv + (long)i * VE));
+    if (part.end >= 0) dx[part.end] = none ? (T)0.f : (T)(f * __builtin_amdgcn_exp2f(fmaf((float)x[part.end], a.c, -mc)));
     // the stores above have to be in memory before another wave writes some of the same places
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();

@@ -2054,14 +2054,15 @@ class _on:
 
 
 def _aligned16(t):
-    """t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes, else a copy; and
-    the strides of the others in elements (0 for dimensions of length one, whose stride says nothing)."""
-    es, strides = t.element_size(), t.stride()
-    strides = [x if n > 1 else 0 for n, x in zip(t.shape, strides)]
-    if strides[-1] != 1 or t.data_ptr() % 16 or any(x * es % 16 for x in strides[:-1]):
+    """[B, L, heads, D] t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes,
+    else a copy; and the strides of the others in elements (0 for dimensions of length one, whose stride says nothing)."""
+    if not (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        es, strides = t.element_size(), [x if n > 1 else 0 for n, x in zip(t.shape, t.stride())]
+        if strides[3] == 1 and t.data_ptr() % 16 == 0 and not any(x * es % 16 for x in strides[:3]):
+            return t, strides[:3]
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = t.stride()
-    return t, strides[:-1]
+    _, L, heads, D = t.shape
+    return t, (L * heads * D, heads * D, D)
 
 
 def _dense16(t):
