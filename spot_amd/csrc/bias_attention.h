@@ -147,6 +147,12 @@ template <bool MAP> __device__ __forceinline__ int coord(const Args& a, int p) {
 __device__ __forceinline__ int key_end(const Args& a, const Seq& s, int q0) {
     return a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
 }
+// whole tiles of keys from the first on that all queries of that workgroup see
+__device__ __forceinline__ int open_end(const Args& a, const Seq& s, int q0, int k_end) {
+    if (a.kpm || s.off + q0 < 0 || s.off + min(q0 + BM, a.Lq) > a.N) return 0;
+    return max(a.causal ? min(k_end, s.off + q0 + 1) : k_end, 0) / BN * BN;
+}
+template <bool B> struct Flag { static constexpr bool value = B; };
 // bit l: key k0 + l is no padding
 __device__ __forceinline__ unsigned long long live_keys(const Args& a, const Seq& s, int b, int k0) {
     const int key = k0 + (threadIdx.x & 63);
@@ -231,10 +237,10 @@ __device__ __forceinline__ void place(int units, int per_unit, bool longest, int
     rest = longest ? j / here : j % per_unit;
 }
 
-// The softmax step of a lane's row: the scores of NT tiles become 2^(s - reference + SHIFT), the sums are scaled where
-// the reference moves.
+// The softmax of a lane's row, tile by tile: the reference moves, and what was summed is scaled, where a score of NT
+// tiles is more than LAG above it; then the scores become 2^(s - reference + SHIFT) and join the sum.
 template <class T, int NT, int NO>
-__device__ __forceinline__ void softmax_step(f32x16* sc, float& m, float& sum, f32x16* o) {
+__device__ __forceinline__ void rescale(const f32x16* sc, float& m, float& sum, f32x16* o) {
     float mx = sc[0][0];
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -248,6 +254,8 @@ __device__ __forceinline__ void softmax_step(f32x16* sc, float& m, float& sum, f
         for (int t = 0; t < NO; ++t) o[t] *= f;
         m = to;
     }
+}
+template <class T, int NT> __device__ __forceinline__ void exponentials(f32x16* sc, float m, float& sum) {
     const float low = (m == -INFINITY ? 0.f : m) - Vec<T>::SHIFT;
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -278,8 +286,10 @@ template <class T> __device__ __forceinline__ void store_stats(const Args& a, in
 }
 
 // --- forward ------------------------------------------------------------------------------------------------------
-// One workgroup: 128 queries of one head, 32 per wave; keys stream through LDS in tiles of 64, the next one in flight in
+// One workgroup: 128 queries of one head, 32 per wave; keys stream through LDS in tiles of 64, the next ones in flight in
 // registers.  Queries sit on the lanes (S^T = K Q^T), so reference and sum are one number per lane.
+// Tiles without hidden keys come first, in a loop of their own: a test inside cuts the instruction stream that the matrix
+// and the vector unit are to share (8 x 8191 x 8191 x 128 f16: 437 -> 375 us without it).
 template <class T, int D, bool MAP>
 __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) qf[c] = frag_or_zero(qr + 16 * c + 8 * h, i < a.Lq);
     }
-    f32x16 o[D / 32];
+    f32x16 o[D / 32], sc[2];
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, sum = 0.f;
@@ -323,48 +333,29 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
         tv.load(vb + k0 * a.v_l, a.v_l, next);
         tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
     };
-    if (k_end > 0) load(0);
-    for (int k0 = 0; k0 < k_end; k0 += BN) {
-        const unsigned long long live = next;
-        __syncthreads();
-        tk.store(sk);
-        tv.store(sv);
-        tw.store(a, bias, sb, a.window);
-        if (MAP && threadIdx.x < BN) su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
-        __syncthreads();
-        if (k0 + BN < k_end) load(k0 + BN);
-
-        f32x16 sc[2] = {f32x16{}, f32x16{}};
+    auto step = [&](int k0, unsigned long long live, auto masked) {
+        sc[0] = sc[1] = f32x16{};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
             for (int u = 0; u < 2; ++u) mma(frag<T>(sk + (32 * u + col) * KT::P + 16 * c + 8 * h), qf[c], sc[u]);
+        const unsigned long long lv = live >> (4 * h);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int j = 32 * u + 8 * g;                        // + 4 h + 0 .. 3
-                int4 x = {lane_u + 4 * h + j, lane_u + 4 * h + j + 1, lane_u + 4 * h + j + 2, lane_u + 4 * h + j + 3};
-                if (MAP) {
-                    const int4 y = *reinterpret_cast<const int4*>(su + j + 4 * h);
-                    x = {lane_u + y.x, lane_u + y.y, lane_u + y.z, lane_u + y.w};
+                int4 y = {j + 4 * h, j + 4 * h + 1, j + 4 * h + 2, j + 4 * h + 3};
+                if (MAP) y = *reinterpret_cast<const int4*>(su + j + 4 * h);
+                const int at[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[u][4 * g + e] = fmaf(sc[u][4 * g + e], a.c, sb[lane_u + at[e]]);
+                    if (decltype(masked)::value && (!((lv >> (j + e)) & 1) || k0 + j + 4 * h + e > last)) sc[u][4 * g + e] = -INFINITY;
                 }
-                sc[u][4 * g] = fmaf(sc[u][4 * g], a.c, sb[x.x]);
-                sc[u][4 * g + 1] = fmaf(sc[u][4 * g + 1], a.c, sb[x.y]);
-                sc[u][4 * g + 2] = fmaf(sc[u][4 * g + 2], a.c, sb[x.z]);
-                sc[u][4 * g + 3] = fmaf(sc[u][4 * g + 3], a.c, sb[x.w]);
             }
-        if (live != ~0ull || __any(last < k0 + BN - 1)) {
-            const unsigned long long lv = live >> (4 * h);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = 32 * u + 8 * (e >> 2) + (e & 3);
-                    if (!((lv >> j) & 1) || k0 + j + 4 * h > last) sc[u][e] = -INFINITY;
-                }
-        }
-        softmax_step<T, 2, D / 32>(sc, m, sum, o);
+        rescale<T, 2, D / 32>(sc, m, sum, o);
+        exponentials<T, 2>(sc, m, sum);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -373,7 +364,23 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t) mma(vcol(32 * u + 16 * c, 32 * t), pf, o[t]);
             }
-    }
+    };
+    auto tile = [&](int k0, auto masked) {
+        const unsigned long long live = next;
+        __syncthreads();
+        tk.store(sk);
+        tv.store(sv);
+        tw.store(a, bias, sb, a.window);
+        if (MAP && threadIdx.x < BN) su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
+        __syncthreads();
+        if (k0 + BN < k_end) load(k0 + BN);
+        step(k0, live, masked);
+    };
+    if (k_end > 0) load(0);
+    const int open = open_end(a, s, q0, k_end);
+    int k0 = 0;
+    for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
+    for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
     sum += __shfl_xor(sum, 32);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (i >= a.Lq) return;
@@ -541,7 +548,8 @@ __global__ __launch_bounds__((64 * FewLds<T, D>::NW), (FewLds<T, D>::NW / 4)) vo
             load(t + NW);
             load_bias();
         }
-        softmax_step<T, 1, D / 32>(sc, m, sum, o);
+        rescale<T, 1, D / 32>(sc, m, sum, o);
+        exponentials<T, 1>(sc, m, sum);
         wave_fence();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -694,7 +702,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
 
     typename Vec<T>::v8 qf[D / 16], gf[D / 16];
-    float m = 0.f, inv = 0.f, delta = 0.f;
+    float m = FLT_MAX, inv = 0.f, delta = 0.f;           // rows behind the last query: probabilities 0
     {
         const bool ok = i < a.Lq;
         const T* qr = static_cast<const T*>(a.q) + b * a.q_b + (long)i * a.q_l + head * a.q_h;
@@ -736,22 +744,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
         tv.load(vb + k0 * a.v_l, a.v_l, next);
         tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
     };
-    if (k_end > 0) load(0);
-    for (int k0 = 0; k0 < k_end; k0 += BN) {
-        const unsigned long long live = next;
-        __syncthreads();
-        tk.store(sk);
-        tv.store(sv);
-        tw.store(a, bias, sb, a.window);
-        if (MAP && threadIdx.x < BN) {
-            su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
-            sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
-        }
-        __syncthreads();
-        if (k0 + BN < k_end) load(k0 + BN);
-
+    const float delta_inv = delta * inv;
+    auto step = [&](int k0, unsigned long long live, auto masked) {
         const unsigned long long lv = live >> (4 * h);
-        const bool masked = live != ~0ull || __any(last < k0 + BN - 1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f32x16 sc = {}, dp = {};
@@ -768,18 +763,11 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int at = lane_u + (MAP ? (e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w) : j + 4 * h + e);
-                    sc[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sc[4 * g + e], a.c, sb[at]) - m) * inv;
+                    float p = __builtin_amdgcn_exp2f(fmaf(sc[4 * g + e], a.c, sb[at]) - m);
+                    if (decltype(masked)::value && (!((lv >> (j + e)) & 1) || k0 + j + 4 * h + e > last)) p = 0.f;
+                    dp[4 * g + e] = p * fmaf(dp[4 * g + e], inv, -delta_inv);
                 }
             }
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = 32 * u + 8 * (e >> 2) + (e & 3);
-                    if (!((lv >> j) & 1) || k0 + j + 4 * h > last) sc[e] = 0.f;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] = sc[e] * (dp[e] - delta);
             if (want) {
                 if (MAP) {
                     f32x16 around = {}, inside = dp;
@@ -806,7 +794,26 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
                 for (int t = 0; t < D / 32; ++t) mma(kcol(32 * u + 16 * c, 32 * t), df, dq[t]);
             }
         }
-    }
+    };
+    auto tile = [&](int k0, auto masked) {
+        const unsigned long long live = next;
+        __syncthreads();
+        tk.store(sk);
+        tv.store(sv);
+        tw.store(a, bias, sb, a.window);
+        if (MAP && threadIdx.x < BN) {
+            su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
+            sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
+        }
+        __syncthreads();
+        if (k0 + BN < k_end) load(k0 + BN);
+        step(k0, live, masked);
+    };
+    if (k_end > 0) load(0);
+    const int open = open_end(a, s, q0, k_end);
+    int k0 = 0;
+    for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
+    for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
     if (want && k_end > 0 && h == 0)
 #pragma unroll
         for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + 31 - col] = carry[cls];
@@ -827,7 +834,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 // One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers; the queries of all
 // heads that share it stream through LDS 64 at a time, 32 for each wave of a pair, so the sums over those heads stay in
 // the accumulators (no atomics, one order) and the pair joins at the end.  Keys sit on the lanes (S = Q K^T), P and dS
-// are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// (garbage for padding, whose sums are dropped) are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
 template <class T, int D> struct DkvLds {
     typedef Tile<T, D, 64> QT;
     static constexpr int TILES = 2 * QT::ELEMS * (int)sizeof(T), JOIN = 2 * 64 * 16 * 4;
@@ -870,46 +877,40 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
 
     const int i_begin = k0 >= s.len ? a.Lq : a.causal ? max(0, (k0 - s.off) / QB * QB) : 0;
     const int blocks = i_begin < a.Lq ? (a.Lq - i_begin + QB - 1) / QB : 0, steps = blocks * a.G;
+    // blocks with queries before some of the keys come first, for all heads
+    const int cut = a.causal ? min(blocks, max(0, (k0 + KB - 1 - s.off - i_begin + QB - 1) / QB)) : 0;
+    auto place_of = [&](int n, int& head, int& i0) {
+        const bool first = n < cut * a.G;
+        const int per = first ? cut : blocks - cut, x = first ? n : n - cut * a.G;
+        head = kvh * a.G + x / per;
+        i0 = i_begin + (x % per + (first ? 0 : cut)) * QB;
+    };
     QT tq, tg;
     Window tw;
     float rm = 0.f, ri = 0.f, rd = 0.f;
     int rl = -1, ru = 0;
-    // step n: query block n % blocks of head n / blocks
+    const float* tw_bias = nullptr;
     auto load = [&](int n) {
-        const int head = kvh * a.G + n / blocks, i0 = i_begin + n % blocks * QB;
+        int head, i0;
+        place_of(n, head, i0);
+        tw_bias = a.bias + (long)head * a.pitch;
         const unsigned long long rows = a.Lq - i0 >= 64 ? ~0ull : (1ull << (a.Lq - i0)) - 1;
         tq.load(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, rows);
         tg.load(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, rows);
         const int u_hi = coord<MAP>(a, max(s.off + i0 + QB - 1, 0));
-        tw.load(a, a.bias + (long)head * a.pitch, u_lo - u_hi + a.ncells / 2, a.window);
+        tw.load(a, tw_bias, u_lo - u_hi + a.ncells / 2, a.window);
         if (threadIdx.x < QB) {
             const int i = i0 + threadIdx.x;
             const long st = ((long)b * a.H + head) * a.Lq + i;
-            const bool ok = i < a.Lq;
-            rm = ok ? a.stats[2 * st] : 0.f;
+            rl = last_key(a, s, i);
+            const bool ok = rl >= 0;                            // else no key: probabilities 0
+            rm = ok ? a.stats[2 * st] : FLT_MAX;
             ri = ok ? a.stats[2 * st + 1] * up<T>() : 0.f;
             rd = ok ? a.delta[st] * down<T>() : 0.f;
-            rl = last_key(a, s, i);
             ru = u_hi - coord<MAP>(a, max(s.off + i, 0));
         }
     };
-    if (steps > 0) load(0);
-    for (int n = 0; n < steps; ++n) {
-        __syncthreads();
-        tq.store(sq);
-        tg.store(sg);
-        tw.store(a, a.bias + (long)(kvh * a.G + n / blocks) * a.pitch, sb, a.window);
-        if (threadIdx.x < QB) {
-            sm[threadIdx.x] = rm;
-            si[threadIdx.x] = ri;
-            sd[threadIdx.x] = rd;
-            sl[threadIdx.x] = rl;
-            su[threadIdx.x] = ru;
-        }
-        __syncthreads();
-        if (n + 1 < steps) load(n + 1);
-        // rows that see not all of this workgroup's keys: behind the last query, out of the buckets, causal
-        const bool masked = __any(!alive) || __any(sl[32 * u + col] < k0 + KB - 1);
+    auto step = [&](auto masked) {
         f32x16 sc = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
@@ -934,16 +935,10 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             for (int e = 0; e < 4; ++e) {
                 const int x = 4 * g + e;
                 sc[x] = __builtin_amdgcn_exp2f(fmaf(sc[x], a.c, sb[at[e]]) - m_[e]) * i_[e];
-                dp[x] = fmaf(dp[x], down<T>(), -d_[e]);
+                if (decltype(masked)::value && key > sl[r + e]) sc[x] = 0.f;
+                dp[x] = sc[x] * fmaf(dp[x], down<T>(), -d_[e]);
             }
         }
-        if (masked) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (!alive || key > sl[32 * u + acc_row(e, h)]) sc[e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] *= sc[e];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const typename Vec<T>::v8 pf = acc_frag<T>(sc, c), df = acc_frag<T>(dp, c);
@@ -953,7 +948,27 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
                 mma(qcol(32 * u + 16 * c, 32 * t), df, dk[t]);
             }
         }
-    }
+    };
+    auto tile = [&](int n, auto masked) {
+        __syncthreads();
+        tq.store(sq);
+        tg.store(sg);
+        tw.store(a, tw_bias, sb, a.window);
+        if (threadIdx.x < QB) {
+            sm[threadIdx.x] = rm;
+            si[threadIdx.x] = ri;
+            sd[threadIdx.x] = rd;
+            sl[threadIdx.x] = rl;
+            su[threadIdx.x] = ru;
+        }
+        __syncthreads();
+        if (n + 1 < steps) load(n + 1);
+        step(masked);
+    };
+    if (steps > 0) load(0);
+    int n = 0;
+    for (; n < cut * a.G; ++n) tile(n, Flag<true>());
+    for (; n < steps; ++n) tile(n, Flag<false>());
     // the pair's sums, one 32-channel block at a time: the second wave's go through LDS to the first
     float* join = reinterpret_cast<float*>(lds) + (w & 1) * 64 * 16 + l;
     const long row = (((long)b * a.Lk + key) * a.Hkv + kvh) * D;
@@ -973,7 +988,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             for (int g = 0; g < 4; ++g) {
                 typename Vec<T>::v4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (T)((acc[4 * g + e] + join[64 * (4 * g + e)]) * f);
+                for (int e = 0; e < 4; ++e) x[e] = alive ? (T)((acc[4 * g + e] + join[64 * (4 * g + e)]) * f) : (T)0.f;
                 *reinterpret_cast<typename Vec<T>::v4*>(out + 8 * g) = x;
             }
         }
