@@ -55,7 +55,7 @@ enum { FWD, FEW, MERGE, DQ, DKV };          // kernels
 template <class T, int D> constexpr int waves_of(int kernel) {
     const int words = D * (int)sizeof(T) / 64;      // 1, 2, 4 for 16-bit heads of 32, 64, 128 channels; twice that in f32
     return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 1 ? 3 : words <= 2 ? 2 : 1)
-                                                                                 : (words <= 1 ? 3 : words <= 2 ? 2 : 1);
+                                                 : (D == 32 ? 3 : words <= 2 ? 2 : 1);
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -647,31 +647,32 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
 
 // --- dQ and the sums along the offsets ------------------------------------------------------------------------------
 // The forward's split.  The table's gradient is the sum of dS along each offset key - query: a wave writes a 32x32 tile
-// of dS to its own LDS, row k turned by k places, so that a column holds one offset before the turn's end and one behind
-// it (t places back, and 32 - t on), and 64 lanes sum the 32 columns' halves.  The next key tile of the same wave goes on
-// with the latter at the same lanes: 32 finished sums are written per tile.  (LDS float additions by atomics, one per
-// element, took 145 cycles per wave instruction and 60 % of the kernel.)  On a map an offset stands for two different
-// column offsets, inside a row and around its end: two sets of sums.
+// of dS to its own LDS with row k moved k places to the left, so that a column holds one offset, and each lane sums one
+// of the 63 columns (the places around the moved rows are zero and stay so).  The offsets of the next key tile of the
+// same wave are 32 further: what 32 lanes hold then is finished, and 32 sums are written per tile.  (LDS float additions
+// by atomics, one per element, took 145 cycles per wave instruction and 60 % of the kernel.)  On a map an offset stands
+// for two different column offsets, inside a row and around its end: two sets of sums.
+constexpr int SP = 73;                          // pitch of a moved row: the wave's halves, four rows apart, meet other banks
 __device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 32; }
-__device__ __forceinline__ void offset_sums(const f32x16& x, float* lds, float& carry, float* out) {
-    const int l = threadIdx.x & 63, col = l & 31, h = l >> 5;
-    // element e of half h is row acc_row(e, h); physical rows 2 e + h: the halves write and read different banks
+// lane t: the sum of offset 31 - t
+__device__ __forceinline__ float offset_sums(const f32x16& x, float* lds) {
+    const int l = threadIdx.x & 63, h = l >> 5;
+    float* to = lds + 4 * h * SP + (l & 31) + 31 - 4 * h;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) lds[(2 * e + h) * 32 + ((col - acc_row(e, h)) & 31)] = x[e];
+    for (int e = 0; e < 16; ++e) to[acc_row(e, 0) * (SP - 1)] = x[e];
     wave_fence();
-    float before = 0.f, behind = 0.f;
+    float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const float v = lds[(2 * e + h) * 32 + col];
-        const bool wraps = acc_row(e, h) + col >= 32;
-        before += wraps ? 0.f : v;
-        behind += wraps ? v : 0.f;
-    }
+    for (int k = 0; k < 32; ++k) s[k & 1] += lds[k * SP + l];
     wave_fence();
-    before += __shfl_xor(before, 32);
-    behind += __shfl_xor(behind, 32);
-    if (h == 0) out[31 - col] = before + carry;
-    carry = behind;
+    return s[0] + s[1];
+}
+// `before`: this lane's sum of the key tile before, whose offsets are 32 smaller
+__device__ __forceinline__ void hand_over(float now, float& before, float* out) {
+    const int l = threadIdx.x & 63;
+    const float x = now + __shfl_xor(before, 32);
+    if (l >= 31 && l < 63) out[62 - l] = x;
+    before = now;
 }
 
 template <class T, int D, bool MAP>
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
     __shared__ float sb[WindowLds<MAP>::N];
     __shared__ __attribute__((aligned(16))) int su[BN], sx[BN];
-    __shared__ float turned[4][32 * 32];
+    __shared__ float moved[4][32 * SP];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
     place(a.B * a.Hkv, a.G * nq, a.causal, unit, rest);
@@ -693,7 +694,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     const Seq s = sequence(a, b);
     const int last = last_key(a, s, i);
     const int u_hi = coord<MAP>(a, max(s.off + q0 + BM - 1, 0)), lane_u = u_hi - coord<MAP>(a, max(s.off + i, 0));
-    const int px = MAP ? max(s.off + i, 0) % a.width : 0;
+    const int px = MAP ? max(s.off + i, 0) % a.width : 0, qx = MAP ? max(s.off + q0 + 32 * w, 0) % a.width : 0;
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
     const float* bias = a.bias + (long)head * a.pitch;
@@ -732,6 +733,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) dq[t] = f32x16{};
     float carry[CLS] = {};
+    if (want)
+        for (int t = l; t < 32 * SP; t += 64) moved[w][t] = 0.f;
 
     const int k_end = key_end(a, s, q0);
     const ColFrag<T, KT::P> kcol(sk);
@@ -769,22 +772,32 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
                 }
             }
             if (want) {
-                if (MAP) {
-                    f32x16 around = {}, inside = dp;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int4 x = *reinterpret_cast<const int4*>(sx + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if ((e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w) < px) {
-                                around[4 * g + e] = dp[4 * g + e];
-                                inside[4 * g + e] = 0.f;
-                            }
-                    }
-                    offset_sums(inside, turned[w], carry[0], part + k0 + 32 * u);
-                    offset_sums(around, turned[w], carry[CLS - 1], part + (CLS - 1) * pitch + k0 + 32 * u);
+                float* out = part + k0 + 32 * u;
+                if (!MAP) {
+                    hand_over(offset_sums(dp, moved[w]), carry[0], out);
                 } else {
-                    offset_sums(dp, turned[w], carry[0], part + k0 + 32 * u);
+                    const int kx = __builtin_amdgcn_readfirstlane(sx[32 * u]);
+                    if (qx + 31 < a.width && kx + 31 < a.width) {
+                        // queries and keys of one row each: the offset decides whether it goes around the row's end
+                        const float t = offset_sums(dp, moved[w]);
+                        const bool in = kx - qx + 31 - l >= 0;
+                        hand_over(in ? t : 0.f, carry[0], out);
+                        hand_over(in ? 0.f : t, carry[CLS - 1], out + (CLS - 1) * pitch);
+                    } else {
+                        f32x16 around = {}, inside = dp;
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int4 x = *reinterpret_cast<const int4*>(sx + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if ((e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w) < px) {
+                                    around[4 * g + e] = dp[4 * g + e];
+                                    inside[4 * g + e] = 0.f;
+                                }
+                        }
+                        hand_over(offset_sums(inside, moved[w]), carry[0], out);
+                        hand_over(offset_sums(around, moved[w]), carry[CLS - 1], out + (CLS - 1) * pitch);
+                    }
                 }
             }
 #pragma unroll
@@ -814,9 +827,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     int k0 = 0;
     for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
     for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
-    if (want && k_end > 0 && h == 0)
+    if (want && k_end > 0 && h == 0)            // what the last tile has begun, and the one place that none has
 #pragma unroll
-        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + 31 - col] = carry[cls];
+        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + (l < 31 ? 30 - l : 31)] = l < 31 ? carry[cls] : 0.f;
     if (i >= a.Lq) return;
     T* out = static_cast<T*>(a.dq) + (((long)b * a.Lq + i) * a.H + head) * D;
 #pragma unroll
