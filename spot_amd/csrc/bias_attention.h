@@ -766,9 +766,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int at = lane_u + (MAP ? (e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w) : j + 4 * h + e);
-                    float p = __builtin_amdgcn_exp2f(fmaf(sc[4 * g + e], a.c, sb[at]) - m);
-                    if (decltype(masked)::value && (!((lv >> (j + e)) & 1) || k0 + j + 4 * h + e > last)) p = 0.f;
-                    dp[4 * g + e] = p * fmaf(dp[4 * g + e], inv, -delta_inv);
+                    float x = fmaf(sc[4 * g + e], a.c, sb[at]) - m;
+                    if (decltype(masked)::value && (!((lv >> (j + e)) & 1) || k0 + j + 4 * h + e > last)) x = -INFINITY;
+                    dp[4 * g + e] = __builtin_amdgcn_exp2f(x) * fmaf(dp[4 * g + e], inv, -delta_inv);
                 }
             }
             if (want) {
@@ -947,8 +947,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int x = 4 * g + e;
-                sc[x] = __builtin_amdgcn_exp2f(fmaf(sc[x], a.c, sb[at[e]]) - m_[e]) * i_[e];
-                if (decltype(masked)::value && key > sl[r + e]) sc[x] = 0.f;
+                float y = fmaf(sc[x], a.c, sb[at[e]]) - m_[e];
+                if (decltype(masked)::value && key > sl[r + e]) y = -INFINITY;
+                sc[x] = __builtin_amdgcn_exp2f(y) * i_[e];
                 dp[x] = sc[x] * fmaf(dp[x], down<T>(), -d_[e]);
             }
         }
