@@ -602,7 +602,7 @@ int spot_clip_grad_norm_f32(float* grads, long n, float max_norm, float* norm_ou
  *
  * q [B, Lq, H, head_dim], k and v [B, Lk, Hkv, head_dim] of one dtype (0 f32, 1 bf16, 2 f16), H a multiple of Hkv (query
  * head h reads key/value head h / (H / Hkv)), head_dim 32, 64 or 128; strides in elements, the last dimension dense;
- * bases and strides are whole numbers of 16 bytes.  out, d_out, dq [B, Lq, H, head_dim] and dk, dv
+ * bases and strides are whole numbers of 16 bytes, stride_l not negative and less than 64 MB.  out, d_out, dq [B, Lq, H, head_dim] and dk, dv
  * [B, Lk, Hkv, head_dim] are dense and of that dtype too.
  *
  * Positions: key j stands at j, query i of sequence b at offset_b + i, where offset_b is q_offset (q_offset_mode 0),

@@ -32,7 +32,6 @@ constexpr int BM = 128;     // queries per workgroup of the forward and dQ kerne
 constexpr int BN = 64;      // keys per LDS tile there
 constexpr int KB = 64;      // keys per workgroup of the dK / dV kernel: 32 per pair of waves
 constexpr int MAXW = 512;   // columns of a map
-constexpr int PADB = 64;    // entries behind the last of a head's spread-out biases
 
 struct Args {               // strides in elements; out, d_out, dq, dk, dv are dense [B, L, heads, D]
     const void *q, *k, *v, *d_out, *table;
@@ -42,7 +41,7 @@ struct Args {               // strides in elements; out, d_out, dq, dk, dv are d
     const unsigned char* kpm;
     long q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
     int B, H, Hkv, G, Lq, Lk, N, width, nb, causal, off_mode, off, table_type;
-    int ncells, pitch, window;  // 2 u(N - 1) + 1; floats of a head's biases; window of a workgroup's tile
+    int ncells, pitch, front, window;       // 2 u(N - 1) + 1; floats of a head's biases, and before its first; window of a tile
     float scale, c;         // c = scale * log2 e
     int heads, queries, tiles, splits;      // few_kernel: heads and queries of a tile of 32 rows, tiles, key ranges
     float *few_o, *few_ml;                  // its partial results if splits > 1
@@ -143,6 +142,10 @@ __device__ __forceinline__ int last_key(const Args& a, const Seq& s, int i) {
 template <bool MAP> __device__ __forceinline__ int coord(const Args& a, int p) {
     return MAP ? p / a.width * (2 * a.width - 1) + p % a.width : p;
 }
+// coordinate of a query: positions outside of the buckets' range see no key, any place near will do for them
+template <bool MAP> __device__ __forceinline__ int query_coord(const Args& a, int p) {
+    return coord<MAP>(a, min(max(p, 0), a.N - 1 + BM));
+}
 // end of the keys that the workgroup of queries q0 .. q0 + BM - 1 has to see
 __device__ __forceinline__ int key_end(const Args& a, const Seq& s, int q0) {
     return a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
@@ -180,23 +183,21 @@ __device__ __forceinline__ float bias_at(const Args& a, int i, int head) {
     return log2_bias(t);
 }
 
-// Window of a head's biases from cell i0 on, by 256 threads; the first 512 entries travel in registers while the tile
-// before is worked on, what a very wide map needs beyond is read when it is stored.
+// Window of a head's biases from `from` on, by 256 threads; the first 512 entries travel in registers while the tile
+// before is worked on, what a very wide map needs beyond is read when it is stored.  The spread-out biases are padded so
+// that no window reaches past them.
 struct Window {
     float r[2];
-    int i0;
-    __device__ __forceinline__ static float at(const Args& a, const float* bias, int i) {
-        return (unsigned)i < (unsigned)a.ncells ? bias[i] : 0.f;
+    const float* from;
+    __device__ __forceinline__ void load(const float* at, int n) {
+        from = at;
+        r[0] = at[threadIdx.x];
+        if (n > 256) r[1] = at[256 + threadIdx.x];
     }
-    __device__ __forceinline__ void load(const Args& a, const float* bias, int from, int n) {
-        i0 = from;
-        r[0] = at(a, bias, from + (int)threadIdx.x);
-        if (n > 256) r[1] = at(a, bias, from + 256 + (int)threadIdx.x);
-    }
-    __device__ __forceinline__ void store(const Args& a, const float* bias, float* lds, int n) const {
+    __device__ __forceinline__ void store(float* lds, int n) const {
         if ((int)threadIdx.x < n) lds[threadIdx.x] = r[0];
         if (n > 256 && (int)threadIdx.x + 256 < n) lds[threadIdx.x + 256] = r[1];
-        for (int t = 512 + threadIdx.x; t < n; t += 256) lds[t] = at(a, bias, i0 + t);
+        for (int t = 512 + threadIdx.x; t < n; t += 256) lds[t] = from[t];
     }
 };
 // entries of a window: keys and queries in a row, u's range on a map
@@ -206,17 +207,29 @@ template <bool MAP> struct WindowLds { static constexpr int N = MAP ? 1280 : BM 
 static_assert(window_of(64, 128, MAXW) <= 1280 && window_of(64, 128, 127) <= 1280, "a tile's window has to fit");
 
 // --- LDS tiles: ROWS x D elements, row-major, 16 bytes a load.  Rows whose bit in `live` is not set are zero: what
-// padding holds (infinities, NaN) does not reach a product.
+// padding holds (infinities, NaN) does not reach a product.  Addresses are a uniform 64-bit base and a lane's 32-bit
+// offset of its own that stays (the library refuses rows 2^26 bytes or more apart).
 template <class T, int D, int ROWS> struct Tile {
     static constexpr int P = D + Vec<T>::PAD, ELEMS = ROWS * P;
     static constexpr int VE = 16 / sizeof(T), VR = D / VE, VECS = ROWS * VR, NV = (VECS + 255) / 256;
     uint4 r[NV];
-    __device__ __forceinline__ void load(const T* base, long stride, unsigned long long live) {
+    __device__ __forceinline__ static unsigned lane_offset(long stride) {
+        return (unsigned)(threadIdx.x / VR) * (unsigned)(stride * sizeof(T)) + threadIdx.x % VR * 16;
+    }
+    // base: the tile's first row; offset: lane_offset(stride)
+    __device__ __forceinline__ void load(const T* base, long stride, unsigned offset, unsigned long long live) {
+        const char* p = reinterpret_cast<const char*>(base);
+        const long step = 256 / VR * stride * (long)sizeof(T);
+        if (live == ~0ull && VECS % 256 == 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int id = threadIdx.x + 256 * i, row = id / VR, c = id % VR;
-            r[i] = make_uint4(0, 0, 0, 0);
-            if ((VECS % 256 == 0 || id < VECS) && ((live >> row) & 1)) r[i] = *reinterpret_cast<const uint4*>(base + row * stride + c * VE);
+            for (int i = 0; i < NV; ++i) r[i] = *reinterpret_cast<const uint4*>(p + i * step + offset);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int row = threadIdx.x / VR + 256 / VR * i;
+                r[i] = make_uint4(0, 0, 0, 0);
+                if (row < ROWS && ((live >> row) & 1)) r[i] = *reinterpret_cast<const uint4*>(p + i * step + offset);
+            }
         }
     }
     __device__ __forceinline__ void store(T* lds) const {
@@ -306,10 +319,10 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
     const int last = last_key(a, s, i);
-    const int u_hi = coord<MAP>(a, max(s.off + q0 + BM - 1, 0)), lane_u = u_hi - coord<MAP>(a, max(s.off + i, 0));
+    const int u_hi = query_coord<MAP>(a, s.off + q0 + BM - 1), lane_u = u_hi - query_coord<MAP>(a, s.off + i);
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
-    const float* bias = a.bias + (long)head * a.pitch;
+    const float* bias = a.bias + (long)head * a.pitch + a.front + a.ncells / 2 - u_hi;       // of offset u(key) from here on
 
     typename Vec<T>::v8 qf[D / 16];
     {
@@ -322,16 +335,17 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
     for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, sum = 0.f;
 
-    const int k_end = key_end(a, s, q0);
+    const int k_end = key_end(a, s, q0), open = open_end(a, s, q0, k_end);
+    const unsigned k_off = KT::lane_offset(a.k_l), v_off = KT::lane_offset(a.v_l);
     const ColFrag<T, KT::P> vcol(sv);
     KT tk, tv;
     Window tw;
     unsigned long long next = 0;
     auto load = [&](int k0) {
-        next = live_keys(a, s, b, k0);
-        tk.load(kb + k0 * a.k_l, a.k_l, next);
-        tv.load(vb + k0 * a.v_l, a.v_l, next);
-        tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
+        next = k0 < open ? ~0ull : live_keys(a, s, b, k0);
+        tk.load(kb + k0 * a.k_l, a.k_l, k_off, next);
+        tv.load(vb + k0 * a.v_l, a.v_l, v_off, next);
+        tw.load(bias + coord<MAP>(a, k0), a.window);
     };
     auto step = [&](int k0, unsigned long long live, auto masked) {
         sc[0] = sc[1] = f32x16{};
@@ -370,14 +384,13 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
         __syncthreads();
         tk.store(sk);
         tv.store(sv);
-        tw.store(a, bias, sb, a.window);
+        tw.store(sb, a.window);
         if (MAP && threadIdx.x < BN) su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
         __syncthreads();
         if (k0 + BN < k_end) load(k0 + BN);
         step(k0, live, masked);
     };
     if (k_end > 0) load(0);
-    const int open = open_end(a, s, q0, k_end);
     int k0 = 0;
     for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
     for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
@@ -444,7 +457,7 @@ __global__ __launch_bounds__((64 * FewLds<T, D>::NW), (FewLds<T, D>::NW / 4)) vo
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
     const int head = f.ok ? f.head : 0, cell0 = a.ncells / 2 - coord<MAP>(a, f.p);
-    const float* bias = a.bias ? a.bias + (long)head * a.pitch + cell0 : nullptr;
+    const float* bias = a.bias ? a.bias + (long)head * a.pitch + a.front + cell0 : nullptr;
     const ColFrag<T, L::P> vcol(sv);
 
     typename Vec<T>::v8 qf[D / 16], kf[D / 16];
@@ -693,11 +706,11 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
     const int last = last_key(a, s, i);
-    const int u_hi = coord<MAP>(a, max(s.off + q0 + BM - 1, 0)), lane_u = u_hi - coord<MAP>(a, max(s.off + i, 0));
+    const int u_hi = query_coord<MAP>(a, s.off + q0 + BM - 1), lane_u = u_hi - query_coord<MAP>(a, s.off + i);
     const int px = MAP ? max(s.off + i, 0) % a.width : 0, qx = MAP ? max(s.off + q0 + 32 * w, 0) % a.width : 0;
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
-    const float* bias = a.bias + (long)head * a.pitch;
+    const float* bias = a.bias + (long)head * a.pitch + a.front + a.ncells / 2 - u_hi;       // of offset u(key) from here on
     const bool want = a.part != nullptr;
     const int pitch = sum_pitch(a.Lk);
     float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
@@ -736,16 +749,17 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     if (want)
         for (int t = l; t < 32 * SP; t += 64) moved[w][t] = 0.f;
 
-    const int k_end = key_end(a, s, q0);
+    const int k_end = key_end(a, s, q0), open = open_end(a, s, q0, k_end);
+    const unsigned k_off = KT::lane_offset(a.k_l), v_off = KT::lane_offset(a.v_l);
     const ColFrag<T, KT::P> kcol(sk);
     KT tk, tv;
     Window tw;
     unsigned long long next = 0;
     auto load = [&](int k0) {
-        next = live_keys(a, s, b, k0);
-        tk.load(kb + k0 * a.k_l, a.k_l, next);
-        tv.load(vb + k0 * a.v_l, a.v_l, next);
-        tw.load(a, bias, coord<MAP>(a, k0) - u_hi + a.ncells / 2, a.window);
+        next = k0 < open ? ~0ull : live_keys(a, s, b, k0);
+        tk.load(kb + k0 * a.k_l, a.k_l, k_off, next);
+        tv.load(vb + k0 * a.v_l, a.v_l, v_off, next);
+        tw.load(bias + coord<MAP>(a, k0), a.window);
     };
     const float delta_inv = delta * inv;
     auto step = [&](int k0, unsigned long long live, auto masked) {
@@ -813,7 +827,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
         __syncthreads();
         tk.store(sk);
         tv.store(sv);
-        tw.store(a, bias, sb, a.window);
+        tw.store(sb, a.window);
         if (MAP && threadIdx.x < BN) {
             su[threadIdx.x] = coord<MAP>(a, k0 + threadIdx.x) - coord<MAP>(a, k0);
             sx[threadIdx.x] = (k0 + threadIdx.x) % a.width;
@@ -823,7 +837,6 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
         step(k0, live, masked);
     };
     if (k_end > 0) load(0);
-    const int open = open_end(a, s, q0, k_end);
     int k0 = 0;
     for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
     for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
@@ -902,16 +915,15 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     Window tw;
     float rm = 0.f, ri = 0.f, rd = 0.f;
     int rl = -1, ru = 0;
-    const float* tw_bias = nullptr;
+    const unsigned q_off = QT::lane_offset(a.q_l), g_off = QT::lane_offset((long)a.H * D);
     auto load = [&](int n) {
         int head, i0;
         place_of(n, head, i0);
-        tw_bias = a.bias + (long)head * a.pitch;
         const unsigned long long rows = a.Lq - i0 >= 64 ? ~0ull : (1ull << (a.Lq - i0)) - 1;
-        tq.load(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, rows);
-        tg.load(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, rows);
-        const int u_hi = coord<MAP>(a, max(s.off + i0 + QB - 1, 0));
-        tw.load(a, tw_bias, u_lo - u_hi + a.ncells / 2, a.window);
+        tq.load(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, q_off, rows);
+        tg.load(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, g_off, rows);
+        const int u_hi = query_coord<MAP>(a, s.off + i0 + QB - 1);
+        tw.load(a.bias + (long)head * a.pitch + a.front + a.ncells / 2 + u_lo - u_hi, a.window);
         if (threadIdx.x < QB) {
             const int i = i0 + threadIdx.x;
             const long st = ((long)b * a.H + head) * a.Lq + i;
@@ -920,7 +932,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             rm = ok ? a.stats[2 * st] : FLT_MAX;
             ri = ok ? a.stats[2 * st + 1] * up<T>() : 0.f;
             rd = ok ? a.delta[st] * down<T>() : 0.f;
-            ru = u_hi - coord<MAP>(a, max(s.off + i, 0));
+            ru = u_hi - query_coord<MAP>(a, s.off + i);
         }
     };
     auto step = [&](auto masked) {
@@ -967,7 +979,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
         __syncthreads();
         tq.store(sq);
         tg.store(sg);
-        tw.store(a, tw_bias, sb, a.window);
+        tw.store(sb, a.window);
         if (threadIdx.x < QB) {
             sm[threadIdx.x] = rm;
             si[threadIdx.x] = ri;

@@ -1,5 +1,7 @@
 // Entry points of the attention with a relative position bias (kernels: bias_attention.h), and the two small kernels
 // that turn the backward's sums along offsets into the gradient of the bias table.
+#include <stdlib.h>
+
 #include "bias_attention.h"
 #include "../../include/spot_hip.h"
 
@@ -7,10 +9,11 @@ namespace ba {
 
 static_assert(MAXW == SPOT_BIAS_ATTN_MAX_WIDTH, "the windows are made for this width");
 
-// The table spread out by offset, times log2 e: bias[head][u(key) - u(query) + u(N - 1)].
+// The table spread out by offset, times log2 e: bias[head][front + u(key) - u(query) + u(N - 1)], zero
+// before and behind.
 __global__ __launch_bounds__(256) void spread_kernel(const Args a) {
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < a.pitch) a.bias[(long)blockIdx.y * a.pitch + i] = i < a.ncells ? bias_at(a, i, blockIdx.y) : 0.f;
+    if (i < a.pitch) a.bias[(long)blockIdx.y * a.pitch + i] = bias_at(a, i - a.front, blockIdx.y);
 }
 
 // Sums of dS along each offset over sequences and queries.  A wave of the dQ kernel has left its sums for keys
@@ -92,7 +95,13 @@ static int cells_of(const spot_bias_attn_desc& d) {
     const int last = d.max_len - 1;
     return 2 * (d.width ? last / d.width * (2 * d.width - 1) + last % d.width : last) + 1;
 }
-static int pitch_of(const spot_bias_attn_desc& d) { return (cells_of(d) + PADB + (d.width ? window_span(FT, d.width) : 0) + 63) / 64 * 64; }
+// floats before a head's first cell: queries reach up to BM positions past the last; and of a head in all: a window of 512
+// (or of a wide map's own size) from the last cell on
+static int front_of(const spot_bias_attn_desc& d) { return (window_span(BM + 2, d.width) + 63) / 64 * 64; }
+static int pitch_of(const spot_bias_attn_desc& d) {
+    const int window = window_of(BN, BM, d.width);
+    return front_of(d) + (cells_of(d) + (window > 512 ? window : 512) + 63) / 64 * 64;
+}
 struct Layout { long sums, delta, bias, part, total; };
 static Layout layout(const spot_bias_attn_desc& d) {
     const long cls = d.width > 0 ? 2 : 1, nw = (d.Lq + BM - 1) / BM * 4, pitch = ((long)d.Lk + BN - 1) / BN * BN + 32;
@@ -160,6 +169,10 @@ static int check(const spot_bias_attn_desc* d, bool backward) {
                             d->v_stride_b, d->v_stride_l, d->v_stride_h};
     for (long s : strides)
         SPOT_CHECK_ARG(s % per == 0, "spot_bias_attention: a stride of %ld elements is no whole number of 16 bytes", s);
+    SPOT_CHECK_ARG(labs(d->q_stride_l) < (1L << 26) / (per == 4 ? 4 : 2) && labs(d->k_stride_l) < (1L << 26) / (per == 4 ? 4 : 2) &&
+                       labs(d->v_stride_l) < (1L << 26) / (per == 4 ? 4 : 2) && d->q_stride_l >= 0 && d->k_stride_l >= 0 && d->v_stride_l >= 0 &&
+                       (long)d->H * d->head_dim < (1L << 24),
+                   "spot_bias_attention: rows of a head have to be less than 64 MB apart, in rising order");
     SPOT_CHECK_ARG(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && aligned16(d->out) && aligned16(d->out_lo),
                    "spot_bias_attention: q, k, v, out and out_lo have to be 16-byte aligned");
     SPOT_CHECK_ARG((long)d->B * d->H * ((d->Lq + 31) / 32) < (1L << 31) && (long)d->B * d->Hkv * ((d->Lk + 31) / 32) < (1L << 31),
@@ -184,7 +197,7 @@ static Args arguments(const spot_bias_attn_desc& d) {
     a.v_b = d.v_stride_b; a.v_l = d.v_stride_l; a.v_h = d.v_stride_h;
     a.B = d.B; a.H = d.H; a.Hkv = d.Hkv; a.G = d.H / d.Hkv; a.Lq = d.Lq; a.Lk = d.Lk; a.N = d.max_len; a.width = d.width;
     a.nb = d.num_buckets; a.causal = d.causal != 0; a.off_mode = d.q_offset_mode; a.off = d.q_offset; a.table_type = d.table_dtype;
-    a.ncells = cells_of(d); a.pitch = pitch_of(d); a.window = window_of(BN, BM, d.width);
+    a.ncells = cells_of(d); a.pitch = pitch_of(d); a.front = front_of(d); a.window = window_of(BN, BM, d.width);
     a.scale = d.scale; a.c = d.scale * LOG2E;
     return a;
 }

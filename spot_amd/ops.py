@@ -2054,11 +2054,11 @@ class _on:
 
 
 def _aligned16(t):
-    """[B, L, heads, D] t itself if its last dimension is dense and its base and strides are whole numbers of 16 bytes,
-    else a copy; and the strides of the others in elements (0 for dimensions of length one, whose stride says nothing)."""
+    """[B, L, heads, D] t itself if its last dimension is dense, its base and strides are whole numbers of 16 bytes and
+    its rows less than 64 MB apart, else a copy; and the strides of the others in elements (0 for dimensions of length one, whose stride says nothing)."""
     if not (t.is_contiguous() and t.data_ptr() % 16 == 0):
         es, strides = t.element_size(), [x if n > 1 else 0 for n, x in zip(t.shape, t.stride())]
-        if strides[3] == 1 and t.data_ptr() % 16 == 0 and not any(x * es % 16 for x in strides[:3]):
+        if strides[3] == 1 and t.data_ptr() % 16 == 0 and not any(x * es % 16 for x in strides[:3]) and strides[1] * es < 1 << 26:
             return t, strides[:3]
         t = t.clone(memory_format=torch.contiguous_format)
     _, L, heads, D = t.shape
