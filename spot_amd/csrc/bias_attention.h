@@ -150,7 +150,8 @@ template <bool MAP> __device__ __forceinline__ int query_coord(const Args& a, in
 __device__ __forceinline__ int key_end(const Args& a, const Seq& s, int q0) {
     return a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
 }
-// whole tiles of keys from the first on that all queries of that workgroup see
+// whole tiles of keys from the first on that all queries of that workgroup see (rows behind the last query do not matter
+// where every row is on its own; sums over rows take masked tiles for them)
 __device__ __forceinline__ int open_end(const Args& a, const Seq& s, int q0, int k_end) {
     if (a.kpm || s.off + q0 < 0 || s.off + min(q0 + BM, a.Lq) > a.N) return 0;
     return max(a.causal ? min(k_end, s.off + q0 + 1) : k_end, 0) / BN * BN;
@@ -716,7 +717,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
 
     typename Vec<T>::v8 qf[D / 16], gf[D / 16];
-    float m = FLT_MAX, inv = 0.f, delta = 0.f;           // rows behind the last query: probabilities 0
+    float m = 0.f, inv = 0.f, delta = 0.f;
     {
         const bool ok = i < a.Lq;
         const T* qr = static_cast<const T*>(a.q) + b * a.q_b + (long)i * a.q_l + head * a.q_h;
@@ -749,7 +750,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     if (want)
         for (int t = l; t < 32 * SP; t += 64) moved[w][t] = 0.f;
 
-    const int k_end = key_end(a, s, q0), open = open_end(a, s, q0, k_end);
+    const int k_end = key_end(a, s, q0), open = q0 + BM > a.Lq ? 0 : open_end(a, s, q0, k_end);
     const unsigned k_off = KT::lane_offset(a.k_l), v_off = KT::lane_offset(a.v_l);
     const ColFrag<T, KT::P> kcol(sk);
     KT tk, tv;
@@ -903,13 +904,16 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
 
     const int i_begin = k0 >= s.len ? a.Lq : a.causal ? max(0, (k0 - s.off) / QB * QB) : 0;
     const int blocks = i_begin < a.Lq ? (a.Lq - i_begin + QB - 1) / QB : 0, steps = blocks * a.G;
-    // blocks with queries before some of the keys come first, for all heads
-    const int cut = a.causal ? min(blocks, max(0, (k0 + KB - 1 - s.off - i_begin + QB - 1) / QB)) : 0;
+    // first, for all heads, the blocks that hold queries before some of the keys, and the last one if it is not full (and
+    // all where queries stand outside of the buckets' range): there hidden scores are masked
+    const int cut = s.off + i_begin < 0 || s.off + a.Lq > a.N ? blocks
+                  : a.causal ? min(blocks, max(0, (k0 + KB - 1 - s.off - i_begin + QB - 1) / QB)) : 0;
+    const int hiding = cut < blocks && (a.Lq - i_begin) % QB != 0 ? cut + 1 : cut;
     auto place_of = [&](int n, int& head, int& i0) {
-        const bool first = n < cut * a.G;
-        const int per = first ? cut : blocks - cut, x = first ? n : n - cut * a.G;
+        const bool first = n < hiding * a.G;
+        const int per = first ? hiding : blocks - hiding, x = first ? n : n - hiding * a.G, y = x % per;
         head = kvh * a.G + x / per;
-        i0 = i_begin + (x % per + (first ? 0 : cut)) * QB;
+        i0 = i_begin + (first ? y < cut ? y : blocks - 1 : cut + y) * QB;
     };
     QT tq, tg;
     Window tw;
@@ -928,8 +932,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             const int i = i0 + threadIdx.x;
             const long st = ((long)b * a.H + head) * a.Lq + i;
             rl = last_key(a, s, i);
-            const bool ok = rl >= 0;                            // else no key: probabilities 0
-            rm = ok ? a.stats[2 * st] : FLT_MAX;
+            const bool ok = rl >= 0;                            // else no key
+            rm = ok ? a.stats[2 * st] : 0.f;
             ri = ok ? a.stats[2 * st + 1] * up<T>() : 0.f;
             rd = ok ? a.delta[st] * down<T>() : 0.f;
             ru = u_hi - query_coord<MAP>(a, s.off + i);
@@ -993,7 +997,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     };
     if (steps > 0) load(0);
     int n = 0;
-    for (; n < cut * a.G; ++n) tile(n, Flag<true>());
+    for (; n < hiding * a.G; ++n) tile(n, Flag<true>());
     for (; n < steps; ++n) tile(n, Flag<false>());
     // the pair's sums, one 32-channel block at a time: the second wave's go through LDS to the first
     float* join = reinterpret_cast<float*>(lds) + (w & 1) * 64 * 16 + l;

@@ -115,27 +115,34 @@ static Layout layout(const spot_bias_attn_desc& d) {
 }
 
 // The forward's kernel.  few_kernel reads keys once for all heads that share them and cuts the keys between its waves and
-// workgroups; fwd_kernel reads them once per 128 queries.  The former is taken for up to 32 rows per key/value head, and
-// where the latter's workgroups would not fill the 256 CUs.
+// workgroups; fwd_kernel reads them once per 128 queries and head and needs fewer instructions per score.  The former is
+// taken for up to 32 rows per key/value head, and where the latter's workgroups, counted by their queries, are few for 256
+// CUs: under 48 of them in 16 bits (8 heads of 64 over 512 tokens, 32 workgroups: 13.0 against 15.2 us; over 1024, 64: 38.7
+// against 24.8), under 192 in f32, where the products weigh more (8 heads of 32, 1024 tokens: 39.8 against 52.5 us, two
+// sequences 50.5 against 52.9, four 70.7 against 53.6).
 struct Few { bool use, spread; int heads, queries, tiles, splits; long o, ml, bias; };
 static Few few(const spot_bias_attn_desc& d) {
     Few f = {};
     const int G = d.H / d.Hkv;
-    f.use = (long)d.Lq * G <= 32 || (long)d.B * d.H * ((d.Lq + BM - 1) / BM) < 256;
+    f.use = (long)d.Lq * G <= 32 || (long)d.B * d.H * d.Lq < (d.dtype == F32 ? 192L : 48L) * BM;
     f.heads = G < 32 ? G : 32;
     f.queries = 32 / f.heads;
     f.tiles = ((d.Lq + f.queries - 1) / f.queries) * ((G + f.heads - 1) / f.heads);
-    // about four workgroups per CU, each with a few tiles for every wave
-    const long units = (long)d.B * d.Hkv * f.tiles, most = d.Lk / (4 * FT * 2);
-    long splits = units ? 1024 / units : 1;
+    // One workgroup per CU, but at least 256 keys for each: the join costs more than idle CUs beyond that (one token, 8 heads
+    // of 128, 16384 keys: 259 us in one range, 40.0 in 16, 42.6 in 32, 66 in 64; 256 units: 389 in one, 398 in two).
+    const long units = (long)d.B * d.Hkv * f.tiles, most = d.Lk / 256;
+    long splits = units ? 256 / units : 1;
     if (splits > most) splits = most;
     f.splits = splits < 1 ? 1 : (int)splits;
     if (f.splits > 1) {
         f.o = units * f.splits * 32 * d.head_dim * 4;
         f.ml = units * f.splits * 32 * 2 * 4;
     }
-    // biases by bucket are two dependent loads per score; spread out they are one, after a launch of a few microseconds
-    f.spread = !f.use || d.Lk / (4 * FT * f.splits) >= 4;
+    // Biases by bucket are two dependent loads per score; spread out they are one, after a launch of a few microseconds:
+    // worth it from four tiles per wave on (32 tokens, 8 heads of 64, 2048 keys: 45 against 52 us; one token over 4096 keys
+    // in 16 ranges: 14.9 against 13.8).
+    const int waves = d.head_dim * (d.dtype == F32 ? 4 : 2) <= 128 ? 8 : 4;
+    f.spread = !f.use || d.Lk / (waves * FT * f.splits) >= 4;
     f.bias = f.spread ? 4L * d.H * pitch_of(d) : 0;
     return f;
 }
@@ -148,7 +155,7 @@ static int check(const spot_bias_attn_desc* d, bool backward) {
                    "spot_bias_attention: dtype %d / table_dtype %d is none of 0 (f32), 1 (bf16), 2 (f16)", d->dtype, d->table_dtype);
     SPOT_CHECK_ARG(d->head_dim == 32 || d->head_dim == 64 || d->head_dim == 128,
                    "spot_bias_attention: head_dim must be 32, 64 or 128, not %d", d->head_dim);
-    SPOT_CHECK_ARG(d->B >= 0 && d->Lq >= 0 && d->Lk >= 0 && d->H > 0 && d->Hkv > 0 && d->H % d->Hkv == 0,
+    SPOT_CHECK_ARG(d->B >= 0 && d->Lq >= 0 && d->Lk >= 0 && d->H > 0 && d->H <= 65535 && d->Hkv > 0 && d->H % d->Hkv == 0,
                    "spot_bias_attention: B %d, Lq %d, Lk %d, %d heads over %d key/value heads", d->B, d->Lq, d->Lk, d->H, d->Hkv);
     SPOT_CHECK_ARG(d->max_len >= 1 && d->max_len <= SPOT_BIAS_ATTN_MAX_LEN && d->Lk <= d->max_len && d->Lq <= SPOT_BIAS_ATTN_MAX_LEN,
                    "spot_bias_attention: max_len %d for %d keys and %d queries (1 to %d, no fewer than the keys)", d->max_len, d->Lk,

@@ -2122,10 +2122,10 @@ def _bias_desc(pointers, strides, numbers, scale, ws=0, ws_bytes=0):
 
 @functools.lru_cache(maxsize=1024)
 def _bias_ws_bytes(query, numbers, with_table):
-    """Workspace of a call of these sizes (the library's answer depends on them alone)."""
+    """Workspace of a call of these sizes (the library's answer depends on them alone); numbers: without q_offset."""
     p = 4096           # the size asks for no data: any address that is not null
     d = _bias_desc((p,) * 4 + (0,) * 2 + (p,) * 2 + (p if numbers[12] == 1 else 0,) + (0,) * 6 + (p if with_table else 0,) + (p,) * 2, (0,) * 9,
-                   numbers, 1.0)
+                   numbers + (0,), 1.0)
     need = C.c_long(0)
     lib.check(getattr(lib.load(), query)(C.byref(d), C.byref(need)), query)
     return need.value
@@ -2148,7 +2148,7 @@ def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_p
     out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
     out_lo = torch.empty_like(out) if train and code else None
     stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device) if train else None
-    need = _bias_ws_bytes("spot_bias_attention_fwd_ws_bytes", numbers, False)
+    need = _bias_ws_bytes("spot_bias_attention_fwd_ws_bytes", numbers[:13], False)
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     d = _bias_desc(
         (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),
@@ -2184,7 +2184,7 @@ class BiasAttentionFn(_Fn):
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
         dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2)) if want[1] or want[2] else (None, None)
         dtable = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[3] else None
-        need = _bias_ws_bytes("spot_bias_attention_bwd_ws_bytes", numbers, want[3])
+        need = _bias_ws_bytes("spot_bias_attention_bwd_ws_bytes", numbers[:13], want[3])
         ws = torch.empty((need,), dtype=torch.uint8, device=dev)
         d = _bias_desc(
             (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),

@@ -207,6 +207,50 @@ def test_few_queries_over_a_cache(ops, t, size):
     run_case(ops, t, *size, masked=B > 1, train=False, seed=13, max_len=Lk + 100)
 
 
+# many rows: the kernel of 128 queries per workgroup (from 48 such workgroups on, 192 in f32)
+MANY = [(130, 130, 4, 2, 64, 0), (70, 300, 4, 4, 32, 0), (144, 144, 4, 1, 128, 0), (260, 260, 2, 2, 64, 20), (129, 65, 4, 4, 128, 0), (192, 192, 4, 4, 32, 32),
+        (100, 100, 4, 2, 64, 40), (128, 64, 4, 2, 32, 64)]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", MANY)
+def test_many_rows(ops, t, size):
+    Lq, Lk, H, Hkv, D, width = size
+    B = -(-(192 if t == "f32" else 48) * 128 // (Lq * H))
+    run_case(ops, t, B, Lq, Lk, H, Hkv, D, width=width, seed=20)
+    run_case(ops, t, B, Lq, Lk, H, Hkv, D, width=width, train=False, masked=True, seed=21)
+    lens = [Lk - (b * 37) % Lk for b in range(B)]
+    run_case(ops, t, B, Lq, Lk, H, Hkv, D, width=width, kv_len=lens, seed=22)
+    if not width:
+        run_case(ops, t, B, Lq, Lk, H, Hkv, D, causal=True, kv_len=lens, q_offset="end", max_len=max(Lq, Lk) + 7, seed=23)
+        run_case(ops, t, B, Lq, Lk, H, Hkv, D, causal=True, q_offset=[b % 9 - 4 for b in range(B)], seed=24)
+        run_case(ops, t, B, Lq, Lk, H, Hkv, D, causal=True, seed=25)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,causal", [(1, 90, False), (1, 90, True), (70, 90, False), (70, 90, True), (1, 1, False), (40, 200, True)])
+def test_entries_that_no_pair_has_may_hold_anything(ops, t, B, L, causal):
+    """NaN and infinities in buckets of offsets that only rows and keys past the end would have."""
+    n = 2 * (L + 300) - 1
+    d = torch.arange(n) - (L + 299)
+    used = (d.abs() < L) & ((d <= 0) | (not causal))
+    cells = torch.where(used, d.abs() % 5, 5 + d.abs() % 3)
+    b = ops.RelativeBuckets(cells, 8, L + 300, device=DEV)
+    T = TYPES[t]
+    q, k, v, g = (torch.randn(B, L, 4, 32, device=DEV).to(T) for _ in range(4))
+    table = torch.randn(8, 4, device=DEV).to(T)
+    clean = [x.clone().requires_grad_() for x in (q, k, v, table)]
+    want = ops.bias_attention(*clean, b, causal=causal)
+    want = (want, *torch.autograd.grad(want, clean, g))
+    table[5], table[6], table[7] = math.nan, math.inf, -math.inf
+    leaves = [x.requires_grad_() for x in (q, k, v, table)]
+    got = ops.bias_attention(*leaves, b, causal=causal)
+    got = (got, *torch.autograd.grad(got, leaves, g))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert not got[4][5:].any()
+
+
 @pytest.mark.parametrize("t,table_t", [("bf16", "f32"), ("f16", "f32"), ("f32", "bf16"), ("f32", "f16")])
 def test_table_of_another_type(ops, t, table_t):
     run_case(ops, t, 2, 100, 100, 4, 2, 64, table_t=table_t, seed=14)
