@@ -53,7 +53,7 @@ enum { FWD, FEW, MERGE, DQ, DKV };          // kernels
 // Waves per SIMD that the registers are cut for: as many as fit without spilling.
 template <class T, int D> constexpr int waves_of(int kernel) {
     const int words = D * (int)sizeof(T) / 64;      // 1, 2, 4 for 16-bit heads of 32, 64, 128 channels; twice that in f32
-    return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 1 ? 3 : words <= 2 ? 2 : 1)
+    return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 1 ? 3 : words <= 4 ? 2 : 1)
                                                  : (D == 32 ? 3 : words <= 2 ? 2 : 1);
 }
 
