@@ -150,8 +150,7 @@ template <bool MAP> __device__ __forceinline__ int query_coord(const Args& a, in
 __device__ __forceinline__ int key_end(const Args& a, const Seq& s, int q0) {
     return a.causal ? min(s.len, s.off + min(q0 + BM, a.Lq)) : s.len;
 }
-// whole tiles of keys from the first on that all queries of that workgroup see (rows behind the last query do not matter
-// where every row is on its own; sums over rows take masked tiles for them)
+// whole tiles of keys from the first on that all queries of that workgroup see
 __device__ __forceinline__ int open_end(const Args& a, const Seq& s, int q0, int k_end) {
     if (a.kpm || s.off + q0 < 0 || s.off + min(q0 + BM, a.Lq) > a.N) return 0;
     return max(a.causal ? min(k_end, s.off + q0 + 1) : k_end, 0) / BN * BN;
@@ -230,6 +229,22 @@ template <class T, int D, int ROWS> struct Tile {
                 const int row = threadIdx.x / VR + 256 / VR * i;
                 r[i] = make_uint4(0, 0, 0, 0);
                 if (row < ROWS && ((live >> row) & 1)) r[i] = *reinterpret_cast<const uint4*>(p + i * step + offset);
+            }
+        }
+    }
+    // the first n rows, zero behind them
+    __device__ __forceinline__ void load_first(const T* base, long stride, unsigned offset, int n) {
+        const char* p = reinterpret_cast<const char*>(base);
+        const long step = 256 / VR * stride * (long)sizeof(T);
+        if (n >= ROWS && VECS % 256 == 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) r[i] = *reinterpret_cast<const uint4*>(p + i * step + offset);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int row = threadIdx.x / VR + 256 / VR * i;
+                r[i] = make_uint4(0, 0, 0, 0);
+                if (row < ROWS && row < n) r[i] = *reinterpret_cast<const uint4*>(p + i * step + offset);
             }
         }
     }
@@ -349,6 +364,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
         tw.load(bias + coord<MAP>(a, k0), a.window);
     };
     auto step = [&](int k0, unsigned long long live, auto masked) {
+        if (decltype(masked)::value && !__any(last >= k0)) return;         // none of this wave's queries sees a key
         sc[0] = sc[1] = f32x16{};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
@@ -707,7 +723,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     const int i = q0 + 32 * w + col;
     const Seq s = sequence(a, b);
     const int last = last_key(a, s, i);
-    const int u_hi = query_coord<MAP>(a, s.off + q0 + BM - 1), lane_u = u_hi - query_coord<MAP>(a, s.off + i);
+    const int u_hi = query_coord<MAP>(a, s.off + q0 + BM - 1), lane_u = u_hi - query_coord<MAP>(a, s.off + min(i, a.Lq - 1));
     const int px = MAP ? max(s.off + i, 0) % a.width : 0, qx = MAP ? max(s.off + q0 + 32 * w, 0) % a.width : 0;
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
@@ -717,7 +733,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
 
     typename Vec<T>::v8 qf[D / 16], gf[D / 16];
-    float m = 0.f, inv = 0.f, delta = 0.f;
+    // rows behind the last query have probability 0 (and the biases of the last: an entry that no pair has may hold anything)
+    float m = FLT_MAX, inv = 0.f, delta = 0.f;
     {
         const bool ok = i < a.Lq;
         const T* qr = static_cast<const T*>(a.q) + b * a.q_b + (long)i * a.q_l + head * a.q_h;
@@ -750,7 +767,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     if (want)
         for (int t = l; t < 32 * SP; t += 64) moved[w][t] = 0.f;
 
-    const int k_end = key_end(a, s, q0), open = q0 + BM > a.Lq ? 0 : open_end(a, s, q0, k_end);
+    const int k_end = key_end(a, s, q0), open = open_end(a, s, q0, k_end);
     const unsigned k_off = KT::lane_offset(a.k_l), v_off = KT::lane_offset(a.v_l);
     const ColFrag<T, KT::P> kcol(sk);
     KT tk, tv;
@@ -767,6 +784,12 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
         const unsigned long long lv = live >> (4 * h);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            if (decltype(masked)::value && !__any(last >= k0 + 32 * u)) {      // none of this wave's queries sees a key
+                if (want)
+#pragma unroll
+                    for (int cls = 0; cls < CLS; ++cls) hand_over(0.f, carry[cls], part + cls * pitch + k0 + 32 * u);
+                continue;
+            }
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
@@ -859,17 +882,19 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 
 // --- dK, dV ---------------------------------------------------------------------------------------------------------
 // One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers; the queries of all
-// heads that share it stream through LDS 64 at a time, 32 for each wave of a pair, so the sums over those heads stay in
+// heads that share it stream through LDS 64 or 128 at a time, half for each wave of a pair, so the sums over those heads stay in
 // the accumulators (no atomics, one order) and the pair joins at the end.  Keys sit on the lanes (S = Q K^T), P and dS
 // (garbage for padding, whose sums are dropped) are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
 template <class T, int D> struct DkvLds {
-    typedef Tile<T, D, 64> QT;
+    // queries per LDS tile: 128 where the registers hold the next tile (8 x 16 heads of 64 x 2048 bf16: 513 -> 450 us against 64)
+    static constexpr int QB = sizeof(T) == 2 && D <= 64 ? 128 : 64;
+    typedef Tile<T, D, QB> QT;
     static constexpr int TILES = 2 * QT::ELEMS * (int)sizeof(T), JOIN = 2 * 64 * 16 * 4;
     static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
 };
 template <class T, int D, bool MAP>
 __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const Args a) {
-    constexpr int QB = 64;                      // queries per LDS tile
+    constexpr int QB = DkvLds<T, D>::QB;
     typedef Tile<T, D, QB> QT;
     __shared__ __attribute__((aligned(16))) char lds[DkvLds<T, D>::BYTES];
     __shared__ float sb[WindowLds<MAP>::N];
@@ -881,7 +906,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     int unit, rest;
     place(a.B * a.Hkv, nk, a.causal, unit, rest);
     const int b = unit / a.Hkv, kvh = unit % a.Hkv, k0 = rest * KB;
-    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5, u = w >> 1;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63, col = l & 31, h = l >> 5;
     const Seq s = sequence(a, b);
     const int key = k0 + 32 * (w & 1) + col;
     const bool alive = key < s.len && !(a.kpm && a.kpm[(long)b * a.Lk + key]);
@@ -909,23 +934,26 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     const int cut = s.off + i_begin < 0 || s.off + a.Lq > a.N ? blocks
                   : a.causal ? min(blocks, max(0, (k0 + KB - 1 - s.off - i_begin + QB - 1) / QB)) : 0;
     const int hiding = cut < blocks && (a.Lq - i_begin) % QB != 0 ? cut + 1 : cut;
-    auto place_of = [&](int n, int& head, int& i0) {
-        const bool first = n < hiding * a.G;
-        const int per = first ? hiding : blocks - hiding, x = first ? n : n - hiding * a.G, y = x % per;
-        head = kvh * a.G + x / per;
-        i0 = i_begin + (first ? y < cut ? y : blocks - 1 : cut + y) * QB;
-    };
+    // the block to load next: head g, number y of `per` of the kind
+    int g = 0, y = 0, per = hiding > 0 ? hiding : blocks;
+    bool first = hiding > 0;
     QT tq, tg;
     Window tw;
     float rm = 0.f, ri = 0.f, rd = 0.f;
     int rl = -1, ru = 0;
     const unsigned q_off = QT::lane_offset(a.q_l), g_off = QT::lane_offset((long)a.H * D);
-    auto load = [&](int n) {
-        int head, i0;
-        place_of(n, head, i0);
-        const unsigned long long rows = a.Lq - i0 >= 64 ? ~0ull : (1ull << (a.Lq - i0)) - 1;
-        tq.load(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, q_off, rows);
-        tg.load(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, g_off, rows);
+    auto load = [&]() {
+        const int head = kvh * a.G + g, i0 = i_begin + (first ? y < cut ? y : blocks - 1 : cut + y) * QB;
+        if (++y == per) {
+            y = 0;
+            if (++g == a.G && first) {
+                g = 0;
+                first = false;
+                per = blocks - hiding;
+            }
+        }
+        tq.load_first(static_cast<const T*>(a.q) + b * a.q_b + head * a.q_h + (long)i0 * a.q_l, a.q_l, q_off, a.Lq - i0);
+        tg.load_first(static_cast<const T*>(a.d_out) + (((long)b * a.Lq + i0) * a.H + head) * D, (long)a.H * D, g_off, a.Lq - i0);
         const int u_hi = query_coord<MAP>(a, s.off + i0 + QB - 1);
         tw.load(a.bias + (long)head * a.pitch + a.front + a.ncells / 2 + u_lo - u_hi, a.window);
         if (threadIdx.x < QB) {
@@ -939,7 +967,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             ru = u_hi - query_coord<MAP>(a, s.off + i);
         }
     };
-    auto step = [&](auto masked) {
+    auto step = [&](int u, auto masked) {
+        if (decltype(masked)::value && !__any(sl[32 * u + col] >= k0 + 32 * (w & 1))) return;        // none of these queries sees a key
         f32x16 sc = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
@@ -992,10 +1021,11 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
             su[threadIdx.x] = ru;
         }
         __syncthreads();
-        if (n + 1 < steps) load(n + 1);
-        step(masked);
+        if (n + 1 < steps) load();
+#pragma unroll
+        for (int u = 0; u < QB / 32; u += 2) step(u + (w >> 1), masked);
     };
-    if (steps > 0) load(0);
+    if (steps > 0) load();
     int n = 0;
     for (; n < hiding * a.G; ++n) tile(n, Flag<true>());
     for (; n < steps; ++n) tile(n, Flag<false>());
@@ -1006,12 +1036,12 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     for (int t = 0; t < 2 * (D / 32); ++t) {
         f32x16& acc = t < D / 32 ? dk[t % (D / 32)] : dv[t % (D / 32)];
         __syncthreads();
-        if (u == 1) {
+        if (w >= 2) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) join[64 * e] = acc[e];
         }
         __syncthreads();
-        if (u == 0 && key < a.Lk) {
+        if (w < 2 && key < a.Lk) {
             T* out = static_cast<T*>(t < D / 32 ? a.dk : a.dv) + row + 32 * (t % (D / 32)) + 4 * h;
             const float f = t < D / 32 ? a.scale : down<T>();
 #pragma unroll
