@@ -2000,6 +2000,7 @@ class RelativeBuckets:
         packed[2 * up(n):] = start
         packed = packed.to(device)
         self.cells, self.order, self.start = packed[:n], packed[up(n):up(n) + n], packed[2 * up(n):]
+        self.where = packed.get_device()
 
 
 def sequence_buckets(max_len, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
@@ -2035,22 +2036,13 @@ def grid_buckets(height, width, device="cuda"):
     return RelativeBuckets(torch.arange(n), n, height * width, width, device)
 
 
-class _on:
-    """Makes a tensor's device the current one for the launches inside the block."""
-    __slots__ = ("guard",)
-
-    def __init__(self, t):
-        i = t.get_device()
-        here = _current_device() if _current_device is not None else torch.cuda.current_device()
-        self.guard = torch.cuda.device(i) if i != here else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(where, name, *args):
+    """A library call with the current stream of device `where`, which it makes the current one for that."""
+    if _current_device is not None and _current_device() == where:
+        lib.call(name, *args, _st())
+    else:
+        with torch.cuda.device(where):
+            lib.call(name, *args, _st())
 
 
 def _aligned16(t):
@@ -2071,11 +2063,12 @@ def _dense16(t):
 
 def _check_bias_attention(q, k, v, table, buckets, q_offset, kv_len, key_padding_mask):
     where, dtype = q.get_device(), q.dtype            # -1: not on a GPU
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (table, "table"), (buckets.cells, "buckets")):
-        if not t.is_cuda:
-            raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
-        if t.get_device() != where:
-            raise RuntimeError("spot_amd: %s is on %s, q on %s" % (name, t.device, q.device))
+    if where < 0 or k.get_device() != where or v.get_device() != where or table.get_device() != where or buckets.where != where:
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (table, "table"), (buckets.cells, "buckets")):
+            if not t.is_cuda:
+                raise RuntimeError("spot_amd: %s must live on the GPU (no CPU path exists)" % name)
+        raise RuntimeError("spot_amd: q, k, v, table and buckets are on %s, %s, %s, %s and %s"
+                           % (q.device, k.device, v.device, table.device, buckets.cells.device))
     if dtype not in _DTYPE_CODE or k.dtype != dtype or v.dtype != dtype or table.dtype not in _DTYPE_CODE:
         raise RuntimeError("spot_amd: q, k and v have one dtype of float32, bfloat16, float16, the table one of these; got %s, %s, %s, %s"
                            % (dtype, k.dtype, v.dtype, table.dtype))
@@ -2145,7 +2138,7 @@ def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_p
                buckets.width, 1 if causal else 0, mode, off)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     strides = (*qs, *ks, *vs)
-    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     out_lo = torch.empty_like(out) if train and code else None
     stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device) if train else None
     need = _bias_ws_bytes("spot_bias_attention_fwd_ws_bytes", numbers[:13], False)
@@ -2154,8 +2147,7 @@ def _bias_attention_fwd(q, k, v, table, buckets, causal, q_offset, kv_len, key_p
         (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),
          _a(off_t), _a(kv_len), _a(kpm), 0, 0, 0, 0, 0, 0, 0), strides, numbers, scale, _a(ws), need)
     lib.keep(q, k, v, out, out_lo, stats, table, buckets.cells, off_t, kv_len, kpm, ws)
-    with _on(q):
-        lib.call("spot_bias_attention_fwd", C.byref(d), _st())
+    _launch(q.get_device(), "spot_bias_attention_fwd", C.byref(d))
     return out, out_lo, stats, (strides, numbers, scale), (q, k, v, table, off_t, kv_len, kpm)
 
 
@@ -2181,17 +2173,17 @@ class BiasAttentionFn(_Fn):
         buckets, want = ctx.buckets, ctx.needs_input_grad
         dout = _dense16(dout)
         dev = q.device
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=dev) for _ in range(2)) if want[1] or want[2] else (None, None)
-        dtable = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[3] else None
+        new = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)
+        dq = new(q)
+        dk, dv = (new(k), new(k)) if want[1] or want[2] else (None, None)
+        dtable = new(table) if want[3] else None
         need = _bias_ws_bytes("spot_bias_attention_bwd_ws_bytes", numbers[:13], want[3])
         ws = torch.empty((need,), dtype=torch.uint8, device=dev)
         d = _bias_desc(
             (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _a(out_lo), _a(stats), table.data_ptr(), buckets.cells.data_ptr(),
              _a(off_t), _a(kv_len), _a(kpm), dout.data_ptr(), dq.data_ptr(), _a(dk), _a(dv), _a(dtable), buckets.order.data_ptr(),
              buckets.start.data_ptr()), strides, numbers, scale, ws.data_ptr(), need)
-        with _on(q):
-            lib.call("spot_bias_attention_bwd", C.byref(d), _st())
+        _launch(q.get_device(), "spot_bias_attention_bwd", C.byref(d))
         return (dq if want[0] else None, dk if want[1] else None, dv if want[2] else None, dtable, None, None, None, None, None, None)
 
 
@@ -2266,8 +2258,7 @@ def top_logits(logits, k):
     if N:
         need = _rows_ws_bytes("spot_top_logits_ws_bytes", code, N, V, k)
         ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
-        with _on(x):
-            lib.call("spot_top_logits", code, _p(x), ld, N, V, k, _p(values), _p(indices), _p(ws), need, _st())
+        _launch(x.get_device(), "spot_top_logits", code, _p(x), ld, N, V, k, _p(values), _p(indices), _p(ws), need)
     return values, indices
 
 
@@ -2286,9 +2277,8 @@ class TopLogitDistillationFn(_Fn):
             ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
             norm = _a(kept)
             lib.keep(kept)
-            with _on(x):
-                lib.call("spot_top_distill_fwd", code, _p(x), ld, _DTYPE_CODE[values.dtype], _p(values), _p(indices), N, V, k, T,
-                         _p(loss), norm, norm + 8 * N if train else None, _p(ws), need, _st())
+            _launch(x.get_device(), "spot_top_distill_fwd", code, _p(x), ld, _DTYPE_CODE[values.dtype], _p(values), _p(indices), N, V,
+                    k, T, _p(loss), norm, norm + 8 * N if train else None, _p(ws), need)
         if train:
             ctx.save_for_backward(x, indices, kept)
             ctx.dims = (student.shape, N, V, k, ld, T)
@@ -2303,9 +2293,8 @@ class TopLogitDistillationFn(_Fn):
         if N:
             dloss = dloss.contiguous()
             norm = kept.data_ptr()
-            with _on(x):
-                lib.call("spot_top_distill_bwd", _DTYPE_CODE[x.dtype], _p(x), ld, _p(indices), norm, norm + 8 * N, _p(dloss), N, V,
-                         k, T, _p(dx), _st())
+            _launch(x.get_device(), "spot_top_distill_bwd", _DTYPE_CODE[x.dtype], _p(x), ld, _p(indices), norm, norm + 8 * N, _p(dloss),
+                    N, V, k, T, _p(dx))
         return dx, None, None, None
 
 

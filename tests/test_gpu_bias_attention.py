@@ -399,11 +399,15 @@ def test_gradients_wanted_of_some(ops):
         assert torch.equal(got, want[i]), i
 
 
-def test_two_streams_and_no_grad(ops):
-    b = ops.sequence_buckets(300, 16, 64, device=DEV)
+@pytest.mark.parametrize("Lq", [1, 300])
+def test_two_streams_and_no_grad(ops, Lq):
+    b = ops.sequence_buckets(2000, 16, 64, device=DEV)
     table = torch.randn(16, 4, device=DEV)
-    xs = [[torch.randn(2, 300, 4, 32, device=DEV) for _ in range(3)] for _ in range(2)]
-    want = [ops.bias_attention(*x, table, b) for x in xs]
+    xs = [[torch.randn(2, n, 4, 32, device=DEV) for n in (Lq, 2000, 2000)] for _ in range(2)]
+    with torch.no_grad():
+        want = [ops.bias_attention(*x, table.requires_grad_(), b) for x in xs]
+    table.requires_grad_(False)
+    assert not want[0].requires_grad
     s = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     got = []

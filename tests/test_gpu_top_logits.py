@@ -178,6 +178,35 @@ def test_distillation_absent_double_and_extreme_entries(ops, t):
     assert loss.item() == math.inf and torch.isfinite(dx).all() and abs(dx[0, 3].item() + 0.5) < 1e-6
 
 
+def test_gradient_larger_than_the_last_level_cache(ops):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    student = torch.randn(70, 1000003, generator=gen, device=DEV)          # 280 MB
+    values, at = ops.top_logits(student, 20)
+    leaf = student.requires_grad_()
+    g = torch.rand(70, generator=gen, device=DEV)
+    loss = ops.top_logit_distillation(leaf, values, at, 2.0)
+    dx, = torch.autograd.grad(loss, leaf, g)
+    for i in range(0, 70, 10):
+        want, tol, wdx, tdx = distill64(student[i:i + 1].detach(), values[i:i + 1], at[i:i + 1], 2.0, g[i:i + 1])
+        assert ((loss[i:i + 1].detach().double() - want).abs() <= tol).all() and ((dx[i:i + 1].double() - wdx).abs() <= tdx).all()
+
+
+def test_two_streams(ops):
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    xs = [torch.randn(3, 60000, generator=gen, device=DEV) for _ in range(2)]
+    want = [(*ops.top_logits(x, 30), ops.top_logit_distillation(x, *ops.top_logits(x, 30), 2.0)) for x in xs]
+    s = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for st, x in zip(s, xs):
+        with torch.cuda.stream(st):
+            v, at = ops.top_logits(x, 30)
+            got.append((v, at, ops.top_logit_distillation(x, v, at, 2.0)))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_distillation_views_and_empty(ops):
     gen = torch.Generator(device=DEV).manual_seed(6)
     for T in (torch.float32, torch.bfloat16):
