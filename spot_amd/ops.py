@@ -1989,7 +1989,6 @@ class RelativeBuckets:
                                % (tuple(cells.shape), max_len, width, n))
         if num_buckets < 1 or int(cells.min()) < 0 or int(cells.max()) >= num_buckets:
             raise RuntimeError("spot_amd: bucket cells from %d to %d for %d buckets" % (int(cells.min()), int(cells.max()), num_buckets))
-        self.num_buckets, self.width, self.max_len = int(num_buckets), int(width), int(max_len)
         start = torch.zeros(num_buckets + 1, dtype=torch.int64)
         start[1:] = torch.bincount(cells, minlength=num_buckets).cumsum(0)
         # one copy to the device: cells | order | start, each at a border of 16 bytes
@@ -1999,8 +1998,12 @@ class RelativeBuckets:
         packed[up(n):up(n) + n] = torch.argsort(cells, stable=True)
         packed[2 * up(n):] = start
         packed = packed.to(device)
-        self.cells, self.order, self.start = packed[:n], packed[up(n):up(n) + n], packed[2 * up(n):]
-        self.where = packed.get_device()
+        self._set(packed[:n], packed[up(n):up(n) + n], packed[2 * up(n):], num_buckets, max_len, width)
+
+    def _set(self, cells, order, start, num_buckets, max_len, width):
+        self.cells, self.order, self.start = cells, order, start
+        self.num_buckets, self.max_len, self.width = int(num_buckets), int(max_len), int(width)
+        self.where = cells.get_device()
 
 
 def sequence_buckets(max_len, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
@@ -2031,9 +2034,14 @@ def grid_buckets(height, width, device="cuda"):
     (dy + height - 1) * (2 width - 1) + dx + width - 1."""
     if height < 1 or width < 1:
         raise RuntimeError("spot_amd: grid_buckets of a %d x %d map" % (height, width))
+    if width > 512 or height * width > 1 << 20:
+        raise RuntimeError("spot_amd: grid_buckets of a %d x %d map (up to 512 columns, 2^20 tokens)" % (height, width))
     # u runs over whole rows of 2 width - 1 column offsets, from (1 - height, 1 - width) on: the bucket is the cell
     n = (2 * height - 1) * (2 * width - 1)
-    return RelativeBuckets(torch.arange(n), n, height * width, width, device)
+    each = torch.arange(n + 1, dtype=torch.int32, device=device)
+    plan = RelativeBuckets.__new__(RelativeBuckets)
+    plan._set(each[:n], each[:n], each, n, height * width, width)
+    return plan
 
 
 def _launch(where, name, *args):

@@ -49,7 +49,7 @@ def test_bucket_plans_refuse():
     for args in ((0, 32, 128), (10, 2, 128), (10, 32, 8), (10, 0, 128)):
         with pytest.raises(RuntimeError, match="spot_amd"):
             ops.sequence_buckets(*args, device="cpu")
-    for args in ((0, 4), (4, 0)):
+    for args in ((0, 4), (4, 0), (4, 513), (1 << 19, 4)):
         with pytest.raises(RuntimeError, match="spot_amd"):
             ops.grid_buckets(*args, device="cpu")
 
