@@ -17,7 +17,7 @@
 // that u(key) - u(query) stands for one offset in either; `bias` is the table spread out by that difference, per head
 // and times log2 e.  A tile of queries x keys meets a window of it, which goes to LDS with the tile.
 //
-// Statistics.  A row's reference (its maximum or a little less) and reciprocal sum are kept apart: as one number (their
+// Statistics.  A row's reference (its maximum or less) and reciprocal sum are kept apart: as one number (their
 // log-sum-exp) a row of scores near the type's lowest value would lose the sum.  A row that sees no key has reference 0
 // and reciprocal 0: its output and gradients are zero.
 #pragma once
@@ -64,7 +64,7 @@ template <class T> struct Vec {
     // probabilities become operands times 2^SHIFT: a half float is subnormal from 2^-14 on, and the rows of a thousand
     // keys hold little else
     static constexpr int SHIFT = 0;
-    // a row's reference may fall behind its maximum by 2^LAG before the sums are scaled again
+    // a row's scores may rise 2^LAG above the maximum its reference was taken from before the sums are scaled again
     static constexpr int LAG = 8;
     static constexpr int PAD = 16 / sizeof(T);      // LDS rows are padded by 16 bytes: eight lanes' 16-byte reads meet all banks
 };
@@ -266,8 +266,13 @@ __device__ __forceinline__ void place(int units, int per_unit, bool longest, int
     rest = longest ? j / here : j % per_unit;
 }
 
-// The softmax of a lane's row, tile by tile: the reference moves, and what was summed is scaled, where a score of NT
-// tiles is more than LAG above it; then the scores become 2^(s - reference + SHIFT) and join the sum.
+// The softmax of a lane's row, tile by tile, against a reference SHIFT under a score that was its maximum: the reference
+// moves, and what was summed is scaled, where a score of NT tiles is more than LAG above that; then the scores become
+// 2^(s - reference) and join the sum.  Far from zero 32 bits do not hold such a difference (from 2^27 on 12 becomes 16,
+// which no half float follows), and the reference is the maximum itself.
+template <class T> __device__ __forceinline__ float reference(float mx) {
+    return Vec<T>::SHIFT && fabsf(mx) < 0x1p20f ? mx - Vec<T>::SHIFT : mx;
+}
 template <class T, int NT, int NO>
 __device__ __forceinline__ void rescale(const f32x16* sc, float& m, float& sum, f32x16* o) {
     float mx = sc[0][0];
@@ -276,8 +281,8 @@ __device__ __forceinline__ void rescale(const f32x16* sc, float& m, float& sum, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any(mx > m + Vec<T>::LAG)) {
-        const float to = fmaxf(mx, m), f = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+    if (__any(mx - m > Vec<T>::LAG + Vec<T>::SHIFT)) {
+        const float to = fmaxf(reference<T>(mx), m), f = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
         sum *= f;
 #pragma unroll
         for (int t = 0; t < NO; ++t) o[t] *= f;
@@ -285,7 +290,7 @@ __device__ __forceinline__ void rescale(const f32x16* sc, float& m, float& sum, 
     }
 }
 template <class T, int NT> __device__ __forceinline__ void exponentials(f32x16* sc, float m, float& sum) {
-    const float low = (m == -INFINITY ? 0.f : m) - Vec<T>::SHIFT;
+    const float low = m == -INFINITY ? 0.f : m;
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -308,10 +313,10 @@ template <class T> __device__ __forceinline__ void store_out(const Args& a, long
     *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + at) = hi;
     if (a.out_lo) *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out_lo) + at) = rem;
 }
-template <class T> __device__ __forceinline__ void store_stats(const Args& a, int b, int head, int i, float m, float inv) {
+__device__ __forceinline__ void store_stats(const Args& a, int b, int head, int i, float m, float inv) {
     float* st = a.stats + (((long)b * a.H + head) * a.Lq + i) * 2;
     st[0] = m == -INFINITY ? 0.f : m;
-    st[1] = inv * up<T>();
+    st[1] = inv;
 }
 
 // --- forward ------------------------------------------------------------------------------------------------------
@@ -422,7 +427,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
             const float x[4] = {o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
             store_out<T>(a, row + 32 * t + 8 * g + 4 * h, x, inv);
         }
-    if (a.stats && h == 0) store_stats<T>(a, b, head, i, m, inv);
+    if (a.stats && h == 0) store_stats(a, b, head, i, m, inv);
 }
 
 // --- forward for few rows -------------------------------------------------------------------------------------------
@@ -641,7 +646,7 @@ __global__ __launch_bounds__((64 * FewLds<T, D>::NW), (FewLds<T, D>::NW / 4)) vo
             a.few_ml[(part * 32 + r) * 2] = top;
             a.few_ml[(part * 32 + r) * 2 + 1] = total;
         } else if (a.stats) {
-            store_stats<T>(a, b, fr.head, fr.i, top, inv);
+            store_stats(a, b, fr.head, fr.i, top, inv);
         }
     }
 }
@@ -672,7 +677,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int e = 0; e < D / 8; e += 4) store_out<T>(a, (((long)b * a.Lq + f.i) * a.H + f.head) * D + d0 + e, x + e, inv);
-    if (a.stats && d0 == 0) store_stats<T>(a, b, f.head, f.i, top, inv);
+    if (a.stats && d0 == 0) store_stats(a, b, f.head, f.i, top, inv);
 }
 
 // --- dQ and the sums along the offsets ------------------------------------------------------------------------------

@@ -493,3 +493,47 @@ def test_refusals(ops):
     first, = torch.autograd.grad(out.sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         first.sum().backward()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Lq,L", [(3, 300), (300, 300), (3000, 64)])
+@pytest.mark.parametrize("low,high", [(0.0, 0.0), (-4.0e5, -4.0e5), (-2.0 ** 25, -2.0 ** 25 + 12), (-2.0 ** 26, -2.0 ** 26 + 12), (-3.4e38, -3.4e38),
+                                      (2.0 ** 26, 2.0 ** 26 + 12), (3.0e38, 3.0e38), (-1.0e6, -2.0), (-3.4e38, 5.0)])
+def test_far_away_references(ops, t, Lq, L, low, high):
+    """Scores that are biases alone, far from zero: entries of `high` share a row evenly, those of `low` count next to
+    nothing.  (log2 e)(high - low) = 17.3 becomes 16 or 24 in the steps of 8 and 16 that 32 bits have there: such a key has a
+    weight of 2^-16 at most, and the bounds allow twice that for each."""
+    T = TYPES[t]
+    n = max(Lq, L)
+    cells = (torch.arange(2 * n - 1) % 5 == 0).long()            # every fifth offset has the high entry
+    b = ops.RelativeBuckets(cells, 2, n, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    k, v, g = (torch.randn(2, m, 2, 64, generator=gen, device=DEV).to(T) for m in (L, L, Lq))
+    q = torch.zeros(2, Lq, 2, 64, device=DEV, dtype=T)
+    table = torch.tensor([[low] * 2, [high] * 2], device=DEV)
+    leaves = [x.requires_grad_() for x in (q, k, v, table)]
+    out = ops.bias_attention(*leaves, b)
+    got = (out, *torch.autograd.grad(out, leaves, g))
+    bucket = b.cells.long()[torch.arange(L, device=DEV)[None] - torch.arange(Lq, device=DEV)[:, None] + n - 1]
+    W = torch.where(bucket == 1, 1.0, 1.0 if low == high else 0.0).double()
+    P = (W / W.sum(1, keepdim=True))[None, None]
+    K, V, G = (x.detach().double().permute(0, 2, 1, 3) for x in (k, v, g))
+    O, dP = P @ V, G @ V.transpose(2, 3)
+    dS = P * (dP - (G * O).sum(3, keepdim=True))
+    # a probability: its rounding, the low entries' weight 2^-16 against at least one high one in five, sums of L terms
+    u = 0.0 if t == "f32" else half_step(T)
+    light = 0.0 if low == high else 2.0 ** -16 * 5
+    tP = P * (u + 2 * light + (L + 16) * U32) + light * 5 / L + (2.0 ** -37 if t == "f16" else 0)
+    tO = tP @ V.abs() + half_step(T) * O.abs()
+    size = G.abs() @ V.abs().transpose(2, 3)
+    tS = tP * (dP.abs() + (G.abs() * O.abs()).sum(3, keepdim=True)) + P * ((G.abs() * tO).sum(3, keepdim=True) + 70 * U32 * size) + u * dS.abs() + \
+        (2.0 ** -25 if t == "f16" else 0)
+    scale = 1 / 8
+    back = lambda x: x.permute(0, 2, 1, 3)
+    by = lambda x: torch.stack([(x * (bucket == i)).sum((0, 2, 3)) for i in (0, 1)])
+    sums = (Lq + L) * U32
+    want = [(O, tO), (scale * dS @ K, scale * (tS + sums * dS.abs()) @ K.abs()), (torch.zeros_like(K), torch.zeros_like(K)),
+            (P.transpose(2, 3) @ G, (tP + sums * P).transpose(2, 3) @ G.abs())]
+    for x, (y, e), name in zip(got, want, ("out", "dq", "dk", "dv")):
+        inside(x, back(y), back(e + half_step(T) * y.abs()), name)
+    inside(got[4], by(dS), by(tS + 256 * U32 * dS.abs()), "dtable")
