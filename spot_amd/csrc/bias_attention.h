@@ -132,6 +132,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
     Seq s;
     s.len = a.kv_len ? min(max(a.kv_len[b], 0), a.Lk) : a.Lk;
     s.off = a.off_mode == 2 ? s.len - a.Lq : a.off_mode == 1 ? min(max(a.q_offsets[b], -(1 << 24)), 1 << 24) : a.off;
+    if (a.causal) s.len = min(s.len, max(s.off + a.Lq, 0));        // no query sees what stands behind the last one
     return s;
 }
 // The last key a query may see: none (-1) for rows behind the last query and for positions outside of the buckets' range

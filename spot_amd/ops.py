@@ -2208,8 +2208,8 @@ def bias_attention(q, k, v, table, buckets, causal=False, q_offset=0, kv_len=Non
     an int32 tensor [B], or "end" - the last Lq of a sequence's keys, as when new tokens attend to a cache that holds
     them already.  A query before position 0, or behind buckets.max_len, sees no key.
     Hidden are keys from kv_len[b] (int32 [B]) on, keys whose key_padding_mask [B, Lk] (bool or uint8) is set, and with
-    ``causal`` keys behind the query.  What kv_len and the mask hide may hold anything; keys that only ``causal`` hides
-    have to be finite.  A bias of -inf hides a key, too; the type's lowest value does not: a row of nothing else is
+    ``causal`` keys behind the query.  What kv_len and the mask hide, and with ``causal`` what stands behind a sequence's
+    last query, may hold anything; a key that is hidden from some of the queries only has to be finite.  A bias of -inf hides a key, too; the type's lowest value does not: a row of nothing else is
     averaged.  A query that sees no key has output 0 and gradients 0.
 
     Scores, probabilities, sums and the table's gradient are 32 bits or more; products of 16-bit inputs take

@@ -537,3 +537,31 @@ def test_far_away_references(ops, t, Lq, L, low, high):
     for x, (y, e), name in zip(got, want, ("out", "dq", "dk", "dv")):
         inside(x, back(y), back(e + half_step(T) * y.abs()), name)
     inside(got[4], by(dS), by(tS + 256 * U32 * dS.abs()), "dtable")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,Lq,off", [(1, 1, 5), (2, 1, 0), (2, 7, 57), (2, 7, [0, 60]), (1, 100, 33), (60, 100, 33), (60, 64, 0), (40, 130, 100), (2, 4, [-9, 12])])
+def test_room_behind_the_last_query_may_hold_anything(ops, t, B, Lq, off):
+    """A cache with free room: causal attention without lengths sees nothing of it, and its gradient there is zero."""
+    T, Lk, H, Hkv, D = TYPES[t], 300, 4, 2, 64
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    q, k, v, g = (torch.randn(B, n, h, D, generator=gen, device=DEV).to(T) for n, h in ((Lq, H), (Lk, Hkv), (Lk, Hkv), (Lq, H)))
+    table = torch.randn(16, H, generator=gen, device=DEV)
+    b = ops.sequence_buckets(Lk, 16, 64, bidirectional=False, device=DEV)
+    offs = torch.tensor(off if isinstance(off, list) else [off] * B, dtype=torch.int32, device=DEV)
+    room = torch.arange(Lk, device=DEV)[None] >= (offs.long() + Lq)[:, None]
+    arg = offs if isinstance(off, list) else off
+    res = []
+    for fill in (0.0, math.nan, math.inf):
+        leaves = [x.requires_grad_() for x in (q.detach(), k.detach().masked_fill(room[:, :, None, None], fill),
+                                               v.detach().masked_fill(room[:, :, None, None], -fill), table.detach())]
+        out = ops.bias_attention(*leaves, b, causal=True, q_offset=arg)
+        res.append((out.detach(), *torch.autograd.grad(out, leaves, g)))
+    want = reference(q, k.masked_fill(room[:, :, None, None], 0), v.masked_fill(room[:, :, None, None], 0), table, b.cells, 0, Lk, True, offs,
+                     torch.full((B,), Lk, device=DEV), None, 1 / 8, g)
+    for got in res:
+        for x, y, (w, tol), name in zip(got, res[0], want, ("out", "dq", "dk", "dv", "dtable")):
+            assert torch.equal(x, y), name
+            inside(x, w, tol, name)
+            if name in ("dk", "dv"):
+                assert not x[room].any(), name
