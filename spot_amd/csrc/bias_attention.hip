@@ -182,8 +182,13 @@ static int check(const spot_bias_attn_desc* d, bool backward) {
                    "spot_bias_attention: rows of a head have to be less than 64 MB apart, in rising order");
     SPOT_CHECK_ARG(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && aligned16(d->out) && aligned16(d->out_lo),
                    "spot_bias_attention: q, k, v, out and out_lo have to be 16-byte aligned");
-    SPOT_CHECK_ARG((long)d->B * d->H * ((d->Lq + 31) / 32) < (1L << 31) && (long)d->B * d->Hkv * ((d->Lk + 31) / 32) < (1L << 31),
-                   "spot_bias_attention: B %d, H %d, Lq %d, Lk %d need too many workgroups", d->B, d->H, d->Lq, d->Lk);
+    // a grid holds fewer than 2^32 threads: 512 or 256 per workgroup of the forward, 256 of the others, as many per bucket
+    const Few f = few(*d);
+    const long fwd = f.use ? 512L * d->B * d->Hkv * f.tiles * f.splits : 256L * d->B * d->H * ((d->Lq + BM - 1) / BM);
+    const long bwd = 256L * d->B * (d->H * ((d->Lq + BM - 1L) / BM) > d->Hkv * ((d->Lk + KB - 1L) / KB)
+                                        ? d->H * ((d->Lq + BM - 1L) / BM) : d->Hkv * ((d->Lk + KB - 1L) / KB));
+    SPOT_CHECK_ARG(fwd < (1L << 32) && (!backward || (bwd < (1L << 32) && d->num_buckets < (1 << 24))),
+                   "spot_bias_attention: B %d, H %d, Lq %d, Lk %d, %d buckets need too many workgroups", d->B, d->H, d->Lq, d->Lk, d->num_buckets);
     if (backward) {
         SPOT_CHECK_ARG(d->Lq == 0 || (d->stats && d->d_out && d->dq), "spot_bias_attention_bwd: stats, d_out and dq are needed");
         SPOT_CHECK_ARG((d->dk == nullptr) == (d->dv == nullptr), "spot_bias_attention_bwd: dk and dv come together");

@@ -4,6 +4,8 @@
 // 5 to 10 lane operations each, which is under the vector rate at the card's copy bandwidth.
 #include <float.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "../../include/spot_hip.h"
 
@@ -251,12 +253,21 @@ int top_run(const void* x, long ld, int N, int V, int k, void* values, int* indi
     return top_launch<T>(wv, (long)pieces * k, N, pieces * k, 1, k, wi, static_cast<T*>(values), indices, stream);
 }
 
+// The same for the loss: about 1024 workgroups where the rows are few, no piece under 4096 elements.
+int distill_pieces(int N, int V) {
+    const long fill = (1024 + N - 1) / N, most = V / 4096;
+    const long pieces = fill < most ? fill : most;
+    return pieces < 1 ? 1 : (int)pieces;
+}
+
 int check_rows(const char* name, int dtype, int N, int V, int k, long ld) {
     SPOT_CHECK_ARG(dtype >= F32 && dtype <= F16, "%s: dtype %d is none of 0 (f32), 1 (bf16), 2 (f16)", name, dtype);
     SPOT_CHECK_ARG(N >= 0 && V >= 1 && V <= SPOT_TOP_LOGITS_MAX_V && ld >= V, "%s: %d rows of %d logits (1 to %d), %ld apart", name, N, V,
                    SPOT_TOP_LOGITS_MAX_V, ld);
     SPOT_CHECK_ARG(k >= 1 && k <= KMAX, "%s: k = %d is not in 1 .. %d", name, k, KMAX);
-    SPOT_CHECK_ARG((long)N * ((V + 2047) / 2048) < (1L << 31), "%s: %d rows of %d logits need too many workgroups", name, N, V);
+    // a grid holds fewer than 2^32 threads
+    const long pieces = N == 0 ? 0 : k <= V ? std::max(top_pieces_of(dtype, N, V, k), distill_pieces(N, V)) : distill_pieces(N, V);
+    SPOT_CHECK_ARG(N * pieces * NT < (1L << 32), "%s: %d rows of %d logits need too many workgroups", name, N, V);
     return SPOT_OK;
 }
 
@@ -464,13 +475,6 @@ template <class T, bool PAST_CACHE> __global__ __launch_bounds__(NT) void distil
             }
         if (first) dx[at] = (T)(g * (inv * __builtin_amdgcn_exp2f(fmaf((float)x[at], a.c, -mc)) - p));
     }
-}
-
-// Pieces per row: about 1024 workgroups where the rows are few, no piece under 4096 elements.
-int distill_pieces(int N, int V) {
-    const long fill = (1024 + N - 1) / N, most = V / 4096;
-    const long pieces = fill < most ? fill : most;
-    return pieces < 1 ? 1 : (int)pieces;
 }
 
 template <class T> int distill_fwd(Distill& a, hipStream_t stream) {

@@ -108,3 +108,25 @@ def test_rows_refuse():
         assert l.spot_top_distill_fwd(*a, p, p, p, None, 0, None) < 0 and b"spot_top_distill" in l.spot_last_error(), a
     assert l.spot_top_distill_bwd(0, p, 10, None, p, p, p, 1, 10, 2, 1.0, p, None) < 0
     assert l.spot_top_logits(0, None, 10, 0, 10, 2, None, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(B=1 << 23, H=1, Hkv=1, Lq=1), dict(B=1 << 24, H=4, Hkv=2, Lq=64, max_len=64), dict(B=1 << 20, H=1 << 12, Hkv=1, Lq=1 << 10, max_len=1 << 10)])
+def test_grids_that_are_too_large(kw):
+    from spot_amd import lib
+    l = lib.load()
+    n = C.c_long(-1)
+    assert l.spot_bias_attention_fwd_ws_bytes(C.byref(_desc(**kw)), C.byref(n)) < 0 and b"too many workgroups" in l.spot_last_error()
+    assert l.spot_bias_attention_fwd(C.byref(_desc(**kw)), None) < 0
+
+
+def test_grids_that_are_too_large_for_a_backward_pass_or_rows():
+    from spot_amd import lib
+    l = lib.load()
+    n = C.c_long(-1)
+    for kw in (dict(B=1 << 20, H=32, Hkv=32, Lq=100, max_len=100), dict(num_buckets=1 << 24), dict(B=1 << 18, Lk=1 << 12, max_len=1 << 12, H=2, Hkv=1, Lq=1)):
+        assert l.spot_bias_attention_bwd(C.byref(_desc(ws=4096, ws_bytes=1 << 60, **kw)), None) < 0
+        assert b"too many workgroups" in l.spot_last_error(), kw
+    for N, V, k in ((1 << 24, 10, 2), (1 << 20, 1 << 20, 2), (1 << 24, 1, 1)):
+        for query in ("spot_top_logits_ws_bytes", "spot_top_distill_ws_bytes"):
+            assert getattr(l, query)(0, N, V, k, C.byref(n)) < 0 and b"too many workgroups" in l.spot_last_error(), (N, V)
+    assert l.spot_top_logits_ws_bytes(0, (1 << 24) - 1, 10, 2, C.byref(n)) == 0 and n.value == 0
