@@ -682,33 +682,44 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
 }
 
 // --- dQ and the sums along the offsets ------------------------------------------------------------------------------
-// The forward's split.  The table's gradient is the sum of dS along each offset key - query: a wave writes a 32x32 tile
-// of dS to its own LDS with row k moved k places to the left, so that a column holds one offset, and each lane sums one
-// of the 63 columns (the places around the moved rows are zero and stay so).  The offsets of the next key tile of the
-// same wave are 32 further: what 32 lanes hold then is finished, and 32 sums are written per tile.  (LDS float additions
-// by atomics, one per element, took 145 cycles per wave instruction and 60 % of the kernel.)  On a map an offset stands
-// for two different column offsets, inside a row and around its end: two sets of sums.
-constexpr int SP = 73;                          // pitch of a moved row: the wave's halves, four rows apart, meet other banks
+// The forward's split.  The table's gradient is the sum of dS along each offset key - query: a wave takes the keys of its
+// dS tiles one after the other, the sums so far move up by one lane, and the key's row is added in lanes 0 .. 31.  So a
+// sum meets every query of the wave, and what has left them is finished: after 32 keys lanes 32 .. 63 hold 32 finished
+// sums, which are written.  A row is brought into the lower lanes, zeros above it, by one exchange of the wave's halves for
+// two rows; moving and adding are one instruction.  On a map an offset stands for two different column offsets, inside a
+// row and around its end: two sets of sums.
 __device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 32; }
-// lane t: the sum of offset 31 - t
-__device__ __forceinline__ float offset_sums(const f32x16& x, float* lds) {
-    const int l = threadIdx.x & 63, h = l >> 5;
-    float* to = lds + 4 * h * SP + (l & 31) + 31 - 4 * h;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) to[acc_row(e, 0) * (SP - 1)] = x[e];
-    wave_fence();
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 32; ++k) s[k & 1] += lds[k * SP + l];
-    wave_fence();
-    return s[0] + s[1];
+// x's lower half in both lanes' places: [low, 0] and [high, 0]
+__device__ __forceinline__ void halves(float x, float& low, float& high) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), 0u, false, false);
+    low = __uint_as_float(y[0]);
+    high = __uint_as_float(y[1]);
 }
-// `before`: this lane's sum of the key tile before, whose offsets are 32 smaller
-__device__ __forceinline__ void hand_over(float now, float& before, float* out) {
+// lane t: the sum of offset 31 - t over a tile, joined to the sums before it, whose offsets were 32 smaller
+__device__ __forceinline__ float offset_sums(const f32x16& x, float t) {
+    auto next = [&](float row) {
+        t = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(t), 0x138 /* lane - 1 */, 0xf, 0xf, true)) + row;
+    };
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        float low[4], high[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) halves(x[4 * g + e], low[e], high[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next(low[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next(high[e]);
+    }
+    return t;
+}
+// the same of a tile of zeros
+__device__ __forceinline__ float move_on(float t) {
+    const auto y = __builtin_amdgcn_permlane32_swap(0u, __float_as_uint(t), false, false);
+    return __uint_as_float(y[0]);
+}
+__device__ __forceinline__ void write_finished(float t, float* out) {
     const int l = threadIdx.x & 63;
-    const float x = now + __shfl_xor(before, 32);
-    if (l >= 31 && l < 63) out[62 - l] = x;
-    before = now;
+    if (l >= 32) out[63 - l] = t;
 }
 
 template <class T, int D, bool MAP>
@@ -719,7 +730,6 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
     __shared__ float sb[WindowLds<MAP>::N];
     __shared__ __attribute__((aligned(16))) int su[BN], sx[BN];
-    __shared__ float moved[4][32 * SP];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
     place(a.B * a.Hkv, a.G * nq, a.causal, unit, rest);
@@ -769,9 +779,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     f32x16 dq[D / 32];
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) dq[t] = f32x16{};
-    float carry[CLS] = {};
-    if (want)
-        for (int t = l; t < 32 * SP; t += 64) moved[w][t] = 0.f;
+    float sums[CLS] = {};
 
     const int k_end = key_end(a, s, q0), open = open_end(a, s, q0, k_end);
     const unsigned k_off = KT::lane_offset(a.k_l), v_off = KT::lane_offset(a.v_l);
@@ -793,7 +801,10 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
             if (decltype(masked)::value && !__any(last >= k0 + 32 * u)) {      // none of this wave's queries sees a key
                 if (want)
 #pragma unroll
-                    for (int cls = 0; cls < CLS; ++cls) hand_over(0.f, carry[cls], part + cls * pitch + k0 + 32 * u);
+                    for (int cls = 0; cls < CLS; ++cls) {
+                        sums[cls] = move_on(sums[cls]);
+                        write_finished(sums[cls], part + cls * pitch + k0 + 32 * u);
+                    }
                 continue;
             }
             f32x16 sc = {}, dp = {};
@@ -816,33 +827,32 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
                 }
             }
             if (want) {
-                float* out = part + k0 + 32 * u;
+                const int kx = MAP ? __builtin_amdgcn_readfirstlane(sx[32 * u]) : 0;
                 if (!MAP) {
-                    hand_over(offset_sums(dp, moved[w]), carry[0], out);
+                    sums[0] = offset_sums(dp, sums[0]);
+                } else if (qx + 31 < a.width && kx + 31 < a.width) {
+                    // queries and keys of one row each: the offset decides whether it goes around the row's end
+                    const float t = offset_sums(dp, 0.f);
+                    const bool in = kx - qx + 31 - l >= 0;
+                    sums[0] = move_on(sums[0]) + (in ? t : 0.f);
+                    sums[CLS - 1] = move_on(sums[CLS - 1]) + (in ? 0.f : t);
                 } else {
-                    const int kx = __builtin_amdgcn_readfirstlane(sx[32 * u]);
-                    if (qx + 31 < a.width && kx + 31 < a.width) {
-                        // queries and keys of one row each: the offset decides whether it goes around the row's end
-                        const float t = offset_sums(dp, moved[w]);
-                        const bool in = kx - qx + 31 - l >= 0;
-                        hand_over(in ? t : 0.f, carry[0], out);
-                        hand_over(in ? 0.f : t, carry[CLS - 1], out + (CLS - 1) * pitch);
-                    } else {
-                        f32x16 around = {}, inside = dp;
+                    f32x16 around = {}, inside = dp;
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int4 x = *reinterpret_cast<const int4*>(sx + 32 * u + 8 * g + 4 * h);
+                    for (int g = 0; g < 4; ++g) {
+                        const int4 x = *reinterpret_cast<const int4*>(sx + 32 * u + 8 * g + 4 * h);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if ((e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w) < px) {
-                                    around[4 * g + e] = dp[4 * g + e];
-                                    inside[4 * g + e] = 0.f;
-                                }
-                        }
-                        hand_over(offset_sums(inside, moved[w]), carry[0], out);
-                        hand_over(offset_sums(around, moved[w]), carry[CLS - 1], out + (CLS - 1) * pitch);
+                        for (int e = 0; e < 4; ++e)
+                            if ((e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w) < px) {
+                                around[4 * g + e] = dp[4 * g + e];
+                                inside[4 * g + e] = 0.f;
+                            }
                     }
+                    sums[0] = offset_sums(inside, sums[0]);
+                    sums[CLS - 1] = offset_sums(around, sums[CLS - 1]);
                 }
+#pragma unroll
+                for (int cls = 0; cls < CLS; ++cls) write_finished(sums[cls], part + cls * pitch + k0 + 32 * u);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -870,9 +880,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     int k0 = 0;
     for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
     for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
-    if (want && k_end > 0 && h == 0)            // what the last tile has begun, and the one place that none has
+    if (want && k_end > 0 && h == 0)            // what the last tile has begun
 #pragma unroll
-        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + (l < 31 ? 30 - l : 31)] = l < 31 ? carry[cls] : 0.f;
+        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + 31 - l] = sums[cls];
     if (i >= a.Lq) return;
     T* out = static_cast<T*>(a.dq) + (((long)b * a.Lq + i) * a.H + head) * D;
 #pragma unroll

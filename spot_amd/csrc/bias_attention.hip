@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void spread_kernel(const Args a) {
 }
 
 // Sums of dS along each offset over sequences and queries.  A wave of the dQ kernel has left its sums for keys
-// - queries = delta at delta + p0 + 31, where p0 is the position of its first query: at most 32 terms each, in 32 bits;
+// - queries = delta at delta + p0 + 32, where p0 is the position of its first query: at most 32 terms each, in 32 bits;
 // from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 4, ... and of
 // each the blocks z / 4, ...
 __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double*
         const Seq s = sequence(a, b);
         // where this offset lies in the first wave's sums; a wave further it is 32 further.  Places outside of a wave's
         // sums are read at their border and not added: loads without a branch overlap.
-        const int at = delta + s.off + 31;
+        const int at = delta + s.off + 32;
         const float* part = a.part + (((long)b * a.H + head) * nw * ncls + cls) * pitch;
 #pragma unroll 8
         for (int w = z >> 2; w < nw; w += 4) {
