@@ -685,10 +685,12 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
 // The forward's split.  The table's gradient is the sum of dS along each offset key - query: a wave takes the keys of its
 // dS tiles one after the other, the sums so far move up by one lane, and the key's row is added in lanes 0 .. 31.  So a
 // sum meets every query of the wave, and what has left them is finished: after 32 keys lanes 32 .. 63 hold 32 finished
-// sums, which are written.  A row is brought into the lower lanes, zeros above it, by one exchange of the wave's halves for
+// sums.  A row is brought into the lower lanes, zeros above it, by one exchange of the wave's halves for
 // two rows; moving and adding are one instruction.  On a map an offset stands for two different column offsets, inside a
 // row and around its end: two sets of sums.
-__device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 32; }
+// The same 32 offsets leave the four waves, whose queries are 32 apart, one 32-key tile after the other: they meet in a
+// ring of eight blocks per wave in LDS and are written together, at most 128 terms in 32 bits.
+__device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 128; }
 // x's lower half in both lanes' places: [low, 0] and [high, 0]
 __device__ __forceinline__ void halves(float x, float& low, float& high) {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), 0u, false, false);
@@ -717,12 +719,27 @@ __device__ __forceinline__ float move_on(float t) {
     const auto y = __builtin_amdgcn_permlane32_swap(0u, __float_as_uint(t), false, false);
     return __uint_as_float(y[0]);
 }
-__device__ __forceinline__ void write_finished(float t, float* out) {
-    const int l = threadIdx.x & 63;
-    if (l >= 32) out[63 - l] = t;
-}
+struct Ring {
+    float block[8][4][32];
+    // after 32-key tile n: lanes 32 .. 63 of wave w
+    __device__ __forceinline__ void put(int n, int w, float t) {
+        const int l = threadIdx.x & 63;
+        if (l >= 32) block[(n - w) & 7][w][63 - l] = t;
+    }
+    // blocks n and n + 1, by one wave, if the waves are through tile `done`
+    __device__ __forceinline__ void write(int n, int done, float* out) const {
+        const int l = threadIdx.x & 63, at = n + (l >> 5);
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float y = block[at & 7][w][l & 31];
+            x += at + w >= 0 && at + w <= done ? y : 0.f;       // else no tile of this wave has been there
+        }
+        out[(n + 3) * 32 + l] = x;
+    }
+};
 
-template <class T, int D, bool MAP>
+template <class T, int D, bool MAP, bool SUMS>      // SUMS: the table's gradient is wanted
 __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Args a) {
     typedef Tile<T, D, BN> KT;
     constexpr int CLS = MAP ? 2 : 1;
@@ -730,6 +747,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     __shared__ __attribute__((aligned(16))) T sv[KT::ELEMS];
     __shared__ float sb[WindowLds<MAP>::N];
     __shared__ __attribute__((aligned(16))) int su[BN], sx[BN];
+    __shared__ Ring ring[CLS];
     const int nq = (a.Lq + BM - 1) / BM;
     int unit, rest;
     place(a.B * a.Hkv, a.G * nq, a.causal, unit, rest);
@@ -744,9 +762,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
     const T* kb = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h;
     const T* vb = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h;
     const float* bias = a.bias + (long)head * a.pitch + a.front + a.ncells / 2 - u_hi;       // of offset u(key) from here on
-    const bool want = a.part != nullptr;
     const int pitch = sum_pitch(a.Lk);
-    float* part = want ? a.part + ((((long)b * a.H + head) * nq + qblk) * 4 + w) * CLS * pitch : nullptr;
+    float* part = SUMS ? a.part + (((long)b * a.H + head) * nq + qblk) * CLS * pitch : nullptr;
 
     typename Vec<T>::v8 qf[D / 16], gf[D / 16];
     // rows behind the last query have probability 0 (and the biases of the last: an entry that no pair has may hold anything)
@@ -799,11 +816,11 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             if (decltype(masked)::value && !__any(last >= k0 + 32 * u)) {      // none of this wave's queries sees a key
-                if (want)
+                if (SUMS)
 #pragma unroll
                     for (int cls = 0; cls < CLS; ++cls) {
                         sums[cls] = move_on(sums[cls]);
-                        write_finished(sums[cls], part + cls * pitch + k0 + 32 * u);
+                        ring[cls].put(k0 / 32 + u, w, sums[cls]);
                     }
                 continue;
             }
@@ -826,7 +843,10 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
                     dp[4 * g + e] = __builtin_amdgcn_exp2f(x) * fmaf(dp[4 * g + e], inv, -delta_inv);
                 }
             }
-            if (want) {
+            // a border for the scheduler: with the sums mixed into the exponentials f32 heads of 32 take longer (40 x 8 x 1024:
+            // 723 against 703 us), 16-bit heads of 64 without sums too (8 x 16 x 2048: 304 against 288)
+            if (SUMS || sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+            if (SUMS) {
                 const int kx = MAP ? __builtin_amdgcn_readfirstlane(sx[32 * u]) : 0;
                 if (!MAP) {
                     sums[0] = offset_sums(dp, sums[0]);
@@ -852,7 +872,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
                     sums[CLS - 1] = offset_sums(around, sums[CLS - 1]);
                 }
 #pragma unroll
-                for (int cls = 0; cls < CLS; ++cls) write_finished(sums[cls], part + cls * pitch + k0 + 32 * u);
+                for (int cls = 0; cls < CLS; ++cls) ring[cls].put(k0 / 32 + u, w, sums[cls]);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -874,15 +894,26 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
         }
         __syncthreads();
         if (k0 + BN < k_end) load(k0 + BN);
+        // of the tile before; what its waves put there is overwritten from the next tile on
+        if (SUMS && k0 > 0)
+#pragma unroll
+            for (int cls = 0; cls < CLS; ++cls)
+                if (w == ((k0 / BN + 2 * cls) & 3)) ring[cls].write(k0 / 32 - 5, k0 / 32 - 1, part + cls * pitch);
         step(k0, live, masked);
     };
     if (k_end > 0) load(0);
     int k0 = 0;
     for (; k0 < open; k0 += BN) tile(k0, Flag<false>());
     for (; k0 < k_end; k0 += BN) tile(k0, Flag<true>());
-    if (want && k_end > 0 && h == 0)            // what the last tile has begun
+    if (SUMS && k_end > 0) {                    // what the last tile has finished and begun
+        const int n = (k_end + BN - 1) / BN * 2;
 #pragma unroll
-        for (int cls = 0; cls < CLS; ++cls) part[cls * pitch + (k_end + BN - 1) / BN * BN + 31 - l] = sums[cls];
+        for (int cls = 0; cls < CLS; ++cls) ring[cls].put(n, w, move_on(sums[cls]));
+        __syncthreads();
+        if (w < 3)
+#pragma unroll
+            for (int cls = 0; cls < CLS; ++cls) ring[cls].write(n - 5 + 2 * w, n, part + cls * pitch);
+    }
     if (i >= a.Lq) return;
     T* out = static_cast<T*>(a.dq) + (((long)b * a.Lq + i) * a.H + head) * D;
 #pragma unroll
@@ -1080,7 +1111,8 @@ template <class T, int D, bool MAP> void launch_one(int what, const Args& a, uns
     if (what == FWD) fwd_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
     else if (what == FEW) few_kernel<T, D, MAP><<<grid, 64 * FewLds<T, D>::NW, 0, stream>>>(a);
     else if (what == MERGE) merge_kernel<T, D><<<grid, 256, 0, stream>>>(a);
-    else if (what == DQ) dq_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
+    else if (what == DQ && a.part) dq_kernel<T, D, MAP, true><<<grid, 256, 0, stream>>>(a);
+    else if (what == DQ) dq_kernel<T, D, MAP, false><<<grid, 256, 0, stream>>>(a);
     else dkv_kernel<T, D, MAP><<<grid, 256, 0, stream>>>(a);
 }
 template <class T> int launch(int what, int D, const Args& a, unsigned grid, hipStream_t stream) {

@@ -16,27 +16,28 @@ __global__ __launch_bounds__(256) void spread_kernel(const Args a) {
     if (i < a.pitch) a.bias[(long)blockIdx.y * a.pitch + i] = bias_at(a, i - a.front, blockIdx.y);
 }
 
-// Sums of dS along each offset over sequences and queries.  A wave of the dQ kernel has left its sums for keys
-// - queries = delta at delta + p0 + 32, where p0 is the position of its first query: at most 32 terms each, in 32 bits;
-// from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 4, ... and of
-// each the blocks z / 4, ...
+// Sums of dS along each offset over sequences and queries.  A workgroup of the dQ kernel has left its sums for keys
+// - queries = delta at delta + p0 + 128, where p0 is the position of its first query: at most 128 terms each, in 32 bits;
+// from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 4, ... and of each the
+// blocks z / 4, ...
 __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
     __shared__ double red[16][64];
-    const int l = threadIdx.x & 63, z = threadIdx.x >> 6, head = blockIdx.y, cls = blockIdx.z, ncls = gridDim.z;
-    const int i = blockIdx.x * 64 + l, delta = i - (a.N - 1);
-    const int nw = (a.Lq + BM - 1) / BM * 4, pitch = sum_pitch(a.Lk);
+    const int l = threadIdx.x & 63, z = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int head = blockIdx.y, cls = blockIdx.z, ncls = gridDim.z;
+    const int i0 = blockIdx.x * 64, i = i0 + l, delta = i - (a.N - 1);
+    const int nq = (a.Lq + BM - 1) / BM, pitch = sum_pitch(a.Lk);
     double sum = 0.;
     const long step = (long)ncls * pitch;
     for (int b = z & 3; b < a.B; b += 4) {
         const Seq s = sequence(a, b);
-        // where this offset lies in the first wave's sums; a wave further it is 32 further.  Places outside of a wave's
-        // sums are read at their border and not added: loads without a branch overlap.
-        const int at = delta + s.off + 32;
-        const float* part = a.part + (((long)b * a.H + head) * nw * ncls + cls) * pitch;
-#pragma unroll 8
-        for (int w = z >> 2; w < nw; w += 4) {
-            const int end = key_end(a, s, w / 4 * BM), len = end > 0 ? (end + BN - 1) / BN * BN + 32 : 0, x = at + 32 * w;
-            const float v = part[w * step + min(max(x, 0), pitch - 1)];
+        // where the workgroup's first offset lies in the first block's sums; a block further it is 128 further.  Places
+        // outside of a block's sums are read at their border and not added: loads without a branch overlap.
+        const int at = i0 - (a.N - 1) + s.off + 128;
+        const float* part = a.part + (((long)b * a.H + head) * nq * ncls + cls) * pitch;
+#pragma unroll 4
+        for (int q = z >> 2; q < nq; q += 4) {
+            const int end = key_end(a, s, q * BM), len = end > 0 ? (end + BN - 1) / BN * BN + 128 : 0, x = at + BM * q + l;
+            const float v = (part + q * step)[(unsigned)min(max(x, 0), max(len - 1, 0))];
             sum += (unsigned)x < (unsigned)len ? v : 0.f;
         }
     }
@@ -104,13 +105,13 @@ static int pitch_of(const spot_bias_attn_desc& d) {
 }
 struct Layout { long sums, delta, bias, part, total; };
 static Layout layout(const spot_bias_attn_desc& d) {
-    const long cls = d.width > 0 ? 2 : 1, nw = (d.Lq + BM - 1) / BM * 4, pitch = ((long)d.Lk + BN - 1) / BN * BN + 32;
+    const long cls = d.width > 0 ? 2 : 1, nq = (d.Lq + BM - 1) / BM, pitch = ((long)d.Lk + BN - 1) / BN * BN + 128;
     Layout l;
     l.sums = 0;
     l.delta = d.dtable ? up16(8 * (long)d.H * cells_of(d)) : 0;
     l.bias = l.delta + up16(4L * d.B * d.H * d.Lq);
     l.part = l.bias + 4L * d.H * pitch_of(d);
-    l.total = l.part + (d.dtable ? 4 * (long)d.B * d.H * nw * cls * pitch : 0);
+    l.total = l.part + (d.dtable ? 4 * (long)d.B * d.H * nq * cls * pitch : 0);
     return l;
 }
 
