@@ -18,8 +18,8 @@ __global__ __launch_bounds__(256) void spread_kernel(const Args a) {
 
 // Sums of dS along each offset over sequences and queries.  A workgroup of the dQ kernel has left its sums for keys
 // - queries = delta at delta + p0 + 128, where p0 is the position of its first query: at most 128 terms each, in 32 bits;
-// from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 4, ... and of each the
-// blocks z / 4, ...
+// from here on the sums are 64 bits.  16 waves per 64 offsets: wave z takes the sequences z % 8, ... and of each the
+// blocks z / 8, ...
 __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double* __restrict__ sums) {
     __shared__ double red[16][64];
     const int l = threadIdx.x & 63, z = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -28,14 +28,14 @@ __global__ __launch_bounds__(1024) void offset_sums_kernel(const Args a, double*
     const int nq = (a.Lq + BM - 1) / BM, pitch = sum_pitch(a.Lk);
     double sum = 0.;
     const long step = (long)ncls * pitch;
-    for (int b = z & 3; b < a.B; b += 4) {
+    for (int b = z & 7; b < a.B; b += 8) {
         const Seq s = sequence(a, b);
         // where the workgroup's first offset lies in the first block's sums; a block further it is 128 further.  Places
         // outside of a block's sums are read at their border and not added: loads without a branch overlap.
         const int at = i0 - (a.N - 1) + s.off + 128;
         const float* part = a.part + (((long)b * a.H + head) * nq * ncls + cls) * pitch;
 #pragma unroll 4
-        for (int q = z >> 2; q < nq; q += 4) {
+        for (int q = z >> 3; q < nq; q += 2) {
             const int end = key_end(a, s, q * BM), len = end > 0 ? (end + BN - 1) / BN * BN + 128 : 0, x = at + BM * q + l;
             const float v = (part + q * step)[(unsigned)min(max(x, 0), max(len - 1, 0))];
             sum += (unsigned)x < (unsigned)len ? v : 0.f;
