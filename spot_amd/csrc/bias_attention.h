@@ -53,8 +53,8 @@ enum { FWD, FEW, MERGE, DQ, DKV };          // kernels
 // Waves per SIMD that the registers are cut for: as many as fit without spilling.
 template <class T, int D> constexpr int waves_of(int kernel) {
     const int words = D * (int)sizeof(T) / 64;      // 1, 2, 4 for 16-bit heads of 32, 64, 128 channels; twice that in f32
-    return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 1 ? 3 : words <= 4 ? 2 : 1)
-                                                 : (D == 32 ? 3 : words <= 2 ? 2 : 1);
+    return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 2 ? 3 : words <= 4 ? 2 : 1)
+                                                 : (D == 32 ? 3 : words <= 4 ? 2 : 1);
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -928,7 +928,7 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 }
 
 // --- dK, dV ---------------------------------------------------------------------------------------------------------
-// One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers; the queries of all
+// One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers or LDS; the queries of all
 // heads that share it stream through LDS 64 or 128 at a time, half for each wave of a pair, so the sums over those heads stay in
 // the accumulators (no atomics, one order) and the pair joins at the end.  Keys sit on the lanes (S = Q K^T), P and dS
 // (garbage for padding, whose sums are dropped) are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
@@ -938,6 +938,10 @@ template <class T, int D> struct DkvLds {
     typedef Tile<T, D, QB> QT;
     static constexpr int TILES = 2 * QT::ELEMS * (int)sizeof(T), JOIN = 2 * 64 * 16 * 4;
     static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
+    // K and V stay in registers or, where two waves per SIMD are to share these, in LDS (8 x 16 heads of 128 channels x 1024
+    // in bf16: 393 us in registers with one wave, 252 in LDS with two; 64 channels, where both have two: bf16
+    // 361 and 354, f32 300 and 292)
+    static constexpr bool HELD = waves_of<T, D>(DKV) != 2;
 };
 template <class T, int D, bool MAP>
 __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const Args a) {
@@ -949,6 +953,8 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     __shared__ __attribute__((aligned(16))) int sl[QB], su[QB];
     T* sq = reinterpret_cast<T*>(lds);
     T* sg = sq + QT::ELEMS;
+    constexpr bool HELD = DkvLds<T, D>::HELD;
+    __shared__ __attribute__((aligned(16))) T skv[HELD ? 8 : 2 * KB * QT::P];
     const int nk = (a.Lk + KB - 1) / KB;
     int unit, rest;
     place(a.B * a.Hkv, nk, a.causal, unit, rest);
@@ -960,13 +966,18 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
     const int u_lo = coord<MAP>(a, k0), lane_u = coord<MAP>(a, key) - u_lo;
 
     typename Vec<T>::v8 kf[D / 16], vf[D / 16];
-    {
+    const T* kl = skv + (32 * (w & 1) + col) * QT::P + 8 * h;
+    if (HELD || w < 2) {
         const T* kr = static_cast<const T*>(a.k) + b * a.k_b + kvh * a.k_h + (long)key * a.k_l;
         const T* vr = static_cast<const T*>(a.v) + b * a.v_b + kvh * a.v_h + (long)key * a.v_l;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
             kf[c] = frag_or_zero(kr + 16 * c + 8 * h, alive);
             vf[c] = frag_or_zero(vr + 16 * c + 8 * h, alive);
+            if (!HELD) {
+                *reinterpret_cast<typename Vec<T>::v8*>(const_cast<T*>(kl) + 16 * c) = kf[c];
+                *reinterpret_cast<typename Vec<T>::v8*>(const_cast<T*>(kl) + KB * QT::P + 16 * c) = vf[c];
+            }
         }
     }
     f32x16 dk[D / 32], dv[D / 32];
@@ -1019,9 +1030,12 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DKV))) void dkv_kernel(const A
         f32x16 sc = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-            mma(frag<T>(sq + (32 * u + col) * QT::P + 16 * c + 8 * h), kf[c], sc);
-            mma(frag<T>(sg + (32 * u + col) * QT::P + 16 * c + 8 * h), vf[c], dp);
+            mma(frag<T>(sq + (32 * u + col) * QT::P + 16 * c + 8 * h), HELD ? kf[c] : frag<T>(kl + 16 * c), sc);
+            mma(frag<T>(sg + (32 * u + col) * QT::P + 16 * c + 8 * h), HELD ? vf[c] : frag<T>(kl + KB * QT::P + 16 * c), dp);
         }
+        // a border for the scheduler where three waves share a SIMD in 16 bits (40 x 8 heads of 32 x 1024 bf16: 218 us
+        // without it, 182 with it; of 64 x 2048 356 and 362)
+        if (sizeof(T) == 2 && D == 32) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int r = 32 * u + 8 * g + 4 * h;
