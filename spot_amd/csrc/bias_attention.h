@@ -17,6 +17,13 @@
 // that u(key) - u(query) stands for one offset in either; `bias` is the table spread out by that difference, per head
 // and times log2 e.  A tile of queries x keys meets a window of it, which goes to LDS with the tile.
 //
+// What bounds them.  f32: the issue of v_mfma_f32_32x32x2_f32 and vector instructions, which share the SIMD's issue slots
+// (measured 86 to 93 % of them; forward 40 x 8 heads of 32 x 1024 400 us, 107 TFLOP/s, dQ 640, 101, dK/dV 760, 113; a
+// library's product of large f32 matrices reaches 153).  16 bits: the vector unit - a 32x32 tile of scores costs 16
+// exponentials and some 100 other vector instructions per wave, beside 4 to 16 matrix instructions of 32 cycles - and LDS, from
+// where each matrix instruction takes an operand (forward 8 x 16 heads of 64 x 2048 bf16 205 us, 670 TFLOP/s, dQ 290, 710,
+// dK/dV 355, 775; forward 8 x 8191 x 8191 of 128 f16 335, 820; a library's product reaches 1146 to 1193).
+//
 // Statistics.  A row's reference (its maximum or less) and reciprocal sum are kept apart: as one number (their
 // log-sum-exp) a row of scores near the type's lowest value would lose the sum.  A row that sees no key has reference 0
 // and reciprocal 0: its output and gradients are zero.
@@ -50,7 +57,8 @@ struct Args {               // strides in elements; out, d_out, dq, dk, dv are d
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 enum { FWD, FEW, MERGE, DQ, DKV };          // kernels
 
-// Waves per SIMD that the registers are cut for: as many as fit without spilling.
+// Waves per SIMD that the registers are cut for: as many as fit with no more than a few words spilled outside of the loops
+// (f32 heads of 32, 40 x 8 x 1024: dQ with two waves 698 us, with three 674).
 template <class T, int D> constexpr int waves_of(int kernel) {
     const int words = D * (int)sizeof(T) / 64;      // 1, 2, 4 for 16-bit heads of 32, 64, 128 channels; twice that in f32
     return kernel == FWD ? (words <= 2 ? 3 : words <= 4 ? 2 : 1) : kernel == DQ ? (words <= 2 ? 3 : words <= 4 ? 2 : 1)
@@ -433,11 +441,15 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(FWD))) void fwd_kernel(const A
 
 // --- forward for few rows -------------------------------------------------------------------------------------------
 // A tile is 32 rows: `heads` query heads of one key/value head for `queries` queries each, so that every key and value
-// is read once for all of them (one new token: its heads).  A workgroup's waves (eight; four from 128 channels on, in f32 from 64) take 32-key tiles in turn and join
-// at the end; where the tiles are few the keys are cut in `splits` ranges, one workgroup each, joined by merge_kernel.
+// is read once for all of them (one new token: its heads).  A workgroup's waves (eight; four for heads of more than 128
+// bytes) take 32-key tiles in turn and join at the end; where the tiles are few the keys are cut in `splits` ranges, one
+// workgroup each, joined by merge_kernel.
 // Keys go from memory to operand registers (a lane's row), values through the wave's own LDS; the next tile is in flight
 // while this one is worked on.  No barrier until the end.  The biases come from memory (first-level cache): spread out
 // if there are many tiles, else (a.bias NULL) by bucket, which saves the launch that spreads them.
+// Long caches are bound by reading them (a new token of 32 sequences over up to 16384 keys, 8 key/value heads of 128 in
+// bf16, 1.9 GB: 361 us, 5.2 TB/s, which is a large copy's rate), short calls by the latency of what follows one another
+// - cells, table, scores, the waves' join (8 heads of 64 over 257 keys f16 9.6 us, 8 of 32 on a 16 x 16 map f32 11.3).
 constexpr int FT = 32;      // keys per tile
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -689,7 +701,9 @@ template <class T, int D> __global__ __launch_bounds__(256) void merge_kernel(co
 // two rows; moving and adding are one instruction.  On a map an offset stands for two different column offsets, inside a
 // row and around its end: two sets of sums.
 // The same 32 offsets leave the four waves, whose queries are 32 apart, one 32-key tile after the other: they meet in a
-// ring of eight blocks per wave in LDS and are written together, at most 128 terms in 32 bits.
+// ring of eight blocks per wave in LDS and are written together, at most 128 terms in 32 bits.  All of this costs some 70
+// vector instructions per tile and wave, a third of the kernel in 16 bits (8 x 16 heads of 64 x 2048 bf16: 395 us with the
+// sums and their reduction, 290 without; through LDS, row by row, it was 440).
 __device__ __forceinline__ int sum_pitch(int Lk) { return (Lk + BN - 1) / BN * BN + 128; }
 // x's lower half in both lanes' places: [low, 0] and [high, 0]
 __device__ __forceinline__ void halves(float x, float& low, float& high) {
@@ -931,7 +945,9 @@ __global__ __launch_bounds__(256, (waves_of<T, D>(DQ))) void dq_kernel(const Arg
 // One workgroup: 64 keys of one key/value head, 32 per pair of waves, their K and V held in registers or LDS; the queries of all
 // heads that share it stream through LDS 64 or 128 at a time, half for each wave of a pair, so the sums over those heads stay in
 // the accumulators (no atomics, one order) and the pair joins at the end.  Keys sit on the lanes (S = Q K^T), P and dS
-// (garbage for padding, whose sums are dropped) are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// (garbage for padding, whose sums are dropped) are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.  S and dP
+// are computed a second time here: dQ from this kernel would need sums over workgroups, by atomics in no fixed order or
+// through memory.
 template <class T, int D> struct DkvLds {
     // queries per LDS tile: 128 where the registers hold the next tile (8 x 16 heads of 64 x 2048 bf16: 513 -> 450 us against 64)
     static constexpr int QB = sizeof(T) == 2 && D <= 64 ? 128 : 64;

@@ -1,7 +1,10 @@
 // The k largest entries of a row with their places, and the distillation loss of a student row against them.
 //
 // Both are bound by reading the rows once (the loss's gradient: reading and writing them once): N * V elements against
-// 5 to 10 lane operations each, which is under the vector rate at the card's copy bandwidth.
+// 5 to 10 lane operations each, which is under the vector rate at the card's copy bandwidth.  Measured: the 64 largest of
+// 4096 x 32000 bf16 59 us, 4.5 TB/s; loss of 4096 x 50257 bf16 78 us, 5.3 TB/s, its gradient 165 us, 5.0 TB/s (a large
+// copy: 5.2).  Few or short rows are bound by latency: 16 of 32 x 1024 f32 6.3 us; 8 of 3 x 100003 f16 6.2 and, for the join of
+// the pieces, 5 us; loss of 5 x 131073 f16 4 and 4 us, gradient 11, which is the stores and then the listed places.
 #include <float.h>
 
 #include <algorithm>
