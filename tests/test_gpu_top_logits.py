@@ -301,3 +301,22 @@ def test_student_learns_positions_from_a_teachers_top_places(ops):
     assert abs(loss.item() - l64.item()) < 1e-4
     for a, b in zip(grads, torch.autograd.grad(l64, deep)):
         assert (a.double() - b).norm() <= 1e-4 * b.norm()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V,k", [(129, 128), (300, 30), (449, 100), (500, 128), (505, 96), (1000, 128), (1023, 127), (1027, 1), (1100, 128)])
+def test_top_logits_of_rows_with_fewer_loads_than_k(ops, t, V, k):
+    """The list holds the whole row, or most of it."""
+    T = TYPES[t]
+    g = torch.Generator(device=DEV).manual_seed(V + k)
+    x = torch.randn(9, V, generator=g, device=DEV)
+    x[1] = (x[1] * 2).round()                               # few values
+    x[2, : V // 2] = x[2, 0]                                # half of the row is one value
+    x[3] = -x[3].abs()
+    x[4, k - 1:] = -math.inf
+    x[5] = torch.where(x[5] > 0, math.inf, x[5])
+    x[6] = x[6] * 1e-6 + 1                                  # next to each other
+    x[7] = 0
+    x[8] = x[8].sort().values
+    check_top(ops, x.to(T), k)
+    check_top(ops, x.to(T)[:, 1:], min(k, V - 1))           # rows that begin between two loads
