@@ -55,8 +55,9 @@ template <class T> __device__ __forceinline__ int order_key(T x) {
 //      element's rank is how many of the list stand before it (greater, or equal at a lower place), and the first k are
 //      written at their rank.  Where k threads have no load the list is the row, and is cut by a bound of its own first
 //      (128 of 4096 x 1000 f16: 843 us without that, 78 with it).
-//   4. Only if a list overflows (many equal values) or the piece holds a NaN, the k-th value is found by bisection over
-//      the order of all elements, and among its equals the last place by bisection over the places.
+//   4. Only if a list overflows or stays long (many equal values), or the piece holds a NaN, the k-th value is searched
+//      among all elements from the bound on, and of its equals the first are taken in the order of their places (4096 x
+//      32000 bf16, k 64: 158 us for rows of one value, 198 for f16 rows of three).
 // Rows too long for one workgroup, or too few to fill the card, are cut in pieces; a second launch of the same kernel
 // takes the pieces' candidates, whose order is that of the places among equals.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -174,37 +175,8 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ x, long l
     }
     __syncthreads();
     int count = s_count;
-    if (s_nan || hits > HITS || count > LIST) {
-        // the largest key that k elements reach
-        auto reach = [&](long key) {
-            int c = 0;
-            for (int e = tid; e < n; e += NT) c += order_key(xr[e]) >= key;
-            return block_sum(c, red);
-        };
-        long low = -0x80000000L, high = 0x80000000L;    // reach(low) >= k > reach(high)
-        while (high - low > 1) {
-            const long mid = (low + high) >> 1;
-            if (reach(mid) >= k) low = mid; else high = mid;
-        }
-        const int kth = (int)low, left = k - reach(high);       // how many of those equal to the k-th are taken
-        int first = -1, last = n - 1;                   // of them, up to `last` at least `left`, up to `first` fewer
-        while (last - first > 1) {
-            const int mid = (first + last) >> 1;
-            int c = 0;
-            for (int e = tid; e <= mid; e += NT) c += order_key(xr[e]) == kth;
-            if (block_sum(c, red) >= left) last = mid; else first = mid;
-        }
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        for (int e = tid; e < n; e += NT) {
-            const int key = order_key(xr[e]);
-            if (key > kth || (key == kth && e <= last)) s_list[atomicAdd(&s_count, 1)] = make_int2(key, e);     // k of them
-        }
-        __syncthreads();
-        count = s_count;
-    }
-    if (count > 2 * k + NT / 4) {
+    const bool over = s_nan || hits > HITS || count > LIST;
+    if (!over && count > 2 * k + NT / 4) {
         // rows of few loads, whose maxima are too few to give a bound: it is taken from the list, all of it in each wave
         int key[LIST / 64];
 #pragma unroll
@@ -232,6 +204,81 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ x, long l
             if (own[i].x >= (int)low && NT * i + tid < count) s_list[atomicAdd(&s_count, 1)] = own[i];
         __syncthreads();
         count = s_count;
+    }
+    if (over || count > 2 * k + NT / 4) {
+        // bits of a key that the type does not use: the others tell its values apart
+        constexpr int S = sizeof(T) == 4 ? 0 : __is_same(T, _Float16) ? 13 : 16;
+        auto each = [&](int at, auto f) {               // the elements of a load from place `at` on
+            if (at + VE <= n) {
+                const typename Vec16<T>::any v = *reinterpret_cast<const typename Vec16<T>::any*>(xr + at);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) f(order_key((T)v[e]), e);
+            } else {
+                for (int e = 0; at + e < n; ++e) f(order_key(xr[at + e]), e);
+            }
+        };
+        auto reach = [&](long key) {
+            int c = 0;
+            for (int at = tid * VE; at < n; at += NT * VE) each(at, [&](int x, int) { c += (x >> S) >= key; });
+            return block_sum(c, red);
+        };
+        // the largest key that k elements reach: from the least of the maxima that reach the bound on in growing steps, then
+        // by bisection.  Many equals: it is that one.  probe stays between low and high, so the search ends.
+        constexpr long HALVES = 1L << 40;
+        const int m4[4] = {mine.x, mine.y, mine.z, mine.w};
+        int least = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) least = m4[i] >= bound ? min(least, m4[i]) : least;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) least = min(least, __shfl_xor(least, o));
+        long low = least >> S, high = (0x7fffffff >> S) + 1L, probe = s_nan ? high - 1 : low + 1, ahead = 1;
+        int above = 0;                                  // elements that reach high: less than k
+        while (high - low > 1) {
+            const int c = reach(probe);
+            if (c >= k) {
+                low = probe;
+                ahead = min(2 * ahead, HALVES);
+            } else {
+                high = probe;
+                above = c;
+                if (!s_nan || probe != 0x7fffffff >> S) ahead = HALVES;
+            }
+            probe = min(low + ahead, (low + high) >> 1);
+        }
+        const int kth = (int)low, left = k - above;     // of those equal to the k-th the first `left` are taken
+        __syncthreads();
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        int before = 0;
+        for (int base = 0; base < n; base += NT * VE) {
+            const int at = base + tid * VE;
+            unsigned equal = 0;
+            int key = 0;
+            each(at, [&](int x, int e) {
+                if ((x >> S) > kth) s_list[atomicAdd(&s_count, 1)] = make_int2(x, at + e);
+                if ((x >> S) == kth) {
+                    equal |= 1u << e;
+                    key = x;
+                }
+            });
+            if (before >= left) continue;
+            int rank = __popc(equal);
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(rank, o);
+                if ((tid & 63) >= o) rank += y;
+            }
+            __syncthreads();
+            if ((tid & 63) == 63) red[tid >> 6] = rank;
+            __syncthreads();
+            rank += before - __popc(equal);
+            for (int w = 0; w < tid >> 6; ++w) rank += red[w];
+            for (; equal && rank < left; equal &= equal - 1, ++rank)
+                s_list[atomicAdd(&s_count, 1)] = make_int2(key, at + __ffs(equal) - 1);
+            before += red[0] + red[1] + red[2] + red[3];
+        }
+        __syncthreads();
+        count = s_count;                                // k
     }
     const long out = (long)blockIdx.x * k;
     for (int c = tid; c < count; c += NT) {

@@ -320,3 +320,23 @@ def test_top_logits_of_rows_with_fewer_loads_than_k(ops, t, V, k):
     x[8] = x[8].sort().values
     check_top(ops, x.to(T), k)
     check_top(ops, x.to(T)[:, 1:], min(k, V - 1))           # rows that begin between two loads
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V,k", [(2500, 100), (9001, 64), (33000, 128)])
+def test_top_logits_of_few_values(ops, t, V, k):
+    """The list is too long or stays so: the k-th value is searched, on either side of zero and beside NaN and infinities."""
+    T = TYPES[t]
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randint(0, 30, (10, V), generator=g, device=DEV).double()
+    x[1] = -x[1] - 1
+    x[2] = x[2] - 15
+    x[3] = x[3] * 2.0 ** -20 + 1
+    x[4] = torch.where(x[4] > 27, math.inf, -x[4])
+    x[5] = torch.where(x[5] > 0, -math.inf, -3.0)
+    x[6, 3:: V // (k // 2)] = math.nan                       # fewer than k
+    x[7, ::5] = math.nan                                     # more
+    x[8] = torch.where(x[8] == 7, -1.0, -2.0)
+    x[8, torch.randint(0, V, (k - 1,), generator=g, device=DEV)] = 5.0       # up to k - 1 above many equals
+    x[9] = -x[9] * 2.0 ** -24
+    check_top(ops, x.to(T), k)
