@@ -2214,7 +2214,8 @@ def bias_attention(q, k, v, table, buckets, causal=False, q_offset=0, kv_len=Non
 
     Scores, probabilities, sums and the table's gradient are 32 bits or more; products of 16-bit inputs take
     probabilities and score gradients rounded to that type.  Deterministic.  Capturable into a graph: the tensors
-    kv_len and q_offset are read when it is replayed.  Not twice differentiable."""
+    kv_len and q_offset are read when it is replayed; a backward pass is captured, as with any function, for leaves that no
+    living eager graph holds (detach them first).  Not twice differentiable."""
     _check_bias_attention(q, k, v, table, buckets, q_offset, kv_len, key_padding_mask)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return BiasAttentionFn.apply(q, k, v, table, buckets, causal, q_offset, kv_len, key_padding_mask, scale)
