@@ -607,8 +607,8 @@ extern "C" int spot_top_distill_ws_bytes(int dtype, int N, int V, int k, long* b
 }
 
 extern "C" int spot_top_distill_fwd(int dtype, const void* student, long ld, int values_dtype, const void* values,
-                                    const int* indices, int N, int V, int k, float temperature, float* loss, float* norm, float* p, void* ws, long ws_bytes,
-                                    hipStream_t stream) {
+                                    const int* indices, int N, int V, int k, float temperature, float* loss, float* norm, float* p,
+                                    void* ws, long ws_bytes, hipStream_t stream) {
     if (const int rc = check_rows("spot_top_distill_fwd", dtype, N, V, k, ld)) return rc;
     SPOT_CHECK_ARG(values_dtype >= F32 && values_dtype <= F16, "spot_top_distill_fwd: values_dtype %d is none of 0 (f32), 1 (bf16), 2 (f16)",
                    values_dtype);
